@@ -10,6 +10,7 @@
 #include <string>
 #include <vector>
 
+#include "ctx.cuh"
 #include "mrl_internal.cuh"
 
 // Scan scratch for mrl_scan_device_static, placed in the module's own global memory so that entry
@@ -38,61 +39,6 @@ const unsigned int kDoneInit[kScratchSets] = {
     0xFFFFFFF0u, 0xFFFFFFF1u, 0xFFFFFFF2u, 0xFFFFFFF3u, 0xFFFFFFF4u, 0xFFFFFFF5u, 0xFFFFFFF6u, 0xFFFFFFF7u,
     0xFFFFFFF8u, 0xFFFFFFF9u, 0xFFFFFFFAu, 0xFFFFFFFBu, 0xFFFFFFFCu, 0xFFFFFFFDu, 0xFFFFFFFEu, 0xFFFFFFFFu};
 }  // namespace
-
-struct mrl_ctx {
-    int device = 0;
-    int sms = 0;
-    cudaStream_t own_stream = nullptr;
-    cudaStream_t stream = nullptr;
-    std::string err;
-    // scan scratch, kScratchSets sets used by consecutive scan launches in turn: launches on the
-    // stream may overlap (programmatic dependent launch), and a launch touches its set only once the
-    // launch that used it before has released it. Per set: per-CTA lists, control words, per-page
-    // owner (grow-only; each set owns an equal share of `owner`).
-    unsigned long long* cta_keys = nullptr;  // per set 2 * sms * 32: scan keys, then their exact keys
-    unsigned int* ctl = nullptr;             // per set mrl::kCtlWords
-    uint8_t* owner = nullptr;
-    size_t owner_bytes = 0;
-    uint32_t scan_seq = 0;      // launches so far; launch s uses scratch set s % kScratchSets
-    uint32_t scan_ctas = 0;     // CTAs per single-query scan launch (0: one per SM)
-    unsigned int* done = nullptr;  // per set: sequence number of the last launch that released it
-    uint32_t list_len_override = 0;
-    // grow-only scratch for host-facing calls: inputs (queries, rows, means) and outputs
-    void* tmp = nullptr;
-    size_t tmp_bytes = 0;
-    void* tmp_out = nullptr;
-    size_t tmp_out_bytes = 0;
-    // device copy of the last codec centres uploaded (64 prefix + 128 mid floats) and its host
-    // twin, so repeated plan builds against one EdenFit issue no host->device copy
-    float* d_means = nullptr;
-    float h_means[192];
-    bool means_valid = false;
-    // grow-only scratch of the exact paths (scores, flag)
-    void* xbuf = nullptr;
-    size_t xbuf_bytes = 0;
-    // two merge records (scan, ring) of mrl_engine_scan
-    void* ebuf = nullptr;
-    size_t ebuf_bytes = 0;
-    // per-(query, CTA) top lists and tensor-core operand tiles of the batched scan
-    void* bbuf = nullptr;
-    size_t bbuf_bytes = 0;
-    uint32_t batch_engine = MRL_BATCH_TENSOR;
-    // pinned host staging of mrl_query_scan, mapped into the device's address space: the query is
-    // copied to the device from here, and the scan kernel stores its results straight into it
-    // (no device-to-host copies on the query path)
-    void* h_io = nullptr;
-    void* h_io_dev = nullptr;
-    size_t h_io_bytes = 0;
-    // pipelined host queries (mrl_query_submit / mrl_query_collect): MRL_MAX_INFLIGHT result slots
-    // in pinned, device-mapped memory, laid out for shortlists up to slot_k; the scan stores each
-    // query's top-k there and then the slot's completion word, on which the host waits
-    unsigned char* h_slots = nullptr;
-    unsigned char* d_slots = nullptr;
-    size_t slot_stride = 0;
-    uint32_t slot_k = 0;
-    uint32_t slot_seq[MRL_MAX_INFLIGHT] = {};
-    bool slot_busy[MRL_MAX_INFLIGHT] = {};
-};
 
 // RingBuffer's pending embeddings (src/ring.rs:49-119) mirrored in HBM: `len` rows of `dims` f32
 // in push order.
@@ -136,26 +82,6 @@ struct mrl_exchange {
 
 namespace {
 
-int fail(mrl_ctx* ctx, int code, const std::string& msg) {
-    if (ctx) ctx->err = msg;
-    return code;
-}
-
-int cuda_fail(mrl_ctx* ctx, cudaError_t e, const char* what) {
-    return fail(ctx, MRL_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
-}
-
-#define MRL_CUDA_TRY(ctx, expr)                                   \
-    do {                                                          \
-        cudaError_t _e = (expr);                                  \
-        if (_e != cudaSuccess) return cuda_fail((ctx), _e, #expr); \
-    } while (0)
-
-int set_device(mrl_ctx* ctx) {
-    const cudaError_t e = cudaSetDevice(ctx->device);
-    return e == cudaSuccess ? MRL_OK : cuda_fail(ctx, e, "cudaSetDevice");
-}
-
 // Device address of g_static_scan_scratch on ctx's device (which must be current), looked up on
 // the first call per device and cached. The lookup may load this module onto the device, so the
 // first mrl_scan_device_static call on a device should come before any stream capture begins.
@@ -176,16 +102,6 @@ int static_scratch(mrl_ctx* ctx, unsigned char** out) {
     return MRL_OK;
 }
 
-int ensure_buf(mrl_ctx* ctx, void** buf, size_t* have, size_t bytes) {
-    if (*have >= bytes) return MRL_OK;
-    if (*buf) cudaFree(*buf);  // synchronises the device: no launch still reads the old buffer
-    *buf = nullptr;
-    *have = 0;
-    const cudaError_t e = cudaMalloc(buf, bytes);
-    if (e != cudaSuccess) return fail(ctx, MRL_ERR_NOMEM, std::string("cudaMalloc scratch: ") + cudaGetErrorString(e));
-    *have = bytes;
-    return MRL_OK;
-}
 int ensure_tmp(mrl_ctx* ctx, size_t bytes) { return ensure_buf(ctx, &ctx->tmp, &ctx->tmp_bytes, bytes); }
 int ensure_host_io(mrl_ctx* ctx, size_t bytes) {
     if (ctx->h_io_bytes >= bytes) return MRL_OK;
@@ -438,6 +354,8 @@ void mrl_ctx_destroy(mrl_ctx* ctx) {
     cudaFree(ctx->xbuf);
     cudaFree(ctx->ebuf);
     cudaFree(ctx->bbuf);
+    for (mrl_kv_scratch& k : ctx->kv) cudaFree(k.buf);
+    if (ctx->join_event) cudaEventDestroy(ctx->join_event);
     if (ctx->h_io) cudaFreeHost(ctx->h_io);
     if (ctx->h_slots) cudaFreeHost(ctx->h_slots);
     if (ctx->own_stream) cudaStreamDestroy(ctx->own_stream);

@@ -1,0 +1,237 @@
+// kv_capi.cu — C ABI of the paged cache and the attention operators (include/mrl_kv.h): argument checks,
+// scratch and launches. Every entry point catches its own failures, as in capi.cu.
+#include <cstdio>
+#include <exception>
+
+#include "ctx.cuh"
+#include "kv.cuh"
+
+namespace {
+
+template <class F> int guarded(mrl_ctx* ctx, F f) {
+    if (!ctx) return MRL_ERR_INVALID;
+    try {
+        if (int rc = set_device(ctx)) return rc;
+        return f();
+    } catch (const std::exception&) {  // std::bad_alloc of a message
+        return MRL_ERR_NOMEM;
+    }
+}
+
+int bad(mrl_ctx* ctx, const char* msg) { return fail(ctx, MRL_ERR_INVALID, msg); }
+int done(mrl_ctx* ctx, int cuda, const char* what) {
+    return cuda == 0 ? MRL_OK : cuda_fail(ctx, (cudaError_t)cuda, what);
+}
+
+bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int check_cache(mrl_ctx* ctx, const mrl_kv_cache* c) {
+    if (!c) return bad(ctx, "kv is NULL");
+    if (!c->codes || !c->scales || !c->tables || !c->lens || !c->refs || !c->status) return bad(ctx, "kv has a NULL buffer");
+    if (!aligned(c->codes)) return bad(ctx, "kv codes must be 16-byte aligned");
+    if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return bad(ctx, "head_dim must be 64, 128 or 256");
+    if (c->layers < 1 || c->layers > 4096) return bad(ctx, "layers must be in [1, 4096]");
+    if (c->kv_heads < 1 || c->kv_heads > 1024) return bad(ctx, "kv_heads must be in [1, 1024]");
+    if (c->pages < 1 || c->pages > (1u << 24)) return bad(ctx, "pages must be in [1, 2^24]");
+    if (c->max_pages < 1 || c->max_pages > (1u << 20)) return bad(ctx, "max_pages must be in [1, 2^20]");
+    if (c->max_seqs < 1 || c->max_seqs > (1u << 24)) return bad(ctx, "max_seqs must be in [1, 2^24]");
+    return MRL_OK;
+}
+
+constexpr uint32_t kMaxSeqs = 65535, kMaxTokens = 1u << 28;
+
+int check_rows(mrl_ctx* ctx, const int32_t* seqs, bool need_seqs, const int32_t* cu, uint32_t n_seqs, uint32_t n_tokens) {
+    if (n_seqs > kMaxSeqs) return bad(ctx, "n_seqs must be at most 65535");
+    if (n_tokens > kMaxTokens) return bad(ctx, "n_tokens must be at most 2^28");
+    if (n_seqs && need_seqs && !seqs) return bad(ctx, "seqs is NULL");
+    if (!cu && n_tokens != n_seqs) return bad(ctx, "without cu there is one row per sequence: n_tokens must equal n_seqs");
+    return MRL_OK;
+}
+
+// A [rows][heads][dims] operand of 16-bit elements: 16-byte aligned pointer and strides.
+int check_rows16(mrl_ctx* ctx, const char* name, const void* p, int64_t row, int64_t head) {
+    if (!p) return fail(ctx, MRL_ERR_INVALID, std::string(name) + " is NULL");
+    if (!aligned(p) || row % 8 || head % 8)
+        return fail(ctx, MRL_ERR_INVALID, std::string(name) + " and its row and head strides must be multiples of 16 bytes");
+    if (row < 0 || head < 0) return fail(ctx, MRL_ERR_INVALID, std::string(name) + " strides must not be negative");
+    return MRL_OK;
+}
+
+// The scratch buffer of the context's current stream: counters in the first kCounterBytes (zero when a
+// buffer is made, and left zero by the kernels that use them), then at least `bytes` for the call.
+constexpr size_t kCounterBytes = 65536;
+int kv_scratch(mrl_ctx* ctx, size_t bytes, void** out, unsigned** counters = nullptr) {
+    bytes += kCounterBytes;
+    mrl_kv_scratch* k = nullptr;
+    for (mrl_kv_scratch& x : ctx->kv)
+        if (x.used && x.stream == ctx->stream) k = &x;
+    if (!k) {
+        k = &ctx->kv[ctx->kv_next];
+        if (k->used) MRL_CUDA_TRY(ctx, cudaDeviceSynchronize());  // its old stream may still use the buffer
+        ctx->kv_next = (ctx->kv_next + 1) % mrl_ctx::kKvStreams;
+        k->stream = ctx->stream;
+        k->used = true;
+    }
+    if (k->bytes < bytes) {
+        size_t want = (bytes + (size_t)0xfffff) & ~(size_t)0xfffff;
+        if (int rc = ensure_buf(ctx, &k->buf, &k->bytes, want)) return rc;
+        MRL_CUDA_TRY(ctx, cudaMemsetAsync(k->buf, 0, k->bytes, ctx->stream));
+    }
+    *out = static_cast<char*>(k->buf) + kCounterBytes;
+    if (counters) *counters = static_cast<unsigned*>(k->buf);
+    return MRL_OK;
+}
+
+int check_attn(mrl_ctx* ctx, const mrl_attn* a, uint32_t kv_heads, uint32_t head_dim, bool paged) {
+    if (a->dtype != MRL_F16 && a->dtype != MRL_BF16) return bad(ctx, "dtype must be MRL_F16 or MRL_BF16");
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256) return bad(ctx, "head_dim must be 64, 128 or 256");
+    if (kv_heads < 1 || kv_heads > 1024) return bad(ctx, "kv_heads must be in [1, 1024]");
+    if (a->q_heads < kv_heads || a->q_heads % kv_heads || a->q_heads / kv_heads > 64)
+        return bad(ctx, "q_heads must be kv_heads times a whole number, at most 64");
+    if (!(a->scale > 0.0f) || !(a->scale < INFINITY)) return bad(ctx, "scale must be positive and finite");
+    if (a->window > 0x7fffffffu || a->sinks > 0x7fffffffu) return bad(ctx, "window and sinks must be below 2^31");
+    if (int rc = check_rows(ctx, a->seqs, paged, a->cu, a->n_seqs, a->n_tokens)) return rc;
+    if (!paged && !a->cu) return bad(ctx, "cu is NULL");
+    if (a->n_tokens == 0) return MRL_OK;
+    if (a->n_seqs == 0) return bad(ctx, "there are rows but no sequences");
+    if (a->max_rows == 0) return bad(ctx, "max_rows must be at least the rows of every sequence");
+    if (int rc = check_rows16(ctx, "q", a->q, a->q_row, a->q_head)) return rc;
+    if (int rc = check_rows16(ctx, "out", a->out, a->o_row, a->o_head)) return rc;
+    if (paged) return MRL_OK;
+    if (int rc = check_rows16(ctx, "k", a->k, a->k_row, a->k_head)) return rc;
+    return check_rows16(ctx, "v", a->v, a->v_row, a->v_head);
+}
+
+}  // namespace
+
+extern "C" {
+
+int mrl_kv_reserve(mrl_ctx* ctx, const mrl_kv_cache* kv, const int32_t* d_seqs, const int32_t* d_add, uint32_t n) {
+    return guarded(ctx, [&]() -> int {
+        if (int rc = check_cache(ctx, kv)) return rc;
+        if (n > kMaxSeqs) return bad(ctx, "n must be at most 65535");
+        if (n == 0) return MRL_OK;
+        if (!d_seqs || !d_add) return bad(ctx, "seqs or add is NULL");
+        void* scratch;
+        if (int rc = kv_scratch(ctx, mrl::kv_list_bytes(*kv, n), &scratch)) return rc;
+        return done(ctx, mrl::launch_kv_reserve(*kv, d_seqs, d_add, n, scratch, ctx->stream), "mrl_kv_reserve");
+    });
+}
+
+int mrl_kv_fork(mrl_ctx* ctx, const mrl_kv_cache* kv, const int32_t* d_parents, const int32_t* d_children, uint32_t n) {
+    return guarded(ctx, [&]() -> int {
+        if (int rc = check_cache(ctx, kv)) return rc;
+        if (n > kMaxSeqs) return bad(ctx, "n must be at most 65535");
+        if (n == 0) return MRL_OK;
+        if (!d_parents || !d_children) return bad(ctx, "parents or children is NULL");
+        void* scratch;
+        if (int rc = kv_scratch(ctx, mrl::kv_list_bytes(*kv, n), &scratch)) return rc;
+        return done(ctx, mrl::launch_kv_fork(*kv, d_parents, d_children, n, ctx->sms, scratch, ctx->stream), "mrl_kv_fork");
+    });
+}
+
+int mrl_kv_release(mrl_ctx* ctx, const mrl_kv_cache* kv, const int32_t* d_seqs, uint32_t n) {
+    return guarded(ctx, [&]() -> int {
+        if (int rc = check_cache(ctx, kv)) return rc;
+        if (n > kMaxSeqs) return bad(ctx, "n must be at most 65535");
+        if (n == 0) return MRL_OK;
+        if (!d_seqs) return bad(ctx, "seqs is NULL");
+        return done(ctx, mrl::launch_kv_release(*kv, d_seqs, n, 0, 0, 0, ctx->stream), "mrl_kv_release");
+    });
+}
+
+int mrl_kv_trim(mrl_ctx* ctx, const mrl_kv_cache* kv, const int32_t* d_seqs, uint32_t n, uint32_t window, uint32_t sinks) {
+    return guarded(ctx, [&]() -> int {
+        if (int rc = check_cache(ctx, kv)) return rc;
+        if (window < 1 || window > 0x7fffffffu || sinks > 0x7fffffffu) return bad(ctx, "window must be in [1, 2^31) and sinks below 2^31");
+        if (n > kMaxSeqs) return bad(ctx, "n must be at most 65535");
+        if (n == 0) return MRL_OK;
+        if (!d_seqs) return bad(ctx, "seqs is NULL");
+        return done(ctx, mrl::launch_kv_release(*kv, d_seqs, n, 1, window, sinks, ctx->stream), "mrl_kv_trim");
+    });
+}
+
+int mrl_kv_compact(mrl_ctx* ctx, const mrl_kv_cache* kv) {
+    return guarded(ctx, [&]() -> int {
+        if (int rc = check_cache(ctx, kv)) return rc;
+        void* scratch;
+        if (int rc = kv_scratch(ctx, mrl::kv_list_bytes(*kv, 0), &scratch)) return rc;
+        return done(ctx, mrl::launch_kv_compact(*kv, ctx->sms, scratch, ctx->stream), "mrl_kv_compact");
+    });
+}
+
+int mrl_kv_copy_pages(mrl_ctx* ctx, const mrl_kv_cache* kv, const int32_t* d_src, const int32_t* d_dst, uint32_t n) {
+    return guarded(ctx, [&]() -> int {
+        if (int rc = check_cache(ctx, kv)) return rc;
+        if (n > kv->pages) return bad(ctx, "n must be at most the cache's pages");
+        if (n == 0) return MRL_OK;
+        if (!d_src || !d_dst) return bad(ctx, "src or dst is NULL");
+        return done(ctx, mrl::launch_kv_copy_pages(*kv, d_src, d_dst, n, ctx->sms, ctx->stream), "mrl_kv_copy_pages");
+    });
+}
+
+int mrl_kv_append(mrl_ctx* ctx, const mrl_kv_cache* kv, uint32_t layer, uint32_t dtype, const void* k, int64_t k_row,
+                  int64_t k_head, const void* v, int64_t v_row, int64_t v_head, const int32_t* d_seqs,
+                  const int32_t* d_cu, uint32_t n_seqs, uint32_t n_tokens) {
+    return guarded(ctx, [&]() -> int {
+        if (int rc = check_cache(ctx, kv)) return rc;
+        if (layer >= kv->layers) return bad(ctx, "layer is not one of the cache's");
+        if (dtype != MRL_F16 && dtype != MRL_BF16) return bad(ctx, "dtype must be MRL_F16 or MRL_BF16");
+        if (int rc = check_rows(ctx, d_seqs, true, d_cu, n_seqs, n_tokens)) return rc;
+        if (n_tokens == 0) return MRL_OK;
+        if (n_seqs == 0) return bad(ctx, "there are rows but no sequences");
+        if (int rc = check_rows16(ctx, "k", k, k_row, k_head)) return rc;
+        if (int rc = check_rows16(ctx, "v", v, v_row, v_head)) return rc;
+        const mrl::kv::Rows r{d_seqs, d_cu, (int)n_seqs, (int)n_tokens};
+        return done(ctx, mrl::launch_kv_append(*kv, layer, dtype, k, k_row, k_head, v, v_row, v_head, r, ctx->stream), "mrl_kv_append");
+    });
+}
+
+int mrl_kv_read(mrl_ctx* ctx, const mrl_kv_cache* kv, uint32_t layer, uint32_t dtype, void* k, void* v,
+                const int32_t* d_seqs, const int32_t* d_cu, uint32_t n_seqs, uint32_t n_tokens) {
+    return guarded(ctx, [&]() -> int {
+        if (int rc = check_cache(ctx, kv)) return rc;
+        if (layer >= kv->layers) return bad(ctx, "layer is not one of the cache's");
+        if (dtype > MRL_F32) return bad(ctx, "dtype must be MRL_F16, MRL_BF16 or MRL_F32");
+        if (int rc = check_rows(ctx, d_seqs, true, d_cu, n_seqs, n_tokens)) return rc;
+        if (n_tokens == 0) return MRL_OK;
+        if (n_seqs == 0) return bad(ctx, "there are rows but no sequences");
+        if (!k || !v) return bad(ctx, "k or v is NULL");
+        if (!aligned(k) || !aligned(v)) return bad(ctx, "k and v must be 16-byte aligned");
+        const mrl::kv::Rows r{d_seqs, d_cu, (int)n_seqs, (int)n_tokens};
+        return done(ctx, mrl::launch_kv_read(*kv, layer, dtype, k, v, r, ctx->stream), "mrl_kv_read");
+    });
+}
+
+int mrl_kv_attend(mrl_ctx* ctx, const mrl_kv_cache* kv, const mrl_attn* a) {
+    return guarded(ctx, [&]() -> int {
+        if (int rc = check_cache(ctx, kv)) return rc;
+        if (!a) return bad(ctx, "args are NULL");
+        if (a->layer >= kv->layers) return bad(ctx, "layer is not one of the cache's");
+        if (int rc = check_attn(ctx, a, kv->kv_heads, kv->head_dim, true)) return rc;
+        if (a->n_tokens == 0) return MRL_OK;
+        return done(ctx, mrl::launch_attend_simple(kv, *a, ctx->stream), "mrl_kv_attend");
+    });
+}
+
+int mrl_window_attention(mrl_ctx* ctx, const mrl_attn* a) {
+    return guarded(ctx, [&]() -> int {
+        if (!a) return bad(ctx, "args are NULL");
+        if (int rc = check_attn(ctx, a, a->kv_heads, a->head_dim, false)) return rc;
+        if (a->n_tokens == 0) return MRL_OK;
+        return done(ctx, mrl::launch_attend_simple(nullptr, *a, ctx->stream), "mrl_window_attention");
+    });
+}
+
+int mrl_ctx_join(mrl_ctx* ctx, void* stream, int to_ctx) {
+    return guarded(ctx, [&]() -> int {
+        cudaStream_t other = static_cast<cudaStream_t>(stream);
+        if (other == ctx->stream) return MRL_OK;
+        if (!ctx->join_event) MRL_CUDA_TRY(ctx, cudaEventCreateWithFlags(&ctx->join_event, cudaEventDisableTiming));
+        MRL_CUDA_TRY(ctx, cudaEventRecord(ctx->join_event, to_ctx ? other : ctx->stream));
+        MRL_CUDA_TRY(ctx, cudaStreamWaitEvent(to_ctx ? ctx->stream : other, ctx->join_event, 0));
+        return MRL_OK;
+    });
+}
+
+}  // extern "C"

@@ -37,6 +37,7 @@ from .api import (  # noqa: F401
     score_bound,
     control_words,
 )
+from .attention import KvCache, window_attention  # noqa: F401
 from .index import (  # noqa: F401
     DeviceRing,
     IndexDir,

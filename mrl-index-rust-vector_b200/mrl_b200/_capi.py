@@ -63,11 +63,28 @@ class ScanCfgC(C.Structure):
     ]
 
 
-# Every exported symbol of include/mrl_cuda.h with its ctypes signature.
+class KvCacheC(C.Structure):
+    """struct mrl_kv_cache of include/mrl_kv.h."""
+
+    _fields_ = [(n, C.c_void_p) for n in ("codes", "scales", "tables", "lens", "refs", "status")] + [
+        (n, C.c_uint32) for n in ("layers", "pages", "kv_heads", "head_dim", "max_seqs", "max_pages")]
+
+
+class AttnC(C.Structure):
+    """struct mrl_attn of include/mrl_kv.h."""
+
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "out", "lse", "seqs", "cu")] + [
+        (n, C.c_int64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head", "o_row", "o_head")] + [
+        (n, C.c_uint32) for n in ("n_seqs", "n_tokens", "max_rows", "q_heads", "kv_heads", "head_dim", "dtype", "causal",
+                                  "window", "sinks")] + [("scale", C.c_float), ("layer", C.c_uint32)]
+
+
+# Every exported symbol of include/mrl_cuda.h and include/mrl_kv.h with its ctypes signature.
 _vp = C.c_void_p
 _u32 = C.c_uint32
 _u64 = C.c_uint64
 _i = C.c_int
+_i64 = C.c_int64
 SIGNATURES = {
     "mrl_ctx_create": (_i, [_i, C.POINTER(_vp)]),
     "mrl_ctx_destroy": (None, [_vp]),
@@ -133,6 +150,17 @@ SIGNATURES = {
     "mrl_set_list_len": (_i, [_vp, _u32]),
     "mrl_set_scan_ctas": (_i, [_vp, _u32]),
     "mrl_set_batch_engine": (_i, [_vp, _u32]),
+    "mrl_kv_reserve": (_i, [_vp, _vp, _vp, _vp, _u32]),
+    "mrl_kv_fork": (_i, [_vp, _vp, _vp, _vp, _u32]),
+    "mrl_kv_release": (_i, [_vp, _vp, _vp, _u32]),
+    "mrl_kv_trim": (_i, [_vp, _vp, _vp, _u32, _u32, _u32]),
+    "mrl_kv_compact": (_i, [_vp, _vp]),
+    "mrl_kv_copy_pages": (_i, [_vp, _vp, _vp, _vp, _u32]),
+    "mrl_kv_append": (_i, [_vp, _vp, _u32, _u32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _u32, _u32]),
+    "mrl_kv_read": (_i, [_vp, _vp, _u32, _u32, _vp, _vp, _vp, _vp, _u32, _u32]),
+    "mrl_kv_attend": (_i, [_vp, _vp, _vp]),
+    "mrl_window_attention": (_i, [_vp, _vp]),
+    "mrl_ctx_join": (_i, [_vp, _vp, _i]),
 }
 
 _lib = None

@@ -210,6 +210,7 @@ class Device:
         if rc != 0:
             raise MrlError(rc, f"cannot create a context on CUDA device {index} (needs an sm_100 GPU)")
         self.index = index
+        self.torch_stream = None  # the stream set by set_stream (None: the context's own)
 
     def close(self) -> None:
         if self.ptr:
@@ -228,6 +229,16 @@ class Device:
 
     def set_stream(self, stream: int) -> None:
         check(self.ptr, self.lib.mrl_ctx_set_stream(self.ptr, C.c_void_p(stream)))
+        self.torch_stream = int(stream) or None
+
+    def use_torch_stream(self) -> None:
+        """Launch on torch's current stream of this device from now on. The attention operators (KvCache,
+        window_attention) are right on any stream; on torch's own they need no events to be ordered with
+        the tensors they are given."""
+        import torch
+
+        # cudaStreamLegacy (1) names the default stream, whose handle 0 means the context's own here
+        self.set_stream(torch.cuda.current_stream(self.index).cuda_stream or 1)
 
     def geometry(self, k: int):
         ctas, ll = C.c_uint32(), C.c_uint32()
