@@ -34,6 +34,7 @@ extern "C" {
 #define MRL_KV_BAD_INDEX 4u  /* a sequence, page or count out of range, or a fork onto a sequence that
                                 is not empty or onto its own parent; the operation did nothing */
 #define MRL_KV_NONFINITE 8u  /* an append met an Inf (stored as the largest code) or a NaN (stored as 0) */
+#define MRL_KV_TIMEOUT 16u   /* a kernel gave up waiting for its own loads; the call's outputs mean nothing */
 
 /* A cache of `layers` layers over one page table. Page p of a layer holds 64 consecutive tokens of a
  * sequence for all heads; K and V of each head have one f32 scale per page: value = code * scale.

@@ -133,5 +133,9 @@ int launch_kv_copy_pages(const mrl_kv_cache& c, const int32_t* src, const int32_
 int launch_kv_append(const mrl_kv_cache& c, uint32_t layer, uint32_t dtype, const void* k, int64_t k_row, int64_t k_head,
                      const void* v, int64_t v_row, int64_t v_head, const kv::Rows& r, cudaStream_t s);
 int launch_kv_read(const mrl_kv_cache& c, uint32_t layer, uint32_t dtype, void* k, void* v, const kv::Rows& r, cudaStream_t s);
+// Decode: scratch for the pieces of split items, and zeroed counters; sequences of one launch
+constexpr uint32_t kKvDecodeSeqs = 1024;
+size_t kv_decode_bytes(uint32_t head_dim, int sms);
+int launch_kv_decode(const mrl_kv_cache& c, const mrl_attn& a, int sms, void* scratch, unsigned* counters, cudaStream_t s);
 int launch_attend_simple(const mrl_kv_cache* c, const mrl_attn& a, cudaStream_t s);
 }  // namespace mrl

@@ -1,6 +1,7 @@
 // kv_capi.cu — C ABI of the paged cache and the attention operators (include/mrl_kv.h): argument checks,
 // scratch and launches. Every entry point catches its own failures, as in capi.cu.
-#include <cstdio>
+#include <algorithm>
+#include <cmath>
 #include <exception>
 
 #include "ctx.cuh"
@@ -210,7 +211,13 @@ int mrl_kv_attend(mrl_ctx* ctx, const mrl_kv_cache* kv, const mrl_attn* a) {
         if (a->layer >= kv->layers) return bad(ctx, "layer is not one of the cache's");
         if (int rc = check_attn(ctx, a, kv->kv_heads, kv->head_dim, true)) return rc;
         if (a->n_tokens == 0) return MRL_OK;
-        return done(ctx, mrl::launch_attend_simple(kv, *a, ctx->stream), "mrl_kv_attend");
+        // units of work of a launch are counted in 32 bits
+        const uint64_t tiles = (uint64_t)a->n_tokens * (a->q_heads / kv->kv_heads) / 16 + std::min(a->n_seqs, mrl::kKvDecodeSeqs);
+        if (tiles * kv->kv_heads * kv->max_pages >= (1ull << 32)) return bad(ctx, "too many rows x pages for one call");
+        void* scratch;
+        unsigned* counters;
+        if (int rc = kv_scratch(ctx, mrl::kv_decode_bytes(kv->head_dim, ctx->sms), &scratch, &counters)) return rc;
+        return done(ctx, mrl::launch_kv_decode(*kv, *a, ctx->sms, scratch, counters, ctx->stream), "mrl_kv_attend");
     });
 }
 

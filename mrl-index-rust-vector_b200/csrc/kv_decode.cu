@@ -1,0 +1,631 @@
+// kv_decode.cu — attention of a few query rows per sequence over the paged 8-bit cache
+// (mrl_kv_attend, include/mrl_kv.h), one launch.
+//
+// An item is 16 query rows (tokens x the query heads of one kv head) of one sequence: their K and V pages
+// are read once and serve all 16. The page is the unit of work: one warp takes a page of 64 tokens,
+// S = Q K^T and O += P V by m16n8k16 products with the codes widened to f16 on the way from shared
+// memory (exact: |code| <= 128), and the page's two scales applied to S and to P, which are f32 there.
+// Softmax statistics are kept per warp in f32, joined over the warps of a team in shared memory, and over
+// teams through global partials that the last team to arrive adds up in team order, so results do not
+// depend on scheduling.
+//
+// The page's layout is the one the products want: a row of 64 bytes has the index that is summed over
+// contiguous, each of 4 lanes takes 16 of them as four k-steps' worth, and 8 lanes cover two rows, so
+// every 16-byte shared-memory load of a warp is free of conflicts and needs no transposition: K's token
+// order in the score tile is chosen so that a lane's scores are 16 consecutive tokens, V's row order.
+//
+// Bound by HBM for long contexts (2 x 64 x head_dim bytes a page), by latency for short ones.
+#include "kv.cuh"
+
+namespace mrl {
+namespace kv {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr uint32_t kPolls = 1u << 22;  // of a wait for a page, each up to the hardware's own time limit
+
+// Warps per CTA: each holds one page's K and V block, 128 KiB in all, enough in flight per SM to cover the
+// latency of HBM.
+template <int D> constexpr int kWarps = 1024 / D;
+template <int D> constexpr int kAccStride = D + 8;  // f32 per row of a joined tile: rows 8 banks apart
+
+struct SeqInfo {
+    unsigned start;  // first unit (or job) of the sequence
+    int len, row, m; // tokens, first row of the call, rows
+};
+
+struct Params {
+    mrl_kv_cache c;
+    mrl_attn a;
+    float* part;         // [slots][16][D] partial outputs, then [slots][16][2] their m (base 2) and l
+    unsigned* counters;  // arrivals per split item, zero between launches
+    int slots;
+    int row0;            // rows of earlier launches of the call (one row per sequence)
+};
+
+// Pages of a sequence that any of its rows sees: [0, head) and [lo, hi).
+struct PageSpan {
+    int head, lo, n;
+};
+__device__ __forceinline__ PageSpan page_span(int len, int m, int window, int sinks) {
+    PageSpan s{0, 0, 0};
+    if (len <= 0 || m <= 0) return s;
+    if (window > 0) {
+        const int lo = max(0, len - m - window + 1);
+        s.lo = min(lo / kPage, pages_of(len));
+        s.head = min(pages_of(min(sinks, lo)), s.lo);
+    }
+    s.n = s.head + pages_of(len) - s.lo;
+    return s;
+}
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void bar_init(uint32_t bar) { asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void load_block(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+                 "r"(bytes), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
+    for (uint32_t i = 0; i < kPolls; ++i) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.b32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (ok) return true;
+    }
+    return false;
+}
+// A team is `threads` threads of consecutive warps; one warp needs no barrier resource.
+__device__ __forceinline__ void team_sync(int team, int threads) {
+    if (threads == 32) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(threads) : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void mma16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Four int8 codes as f16 pairs (0, 1) and (2, 3): the byte with its sign bit flipped (code + 128) becomes
+// the low bits of 1024 + code + 128, and 1152 is taken off again; all steps are exact.
+__device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    w ^= 0x80808080u;
+    const __half2 off = __half2half2(__ushort_as_half(0x6480));  // 1152
+    uint32_t x = __byte_perm(w, 0x64646464u, 0x4140), y = __byte_perm(w, 0x64646464u, 0x4342);
+    __half2 a = __hsub2(*reinterpret_cast<__half2*>(&x), off), b = __hsub2(*reinterpret_cast<__half2*>(&y), off);
+    lo = *reinterpret_cast<uint32_t*>(&a);
+    hi = *reinterpret_cast<uint32_t*>(&b);
+}
+__device__ __forceinline__ uint32_t pack_half(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float quad_max(float x) {
+    x = fmaxf(x, __shfl_xor_sync(~0u, x, 1));
+    return fmaxf(x, __shfl_xor_sync(~0u, x, 2));
+}
+__device__ __forceinline__ float quad_sum(float x) {
+    x += __shfl_xor_sync(~0u, x, 1);
+    return x + __shfl_xor_sync(~0u, x, 2);
+}
+
+// How the launch's pages are dealt out to its teams.
+struct Plan {
+    unsigned units;  // pages of all items
+    unsigned jobs;   // short: pieces of items, each at most one page per warp of a team
+    int teams, width;  // teams of the launch, warps per team
+    bool few;        // short launch: jobs instead of equal shares of the units
+};
+
+// A run of pages [p0, p1) of one item, by one team.
+struct Segment {
+    int b, head, tile;     // sequence of the call, kv head, 16-row tile
+    int p0, p1;
+    int parts, part, first;  // pieces the item is in, this one's number, and the first one's team (or job)
+};
+
+template <class T, int D> __global__ void __launch_bounds__(kWarps<D> * 32, 1) decode_kernel(Params pr) {
+    constexpr int NW = kWarps<D>, kThreads = NW * 32, kBlock = kPage * D;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    unsigned char* ring = smem;                                              // per warp: K block, V block
+    float* acc_s = reinterpret_cast<float*>(ring + (size_t)NW * 2 * kBlock);  // per warp 16 rows of kAccStride
+    float* ml_s = acc_s + NW * 16 * kAccStride<D>;                           // per warp 16 x {m, l}
+    uint64_t* bars = reinterpret_cast<uint64_t*>(ml_s + NW * 32);            // per warp {K, V}
+    SeqInfo* info = reinterpret_cast<SeqInfo*>(bars + NW * 2);               // [n]
+    int* seq_s = reinterpret_cast<int*>(info + pr.a.n_seqs);                 // [n] table row, or -1
+    __shared__ unsigned scan_s[NW][2];
+    __shared__ unsigned arrived_s[NW];
+
+    const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const mrl_kv_cache& c = pr.c;
+    const mrl_attn& a = pr.a;
+    const int n = (int)a.n_seqs, group = (int)(a.q_heads / c.kv_heads);
+    const int window = (int)a.window, sinks = (int)a.sinks;
+    const uint32_t bar_k = smem_addr(&bars[warp * 2]), bar_v = bar_k + 8;
+    if (lane == 0) {
+        bar_init(bar_k);
+        bar_init(bar_v);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+
+    // ---- the call's sequences: their items and pages, summed up
+    const Rows rows{a.seqs, a.cu, n, (int)a.n_tokens};
+    unsigned my_items = 0, my_units = 0;
+    for (int b = tid; b < n; b += kThreads) {
+        SeqInfo s;
+        s.row = a.cu ? rows.begin(b) : pr.row0 + b;
+        s.m = a.cu ? rows.end(b) - s.row : 1;
+        const int seq = a.seqs[b];
+        const bool known = seq >= 0 && seq < (int)c.max_seqs;
+        s.len = known ? min(max(c.lens[seq], 0), (int)c.max_pages * kPage) : 0;
+        seq_s[b] = known ? seq : -1;
+        s.start = 0;
+        info[b] = s;
+        if (s.m > 0) {
+            const unsigned items = (unsigned)((s.m * group + 15) / 16) * c.kv_heads;
+            my_items += items;
+            my_units += items * (unsigned)max(1, page_span(s.len, s.m, window, sinks).n);
+        }
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) {
+        my_items += __shfl_xor_sync(~0u, my_items, d);
+        my_units += __shfl_xor_sync(~0u, my_units, d);
+    }
+    if (lane == 0) {
+        scan_s[warp][0] = my_items;
+        scan_s[warp][1] = my_units;
+    }
+    __syncthreads();
+    unsigned items = 0;
+    Plan pl;
+    pl.units = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+        items += scan_s[w][0];
+        pl.units += scan_s[w][1];
+    }
+    if (pl.units == 0) return;
+    // Warps per team: an item's share of the launch's warps, so that an item is in few pieces, none of
+    // them joined by fewer threads than it has to (few items: whole CTAs; many: each warp on its own).
+    pl.width = NW;
+    while (pl.width > 1 && items * pl.width > gridDim.x * (unsigned)NW) pl.width >>= 1;
+    const int per_cta = NW / pl.width;
+    pl.teams = (int)gridDim.x * per_cta;
+    // With no more than a page per warp an item's pieces are whole jobs, so that short items are not split
+    // at a team's border; beyond that every team takes an equal run of pages.
+    pl.few = pl.units <= (unsigned)(pl.teams * pl.width);
+    __syncthreads();  // scan_s is read
+    // Exclusive sums over the sequences of their units, or of their jobs.
+    unsigned carry = 0;
+    for (int at = 0; at < n; at += kThreads) {
+        const int b = at + tid;
+        unsigned v = 0;
+        if (b < n && info[b].m > 0) {
+            const int np = max(1, page_span(info[b].len, info[b].m, window, sinks).n);
+            v = (unsigned)((info[b].m * group + 15) / 16) * c.kv_heads * (unsigned)(pl.few ? (np + pl.width - 1) / pl.width : np);
+        }
+        unsigned x = v;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const unsigned y = __shfl_up_sync(~0u, x, d);
+            if (lane >= d) x += y;
+        }
+        if (lane == 31) scan_s[warp][0] = x;
+        __syncthreads();
+        unsigned before = carry;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            if (w < warp) before += scan_s[w][0];
+            carry += scan_s[w][0];
+        }
+        if (b < n) info[b].start = before + x - v;
+        __syncthreads();
+    }
+    pl.jobs = carry;
+
+    // ---- this team's run
+    const int team = warp / pl.width, w_in = warp % pl.width, threads = pl.width * 32, t_in = w_in * 32 + lane;
+    const long long t_all = (long long)blockIdx.x + (long long)team * gridDim.x;  // neighbours in work on different SMs
+    long long pos = pl.few ? t_all : (long long)pl.units * t_all / pl.teams;
+    const long long stop = pl.few ? (long long)pl.jobs : (long long)pl.units * (t_all + 1) / pl.teams;
+
+    // The segment at unit (or job) x; *next is where the following one starts.
+    auto segment_at = [&](long long x, long long* next) {
+        Segment s;
+        int lo = 0, hi = n;  // last sequence that starts at or before x: those without work are passed over
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if ((long long)info[mid].start <= x) lo = mid;
+            else hi = mid;
+        }
+        s.b = lo;
+        const SeqInfo q = info[lo];
+        const int np = max(1, page_span(q.len, q.m, window, sinks).n), tiles = (q.m * group + 15) / 16;
+        const unsigned local = (unsigned)(x - q.start);
+        if (pl.few) {
+            const int k = (np + pl.width - 1) / pl.width;
+            const int item = (int)(local / (unsigned)k), piece = (int)(local % (unsigned)k);
+            s.head = item / tiles;
+            s.tile = item % tiles;
+            s.p0 = (int)((long long)piece * np / k);
+            s.p1 = (int)((long long)(piece + 1) * np / k);
+            s.parts = k;
+            s.part = piece;
+            s.first = (int)(x - piece);
+            *next = x + pl.teams;
+        } else {
+            const int item = (int)(local / (unsigned)np);
+            s.p0 = (int)(local % (unsigned)np);
+            const long long begin = x - s.p0, end = begin + np;
+            s.p1 = (int)(min(end, stop) - begin);
+            s.head = item / tiles;
+            s.tile = item % tiles;
+            const long long t0 = ((begin + 1) * pl.teams - 1) / pl.units, t1 = (end * pl.teams - 1) / pl.units;
+            s.parts = (int)(t1 - t0) + 1;
+            s.part = (int)(t_all - t0);
+            s.first = (int)t0;
+            *next = begin + s.p1;
+        }
+        return s;
+    };
+    auto slot_of = [&](const Segment& s, int part) { return pl.few ? s.first + part : (s.first + part) * 2 + (part == 0 ? 1 : 0); };
+    // Page of the pool holding the i-th visible page of a segment's sequence, -1: none; *index its page of
+    // the sequence.
+    auto page_at = [&](const Segment& s, int i, int* index) {
+        const SeqInfo q = info[s.b];
+        const PageSpan sp = page_span(q.len, q.m, window, sinks);
+        *index = i < sp.head ? i : sp.lo + i - sp.head;
+        if (i >= sp.n) return -1;
+        const int page = c.tables[(size_t)seq_s[s.b] * c.max_pages + *index];
+        return page >= 0 && page < (int)c.pages ? page : -1;
+    };
+
+    // ---- the page after the current one: found early, its K and V loaded as their slots come free
+    Segment ns;
+    long long npos = pos;
+    int ni = 0, npage = -1, nindex = 0;
+    float nks = 0.0f, nvs = 0.0f;
+    uint32_t parity = 0;
+    bool fine = true;  // no wait has run out
+    auto advance = [&](bool start) {
+        if (!start) ni += pl.width;
+        while (start || ni >= ns.p1) {
+            start = false;
+            if (npos >= stop) {
+                npage = -1;
+                return;
+            }
+            ns = segment_at(npos, &npos);
+            ni = ns.p0 + w_in;
+        }
+        npage = page_at(ns, ni, &nindex);
+    };
+    auto fetch = [&](int which) {
+        if (npage < 0 || !fine) return;
+        const size_t block = block_index(c, a.layer, npage, which, ns.head);
+        if (which == 0) {
+            nks = c.scales[block];
+            nvs = c.scales[block + c.kv_heads];
+        }
+        if (lane == 0)
+            load_block(smem_addr(ring + (size_t)(warp * 2 + which) * kBlock), c.codes + block * (size_t)kBlock, kBlock, which ? bar_v : bar_k);
+    };
+    advance(true);
+    fetch(0);
+    fetch(1);
+
+    const int g = lane >> 2, t = lane & 3;
+    const unsigned char* kb = ring + (size_t)(warp * 2) * kBlock;
+    const unsigned char* vb = kb + kBlock;
+    while (pos < stop) {
+        const Segment s = segment_at(pos, &pos);
+        const SeqInfo q = info[s.b];
+        // Rows of this lane: r, token of the sequence r / group, query head r % group.
+        const int r0 = s.tile * 16 + g, r1 = r0 + 8, rows_all = q.m * group;
+        const int first = q.len - q.m;
+        const Span v0 = visible(first + r0 / group, q.len, 1, window, sinks), v1 = visible(first + r1 / group, q.len, 1, window, sinks);
+        const int low_pos = first + s.tile * 16 / group, high_pos = first + min(rows_all - 1, s.tile * 16 + 15) / group;
+        uint32_t qf[D / 16][4];
+        float c0 = a.scale * kLog2e, c1 = c0;
+        {
+            const T* base = static_cast<const T*>(a.q);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int r = h ? r1 : r0;
+                const bool in = r < rows_all;
+                const T* p = base + (int64_t)(q.row + r / group) * a.q_row + (int64_t)(s.head * group + r % group) * a.q_head + 16 * t;
+                uint4 raw[D / 32];
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i)
+                    raw[i] = in ? *reinterpret_cast<const uint4*>(p + (i >> 1) * 64 + (i & 1) * 8) : make_uint4(0, 0, 0, 0);
+                const T* e = reinterpret_cast<const T*>(raw);
+                float down = 1.0f;
+                if (sizeof(T) == 2 && !__is_same(T, __half)) {
+                    // bf16 has more range than f16: the row is brought to [1, 2) by a power of two, which is put
+                    // back with the softmax scale. What leaves f16's range below is 2^-24 of the row's largest.
+                    float top = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < D / 4; ++i) top = fmaxf(top, fabsf(to_f32<T>(e[i])));
+                    top = quad_max(top);
+                    const uint32_t ex = __float_as_uint(top) >> 23;  // biased exponent
+                    if (ex > 0 && ex < 255) {
+                        const uint32_t up = min(ex, 253u);
+                        down = __uint_as_float((254u - up) << 23);
+                        (h ? c1 : c0) *= __uint_as_float(up << 23);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {  // k-step i: block i / 4, word i % 4 of the lane's 16 dims
+                    const T* x = e + (i >> 2) * 16 + (i & 3) * 4;
+                    qf[i][h] = pack_half(to_f32<T>(x[0]) * down, to_f32<T>(x[1]) * down);
+                    qf[i][2 + h] = pack_half(to_f32<T>(x[2]) * down, to_f32<T>(x[3]) * down);
+                }
+            }
+        }
+        float o[D / 8][4];
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f, vref = 0.0f;
+
+        for (int i = s.p0 + w_in; i < s.p1; i += pl.width) {
+            const int page = npage, index = nindex;
+            const float ks = nks, vs = nvs;
+            advance(false);
+            if (page < 0) {  // nothing of it was loaded
+                fetch(0);
+                fetch(1);
+                continue;
+            }
+            fine = fine && bar_wait(bar_k, parity);
+            float sc[8][4];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.0f;
+            if (fine) {
+#pragma unroll
+                for (int db = 0; db < D / 64; ++db) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(kb + db * 4096 + (16 * (g >> 1) + 2 * j + (g & 1)) * 64 + 16 * t);
+                        uint32_t b0, b1;
+                        widen4(w.x, b0, b1);
+                        mma16816(sc[j], qf[db * 4 + 0], b0, b1);
+                        widen4(w.y, b0, b1);
+                        mma16816(sc[j], qf[db * 4 + 1], b0, b1);
+                        widen4(w.z, b0, b1);
+                        mma16816(sc[j], qf[db * 4 + 2], b0, b1);
+                        widen4(w.w, b0, b1);
+                        mma16816(sc[j], qf[db * 4 + 3], b0, b1);
+                    }
+                }
+            }
+            __syncwarp();
+            fetch(0);
+            const float f0 = c0 * ks, f1 = c1 * ks;
+            const int key0 = index * kPage;
+            float n0 = m0, n1 = m1;
+            // Token 16 t + 2 j + e of the page is column e of score tile j here.
+            if (key0 + kPage - 1 <= low_pos && (window == 0 || key0 > high_pos - window || key0 + kPage <= sinks)) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    sc[j][0] *= f0;
+                    sc[j][1] *= f0;
+                    sc[j][2] *= f1;
+                    sc[j][3] *= f1;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int key = key0 + 16 * t + 2 * j + e;
+                        sc[j][e] = key < v0.head || (key >= v0.lo && key < v0.hi) ? sc[j][e] * f0 : -INFINITY;
+                        sc[j][2 + e] = key < v1.head || (key >= v1.lo && key < v1.hi) ? sc[j][2 + e] * f1 : -INFINITY;
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                n0 = fmaxf(n0, fmaxf(sc[j][0], sc[j][1]));
+                n1 = fmaxf(n1, fmaxf(sc[j][2], sc[j][3]));
+            }
+            n0 = quad_max(n0);
+            n1 = quad_max(n1);
+            // P carries V's scale relative to the largest one so far, and O is in units of that.
+            const float up = fmaxf(vref, vs), vf = up > 0.0f ? vs / up : 0.0f;
+            if (__any_sync(~0u, n0 != m0 || n1 != m1) || up != vref) {
+                const float unit = up > 0.0f ? vref / up : 0.0f;
+                const float k0 = m0 == -INFINITY ? 0.0f : ex2(m0 - n0), k1 = m1 == -INFINITY ? 0.0f : ex2(m1 - n1);
+                l0 *= k0;
+                l1 *= k1;
+                const float a0 = k0 * unit, a1 = k1 * unit;
+#pragma unroll
+                for (int x = 0; x < D / 8; ++x) {
+                    o[x][0] *= a0;
+                    o[x][1] *= a0;
+                    o[x][2] *= a1;
+                    o[x][3] *= a1;
+                }
+                m0 = n0;
+                m1 = n1;
+                vref = up;
+            }
+            const float z0 = m0 == -INFINITY ? 0.0f : m0, z1 = m1 == -INFINITY ? 0.0f : m1;
+            uint32_t pf[4][4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    float* w = sc[2 * x + y];
+                    w[0] = ex2(w[0] - z0);
+                    w[1] = ex2(w[1] - z0);
+                    w[2] = ex2(w[2] - z1);
+                    w[3] = ex2(w[3] - z1);
+                    l0 += w[0] + w[1];
+                    l1 += w[2] + w[3];
+                    pf[x][2 * y] = pack_half(w[0] * vf, w[1] * vf);
+                    pf[x][2 * y + 1] = pack_half(w[2] * vf, w[3] * vf);
+                }
+            }
+            fine = fine && bar_wait(bar_v, parity);
+            parity ^= 1;
+            if (fine) {
+#pragma unroll
+                for (int x = 0; x < D / 8; ++x) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(vb + (8 * x + g) * 64 + 16 * t);
+                    uint32_t b0, b1;
+                    widen4(w.x, b0, b1);
+                    mma16816(o[x], pf[0], b0, b1);
+                    widen4(w.y, b0, b1);
+                    mma16816(o[x], pf[1], b0, b1);
+                    widen4(w.z, b0, b1);
+                    mma16816(o[x], pf[2], b0, b1);
+                    widen4(w.w, b0, b1);
+                    mma16816(o[x], pf[3], b0, b1);
+                }
+            }
+            __syncwarp();
+            fetch(1);
+        }
+        l0 = quad_sum(l0);
+        l1 = quad_sum(l1);
+
+        // ---- the team's warps joined: O in real units, then rescaled to the rows' common maximum
+        float* mine = acc_s + warp * 16 * kAccStride<D>;
+#pragma unroll
+        for (int x = 0; x < D / 8; ++x) {
+            *reinterpret_cast<float2*>(mine + g * kAccStride<D> + 8 * x + 2 * t) = make_float2(o[x][0] * vref, o[x][1] * vref);
+            *reinterpret_cast<float2*>(mine + (g + 8) * kAccStride<D> + 8 * x + 2 * t) = make_float2(o[x][2] * vref, o[x][3] * vref);
+        }
+        if (t == 0) {
+            *reinterpret_cast<float2*>(ml_s + (warp * 16 + g) * 2) = make_float2(m0, l0);
+            *reinterpret_cast<float2*>(ml_s + (warp * 16 + g + 8) * 2) = make_float2(m1, l1);
+        }
+        team_sync(team, threads);
+        const int tile_rows = min(16, rows_all - s.tile * 16);
+        const int w0 = team * pl.width;
+        auto emit = [&](int r, int d, float4 x, float m, float l) {
+            const int row = s.tile * 16 + r;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            T* dst = static_cast<T*>(a.out) + (int64_t)(q.row + row / group) * a.o_row + (int64_t)(s.head * group + row % group) * a.o_head + d;
+            T y[4] = {from_f32<T>(x.x * inv), from_f32<T>(x.y * inv), from_f32<T>(x.z * inv), from_f32<T>(x.w * inv)};
+            *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(y);
+            if (a.lse && d == 0)
+                a.lse[(size_t)(q.row + row / group) * a.q_heads + s.head * group + row % group] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+        };
+        float* const ml_g = pr.part + (size_t)pr.slots * 16 * D;
+        for (int i = t_in; i < tile_rows * (D / 4); i += threads) {
+            const int r = i / (D / 4), d = i % (D / 4) * 4;
+            float m = -INFINITY;
+            for (int w = 0; w < pl.width; ++w) m = fmaxf(m, ml_s[((w0 + w) * 16 + r) * 2]);
+            const float z = m == -INFINITY ? 0.0f : m;
+            float l = 0.0f;
+            float4 x = make_float4(0, 0, 0, 0);
+            for (int w = 0; w < pl.width; ++w) {
+                const float k = ex2(ml_s[((w0 + w) * 16 + r) * 2] - z);
+                const float4 y = *reinterpret_cast<const float4*>(acc_s + ((w0 + w) * 16 + r) * kAccStride<D> + d);
+                l = fmaf(k, ml_s[((w0 + w) * 16 + r) * 2 + 1], l);
+                x.x = fmaf(k, y.x, x.x);
+                x.y = fmaf(k, y.y, x.y);
+                x.z = fmaf(k, y.z, x.z);
+                x.w = fmaf(k, y.w, x.w);
+            }
+            if (s.parts == 1) {
+                emit(r, d, x, m, l);
+            } else {
+                const size_t slot = (size_t)slot_of(s, s.part);
+                __stcg(reinterpret_cast<float4*>(pr.part + (slot * 16 + r) * D + d), x);
+                if (d == 0) __stcg(reinterpret_cast<float2*>(ml_g + (slot * 16 + r) * 2), make_float2(m, l));
+            }
+        }
+        if (s.parts > 1) {
+            __threadfence();
+            team_sync(team, threads);
+            if (t_in == 0) {
+                const unsigned before = atomicAdd(&pr.counters[s.first], 1u);
+                if (before + 1 == (unsigned)s.parts) pr.counters[s.first] = 0;
+                arrived_s[warp] = before + 1;
+            }
+            team_sync(team, threads);
+            if (arrived_s[w0] == (unsigned)s.parts) {
+                __threadfence();
+                for (int i = t_in; i < tile_rows * (D / 4); i += threads) {
+                    const int r = i / (D / 4), d = i % (D / 4) * 4;
+                    float m = -INFINITY;
+                    for (int k = 0; k < s.parts; ++k) m = fmaxf(m, __ldcg(ml_g + ((size_t)slot_of(s, k) * 16 + r) * 2));
+                    const float z = m == -INFINITY ? 0.0f : m;
+                    float l = 0.0f;
+                    float4 x = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+                    for (int k = 0; k < s.parts; ++k) {
+                        const size_t slot = (size_t)slot_of(s, k);
+                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(ml_g + (slot * 16 + r) * 2));
+                        const float4 y = __ldcg(reinterpret_cast<const float4*>(pr.part + (slot * 16 + r) * D + d));
+                        const float e = ex2(ml.x - z);
+                        l = fmaf(e, ml.y, l);
+                        x.x = fmaf(e, y.x, x.x);
+                        x.y = fmaf(e, y.y, x.y);
+                        x.z = fmaf(e, y.z, x.z);
+                        x.w = fmaf(e, y.w, x.w);
+                    }
+                    emit(r, d, x, m, l);
+                }
+            }
+        }
+        team_sync(team, threads);  // the joined tiles are free again
+    }
+    if (!fine && lane == 0) atomicOr(c.status, MRL_KV_TIMEOUT);
+}
+
+template <class T, int D> cudaError_t launch(const Params& p, int sms, cudaStream_t s) {
+    constexpr int NW = kWarps<D>;
+    const size_t smem = (size_t)NW * 2 * kPage * D + sizeof(float) * NW * 16 * kAccStride<D> + sizeof(float) * NW * 32 + 16 * NW +
+                        (sizeof(SeqInfo) + sizeof(int)) * p.a.n_seqs;
+    if (const cudaError_t e = cudaFuncSetAttribute(decode_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return e;
+    decode_kernel<T, D><<<sms, NW * 32, smem, s>>>(p);
+    return cudaGetLastError();
+}
+
+}  // namespace
+}  // namespace kv
+
+// Pieces: one per job or two per team, jobs at most pages / width + items <= 2 warps of the launch.
+static int decode_slots(uint32_t head_dim, int sms) { return 2 * sms * (int)(1024 / head_dim) + 2; }
+size_t kv_decode_bytes(uint32_t head_dim, int sms) { return (size_t)decode_slots(head_dim, sms) * 16 * (head_dim + 2) * sizeof(float); }
+
+int launch_kv_decode(const mrl_kv_cache& c, const mrl_attn& a, int sms, void* scratch, unsigned* counters, cudaStream_t s) {
+    kv::Params p;
+    p.c = c;
+    p.a = a;
+    p.part = static_cast<float*>(scratch);
+    p.counters = counters;
+    p.slots = decode_slots(c.head_dim, sms);
+    p.row0 = 0;
+    const bool half = a.dtype == MRL_F16;
+    for (uint32_t at = 0; at < a.n_seqs; at += kKvDecodeSeqs) {
+        p.a.n_seqs = a.n_seqs - at < kKvDecodeSeqs ? a.n_seqs - at : kKvDecodeSeqs;
+        p.a.seqs = a.seqs + at;
+        p.a.cu = a.cu ? a.cu + at : nullptr;
+        p.row0 = (int)at;
+        cudaError_t e;
+        if (c.head_dim == 64) e = half ? kv::launch<__half, 64>(p, sms, s) : kv::launch<__nv_bfloat16, 64>(p, sms, s);
+        else if (c.head_dim == 128) e = half ? kv::launch<__half, 128>(p, sms, s) : kv::launch<__nv_bfloat16, 128>(p, sms, s);
+        else e = half ? kv::launch<__half, 256>(p, sms, s) : kv::launch<__nv_bfloat16, 256>(p, sms, s);
+        if (e != cudaSuccess) return (int)e;
+    }
+    return 0;
+}
+
+}  // namespace mrl
