@@ -1,0 +1,889 @@
+// attend_tc.cu — attention on the 5th-generation tensor cores (tcgen05, sm_100a): mrl_window_attention over
+// ragged 16-bit rows, and mrl_kv_attend over the paged 8-bit cache where sequences have many query rows.
+//
+// A tile is 128 query rows of one sequence and kv head: 128 / group tokens x the group's query heads, so
+// all query heads of a kv head share its K and V. Per 128 keys a tile does S = Q K^T (both from shared
+// memory, S in tensor memory), softmax on 128 threads, one row each, that put P back into tensor memory
+// over S as 16-bit pairs, and O += P V with P from there. head_dim 64 and 128 run two tiles per CTA that
+// share each K and V: while one tile's S is exponentiated the tensor core works for the other. head_dim 256
+// has tensor memory for one O only, and runs one tile with two S buffers instead.
+//
+// The running maximum a row subtracts moves only when a new one exceeds it by 2^8 (base-2 logits): O and
+// the sum l are kept relative to the stale one, which cancels in o = O / l, and O is rescaled rarely. P is
+// at most 2^8, well inside f16, and its rounding is relative either way.
+//
+// Roles: warps 0-3 and 4-7 softmax and epilogue of the tiles (they also load their rows of Q), warp 8
+// issues the products, warp 9 loads K and V by TMA (16-bit rows) or, over the cache, warps 9-12 bring the
+// int8 blocks in by bulk copies and widen them to f16 (exact) into the operand layout; the blocks' scales
+// go to S and P, which are f32 there. Every wait is bounded; when one runs out the kernel records it and
+// ends.
+//
+// Bound by the tensor core and the exponentials together: per 128 x 128 x D tile pair 2 x 2 x 128 x 128 x D
+// products against 2 x 16384 exponentials at 16 per clock and SM.
+#include <cuda.h>
+
+#include "kv.cuh"
+#include "umma.cuh"
+
+namespace mrl {
+namespace kv {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr long long kWaitClocks = 4000000000ll;  // about two seconds
+constexpr int kKeys = 128;        // keys per step
+constexpr float kSlack = 8.0f;    // log2 by which a row's maximum may lead the one it subtracts
+constexpr float kScaleSlack = 64.0f;  // the same for V's scales over the cache (a factor)
+constexpr int kInfo = 8;          // steps of scales kept
+
+// What a template instance is: D, two tiles or one, stages of K and V, and its threads.
+template <int D, bool PAGED> struct Shape {
+    static constexpr int tiles = D == 256 ? 1 : 2;
+    static constexpr int sbufs = D == 256 ? 2 : 1;
+    static constexpr int stages = D == 64 ? 3 : D == 128 ? 2 : 1;
+    static constexpr int q_bytes = 128 * D * 2, kv_bytes = kKeys * D * 2;
+    static constexpr int block = kPage * D;  // codes of a page and head
+    static constexpr int slots = PAGED ? (D == 64 ? 8 : D == 128 ? 3 : 2) : 0;  // staged blocks
+    static constexpr int seqs = !PAGED || D == 64 ? 512 : D == 128 ? 384 : 64;  // sequences per launch (their table is in shared memory)
+    static constexpr int conv_warps = PAGED ? 4 : 0;
+    static constexpr int threads = (9 + (PAGED ? conv_warps : 1)) * 32;
+    static constexpr int tmem_s = 0;                           // S (and P) columns of tile or buffer i at 128 i
+    static constexpr int tmem_o = 256;                         // O columns of tile i at 256 + D i
+    static constexpr size_t smem = 1024 + (size_t)tiles * q_bytes + 2 * stages * kv_bytes + (size_t)slots * block;
+};
+
+struct SeqItem {
+    unsigned start;  // first item of the sequence
+    int len, row, m;
+};
+
+struct TcParams {
+    mrl_kv_cache c;
+    mrl_attn a;
+    int heads, group, tokens;  // kv heads, query heads per kv head, tokens per tile
+    int causal, keys_inner;    // keys_inner: the maps' second dimension is the row, not the head
+};
+
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
+    if (tc::mbar_wait(bar, parity, 16)) return true;
+    const long long start = clock64();
+    while (!tc::mbar_wait(bar, parity, 16)) {
+        if (*failed) return false;
+        if (clock64() - start > kWaitClocks) {
+            *failed = 1;
+            return false;
+        }
+    }
+    return true;
+}
+__device__ __forceinline__ void arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc::smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void expect(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(tc::smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void tma3(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(tc::smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void bulk(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),
+                 "r"(tc::smem_u32(bar))
+                 : "memory");
+}
+
+// kind::f16 products, f32 accumulators; A and B of the same 16-bit type.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
+                 "l"(b), "r"(idesc), "r"(acc)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a),
+                 "l"(b), "r"(idesc), "r"(acc)
+                 : "memory");
+}
+// M 128, N n; bf: bf16 operands, else f16; mn: B is N-major.
+__host__ __device__ constexpr uint32_t idesc_f16(int n, bool bf, bool mn) {
+    return (1u << 4) | ((bf ? 1u : 0u) << 7) | ((bf ? 1u : 0u) << 10) | ((mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+}
+// 128-byte swizzle: 8 rows of 128 bytes per 1024-byte atom, atoms `sbo` apart along the rows, and for a
+// B that is N-major, 64-wide column blocks `lbo` apart.
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | (uint64_t)((lbo >> 4) & 0x3FFFu) << 16 | (uint64_t)((sbo >> 4) & 0x3FFFu) << 32 | (uint64_t)1 << 46 |
+           (uint64_t)2 << 61;
+}
+
+#define MRL_TC_LD32(r, taddr)                                                                                                            \
+    asm volatile(                                                                                                                        \
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "  \
+        "%19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"                                                       \
+        : "=r"((r)[0]), "=r"((r)[1]), "=r"((r)[2]), "=r"((r)[3]), "=r"((r)[4]), "=r"((r)[5]), "=r"((r)[6]), "=r"((r)[7]), "=r"((r)[8]),  \
+          "=r"((r)[9]), "=r"((r)[10]), "=r"((r)[11]), "=r"((r)[12]), "=r"((r)[13]), "=r"((r)[14]), "=r"((r)[15]), "=r"((r)[16]),         \
+          "=r"((r)[17]), "=r"((r)[18]), "=r"((r)[19]), "=r"((r)[20]), "=r"((r)[21]), "=r"((r)[22]), "=r"((r)[23]), "=r"((r)[24]),        \
+          "=r"((r)[25]), "=r"((r)[26]), "=r"((r)[27]), "=r"((r)[28]), "=r"((r)[29]), "=r"((r)[30]), "=r"((r)[31])                        \
+        : "r"(taddr)                                                                                                                     \
+        : "memory")
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <bool BF> __device__ __forceinline__ uint32_t pack16(float a, float b) {
+    uint32_t r;
+    if (BF) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        r = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        const __half2 h = __floats2half2_rn(a, b);
+        r = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return r;
+}
+__device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {  // exact, as in kv_decode.cu
+    w ^= 0x80808080u;
+    const __half2 off = __half2half2(__ushort_as_half(0x6480));
+    uint32_t x = __byte_perm(w, 0x64646464u, 0x4140), y = __byte_perm(w, 0x64646464u, 0x4342);
+    __half2 a = __hsub2(*reinterpret_cast<__half2*>(&x), off), b = __hsub2(*reinterpret_cast<__half2*>(&y), off);
+    lo = *reinterpret_cast<uint32_t*>(&a);
+    hi = *reinterpret_cast<uint32_t*>(&b);
+}
+
+// Key steps of a tile: [0, head) and [lo, hi), of 128 keys each. Empty: hi == 0.
+struct Steps {
+    int head, lo, hi;
+    __device__ __forceinline__ bool has(int s) const { return s < head || (s >= lo && s < hi); }
+};
+// Of the tokens at positions [p0, p1] of a sequence of n keys.
+__device__ __forceinline__ Steps steps_of(int p0, int p1, int n, int causal, int window, int sinks) {
+    const Span a = visible(p0, n, causal, window, sinks), b = visible(p1, n, causal, window, sinks);
+    Steps s{0, 0, 0};
+    if (imax(a.hi, b.hi) <= 0) return s;
+    s.hi = (imax(a.hi, b.hi) + kKeys - 1) / kKeys;
+    s.lo = imin(a.lo, s.hi * kKeys) / kKeys;
+    s.head = imin((imax(a.head, b.head) + kKeys - 1) / kKeys, s.lo);
+    return s;
+}
+
+// One item: `tiles` tiles of consecutive tokens of one sequence and kv head.
+template <int TILES> struct Item {
+    int b, head, first;  // first: token (row of the sequence) of the item
+    int len, row, m;
+    Steps st[TILES];
+    Steps all;
+    __device__ __forceinline__ int next(int s) const { return s + 1 == all.head ? (all.lo > s + 1 ? all.lo : s + 1) : s + 1; }
+    __device__ __forceinline__ int begin() const { return all.head > 0 ? 0 : all.lo; }
+};
+
+// The exact result of one row whose fast one is not finite: Inf or NaN in a value that the row does not see
+// reaches a product as 0 x Inf; here only the visible keys are read. Lane e holds dims e D/32 .. .
+template <class T, int D> __device__ __noinline__ void slow_row(const mrl_attn& a, int row0, int n, int p, int t_row, int h, int kvh, int causal) {
+    constexpr int E = D / 32;
+    const int lane = (int)threadIdx.x & 31;
+    const Span span = visible(p, n, causal, (int)a.window, (int)a.sinks);
+    float q[E], o[E];
+    const T* qp = static_cast<const T*>(a.q) + (int64_t)t_row * a.q_row + (int64_t)h * a.q_head + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        q[e] = to_f32<T>(qp[e]);
+        o[e] = 0.0f;
+    }
+    float m = -INFINITY, l = 0.0f;
+    for (int part = 0; part < 2; ++part) {
+        const int from = part ? span.lo : 0, to = part ? span.hi : span.head;
+        for (int j = from; j < to; ++j) {
+            const T* kp = static_cast<const T*>(a.k) + (int64_t)(row0 + j) * a.k_row + (int64_t)kvh * a.k_head + lane * E;
+            const T* vp = static_cast<const T*>(a.v) + (int64_t)(row0 + j) * a.v_row + (int64_t)kvh * a.v_head + lane * E;
+            float s = 0.0f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) s = fmaf(q[e], to_f32<T>(kp[e]), s);
+#pragma unroll
+            for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
+            s *= a.scale;
+            const float top = s > m || s != s ? s : m;  // a NaN stays
+            const float keep = m == -INFINITY ? 0.0f : expf(m - top), add = s == -INFINITY && top == -INFINITY ? 0.0f : expf(s - top);
+            m = top;
+            l = fmaf(l, keep, add);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = (keep == 0.0f ? 0.0f : o[e] * keep) + add * to_f32<T>(vp[e]);
+        }
+    }
+    T* op = static_cast<T*>(a.out) + (int64_t)t_row * a.o_row + (int64_t)h * a.o_head + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) op[e] = from_f32<T>(l == 0.0f ? 0.0f : o[e] / l);
+    if (a.lse && lane == 0) a.lse[(size_t)t_row * a.q_heads + h] = l == 0.0f ? -INFINITY : m + logf(l);
+}
+
+template <class T, int D, bool PAGED>
+__global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
+    tc_kernel(const __grid_constant__ TcParams pr, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
+    using S = Shape<D, PAGED>;
+    constexpr bool kBf = !PAGED && !__is_same(T, __half);  // operand type of the products
+    constexpr int TILES = S::tiles, SB = S::sbufs, ST = S::stages;
+    extern __shared__ unsigned char raw[];
+    unsigned char* smem = raw + (1024 - (tc::smem_u32(raw) & 1023)) % 1024;
+    unsigned char* q_s = smem;                                  // per tile [D/64][128 rows][128 B], swizzled
+    unsigned char* k_s = q_s + (size_t)TILES * S::q_bytes;      // per stage [D/64][128 keys][128 B]
+    unsigned char* v_s = k_s + (size_t)ST * S::kv_bytes;        // per stage the same, over the cache [2 pages][D][128 B]
+    unsigned char* stage_s = v_s + (size_t)ST * S::kv_bytes;    // codes
+    __shared__ SeqItem info[S::seqs];
+    __shared__ int seq_s[PAGED ? S::seqs : 1];
+    __shared__ unsigned scan_s[32];
+    __shared__ uint64_t q_full[TILES], k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], s_full[2], p_full[2], o_full[TILES], o_free[TILES],
+        pv_done[2], code_full[PAGED ? S::slots : 1];
+    __shared__ uint32_t tmem_s;
+    __shared__ volatile int failed;
+    __shared__ float4 scales_s[kInfo];  // over the cache: K scales of a step's two pages, V scales
+    __shared__ int present_s[kInfo];    // bit i: page i of the step exists
+
+    const mrl_attn& a = pr.a;
+    const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int n = (int)a.n_seqs, group = pr.group, tokens = pr.tokens;
+    const int window = (int)a.window, sinks = (int)a.sinks, causal = pr.causal;
+
+    if (tid == 0) {
+        failed = 0;
+        for (int i = 0; i < TILES; ++i) {
+            tc::mbar_init(&q_full[i], 128);
+            tc::mbar_init(&o_full[i], 1);
+            tc::mbar_init(&o_free[i], 128);
+        }
+        for (int i = 0; i < ST; ++i) {
+            tc::mbar_init(&k_full[i], PAGED ? S::conv_warps : 1);
+            tc::mbar_init(&k_empty[i], 1);
+            tc::mbar_init(&v_full[i], PAGED ? S::conv_warps : 1);
+            tc::mbar_init(&v_empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            tc::mbar_init(&s_full[i], 1);
+            tc::mbar_init(&p_full[i], 128);
+            tc::mbar_init(&pv_done[i], 1);
+        }
+        for (int i = 0; i < (PAGED ? S::slots : 1); ++i) tc::mbar_init(&code_full[i], 1);
+        tc::fence_mbar_init();
+    }
+    if (warp == 8) {
+        tc::tmem_alloc(&tmem_s, 512);
+        tc::tmem_relinquish();
+    }
+    // ---- the call's sequences and their items
+    unsigned carry = 0;
+    for (int at = 0; at < n; at += S::threads) {
+        const int b = at + tid;
+        unsigned v = 0;
+        SeqItem q{0, 0, 0, 0};
+        if (b < n) {
+            const Rows r{a.seqs, a.cu, n, (int)a.n_tokens};
+            q.row = r.begin(b);
+            q.m = r.end(b) - q.row;
+            q.len = q.m;
+            if (PAGED) {
+                const int seq = a.seqs[b];
+                const bool known = seq >= 0 && seq < (int)pr.c.max_seqs;
+                seq_s[b] = known ? seq : 0;
+                q.len = known ? min(max(pr.c.lens[seq], 0), (int)pr.c.max_pages * kPage) : 0;
+            }
+            v = q.m > 0 ? (unsigned)((q.m + TILES * tokens - 1) / (TILES * tokens)) * (unsigned)pr.heads : 0;
+        }
+        unsigned x = v;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const unsigned y = __shfl_up_sync(~0u, x, d);
+            if (lane >= d) x += y;
+        }
+        if (lane == 31) scan_s[warp] = x;
+        __syncthreads();
+        unsigned before = carry;
+        for (int w = 0; w < S::threads / 32; ++w) {
+            if (w < warp) before += scan_s[w];
+            carry += scan_s[w];
+        }
+        q.start = before + x - v;
+        if (b < n) info[b] = q;
+        __syncthreads();
+    }
+    const unsigned items = carry;
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = tmem_s;
+
+    // Item i; the tiles with the latest tokens come first, they have the most keys where the mask is causal.
+    auto item_at = [&](unsigned i) {
+        Item<TILES> it;
+        int lo = 0, hi = n;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (info[mid].start <= i) lo = mid;
+            else hi = mid;
+        }
+        const SeqItem q = info[lo];
+        const int count = (q.m + TILES * tokens - 1) / (TILES * tokens);
+        const unsigned local = i - q.start;
+        it.b = lo;
+        it.head = (int)(local % (unsigned)pr.heads);
+        it.first = (count - 1 - (int)(local / (unsigned)pr.heads)) * TILES * tokens;
+        it.len = q.len;
+        it.row = q.row;
+        it.m = q.m;
+        it.all = Steps{0, 0, 0};
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+            const int f = it.first + t * tokens, base = q.len - q.m;
+            it.st[t] = f < q.m ? steps_of(base + f, base + imin(f + tokens, q.m) - 1, q.len, causal, window, sinks) : Steps{0, 0, 0};
+            if (it.st[t].hi > 0) {
+                const bool none = it.all.hi == 0;
+                it.all.hi = imax(it.all.hi, it.st[t].hi);
+                it.all.lo = none ? it.st[t].lo : imin(it.all.lo, it.st[t].lo);
+                it.all.head = imax(it.all.head, it.st[t].head);
+            }
+        }
+        it.all.head = imin(it.all.head, it.all.lo);
+        return it;
+    };
+
+    if (warp < 4 * TILES) {
+        // ---- softmax and epilogue of tile `tile`: thread = row
+        const int tile = warp >> 2, r = tid & 127;
+        const uint32_t lane_off = (uint32_t)(warp & 3) << 21;  // lane 32 (warp % 4) of tensor memory
+        unsigned char* q_tile = q_s + (size_t)tile * S::q_bytes;
+        const int tok = r / group, qh = r % group;
+        const bool row_used = tok < tokens;
+        uint32_t s_par = 0, o_par = 0;  // bit i: buffer i
+        int step_no = 0, used = 0;
+        float c0 = 0.0f;  // softmax scale in base 2 (over the cache with the row's power of two)
+        // This thread's row of Q for item `it` into shared memory.
+        auto load_q = [&](const Item<TILES>& it) {
+            const int f = it.first + tile * tokens + tok;
+            const bool in = row_used && f < it.m;
+            const T* p = static_cast<const T*>(a.q) + (int64_t)(it.row + f) * a.q_row + (int64_t)(it.head * group + qh) * a.q_head;
+            c0 = a.scale * kLog2e;
+            float down = 1.0f;
+            if (PAGED && !__is_same(T, __half)) {
+                // bf16 to f16 by way of [1, 2): see kv_decode.cu
+                float top = 0.0f;
+                if (in) {
+                    for (int i = 0; i < D / 8; ++i) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(p + i * 8);
+                        const T* e = reinterpret_cast<const T*>(&x);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(to_f32<T>(e[j])));
+                    }
+                }
+                const uint32_t ex = __float_as_uint(top) >> 23;
+                if (ex > 0 && ex < 255) {
+                    const uint32_t up = min(ex, 253u);
+                    down = __uint_as_float((254u - up) << 23);
+                    c0 *= __uint_as_float(up << 23);
+                }
+            }
+#pragma unroll 4
+            for (int i = 0; i < D / 8; ++i) {
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (in) x = *reinterpret_cast<const uint4*>(p + i * 8);
+                if (PAGED && !__is_same(T, __half)) {
+                    const T* e = reinterpret_cast<const T*>(&x);
+                    uint32_t y[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) y[j] = pack16<false>(to_f32<T>(e[2 * j]) * down, to_f32<T>(e[2 * j + 1]) * down);
+                    x = make_uint4(y[0], y[1], y[2], y[3]);
+                }
+                *reinterpret_cast<uint4*>(q_tile + (i >> 3) * 16384 + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = x;
+            }
+            tc::fence_proxy_async_smem();
+            arrive(&q_full[tile]);
+        };
+        Item<TILES> it;
+        if (blockIdx.x < items) {
+            it = item_at(blockIdx.x);
+            if (it.st[tile].hi > 0) load_q(it);
+        }
+        for (unsigned i = blockIdx.x; i < items && !failed; i += gridDim.x) {
+            const float cur = c0;
+            const int f = it.first + tile * tokens, base = it.len - it.m;
+            const Steps st = it.st[tile];
+            const int p = base + f + tok;
+            const Span span = f + tok < it.m ? visible(p, it.len, causal, window, sinks) : Span{0, 0, 0};
+            // all of the tile's rows see keys [full_lo, full_hi) (and the sinks)
+            const int p_lo = base + f, p_hi = base + imin(f + tokens, it.m) - 1;
+            float m = -INFINITY, l = 0.0f, vref = 0.0f;
+            bool any = false;
+            for (int s = it.begin(); s < it.all.hi; s = it.next(s), ++step_no) {
+                if (!st.has(s)) continue;
+                const int buf = SB == 2 ? used & 1 : tile;
+                if (!wait(&s_full[buf], (s_par >> buf) & 1, &failed)) break;
+                s_par ^= 1u << buf;
+                tc::fence_after();
+                const uint32_t s_col = tmem + lane_off + S::tmem_s + buf * 128;
+                const int key0 = s * kKeys;
+                float ka = cur, kb = cur, va = 1.0f, vb = 1.0f;
+                bool full = key0 + kKeys <= it.len && (!causal || key0 + kKeys - 1 <= p_lo) &&
+                            (window == 0 || key0 + kKeys <= sinks || (key0 > p_hi - window && (causal || key0 + kKeys - 1 < p_lo + window)));
+                int there = 3;
+                if (PAGED) {
+                    const float4 x = scales_s[step_no & (kInfo - 1)];
+                    there = present_s[step_no & (kInfo - 1)];
+                    ka *= x.x;
+                    kb *= x.y;
+                    va = x.z;
+                    vb = x.w;
+                    full = full && there == 3;
+                }
+                // pass 1: the largest score
+                float top = -INFINITY;
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    uint32_t x[32];
+                    MRL_TC_LD32(x, s_col + h * 32);
+                    tc::wait_ld();
+                    float mx = -INFINITY;
+                    if (full) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) mx = fmaxf(mx, __uint_as_float(x[j]));
+                    } else if (there >> (h >> 1) & 1) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            const int key = key0 + h * 32 + j;
+                            if (key < span.head || (key >= span.lo && key < span.hi)) mx = fmaxf(mx, __uint_as_float(x[j]));
+                        }
+                    }
+                    top = fmaxf(top, mx * (h < 2 ? ka : kb));
+                }
+                // the maximum that is subtracted, and V's scale unit, move rarely
+                float keep = 1.0f;
+                const float vmax = fmaxf(va, vb);
+                const bool grow = top > m + kSlack;
+                if (PAGED && vmax > kScaleSlack * vref) {
+                    keep = vref / vmax;
+                    vref = vmax;
+                }
+                if (grow) {
+                    const float le = m == -INFINITY ? 1.0f : ex2(m - top);  // O and l are 0 until a key was seen
+                    keep *= le;
+                    l *= le;
+                    m = top;
+                }
+                if (any && __any_sync(~0u, keep != 1.0f)) {
+                    if (SB == 2) {  // the product of the step before may still be adding to O
+                        if (!wait(&pv_done[buf ^ 1], (uint32_t)((used - 1) >> 1) & 1, &failed)) break;
+                        tc::fence_after();
+                    }
+                    const uint32_t o_col = tmem + lane_off + S::tmem_o + tile * D;
+#pragma unroll 1
+                    for (int h = 0; h < D / 16; ++h) {
+                        uint32_t x[16];
+                        TC_LD16(x, o_col + h * 16);
+                        tc::wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * keep);
+                        TC_ST16(o_col + h * 16, x);
+                    }
+                    tc::wait_st();
+                }
+                any = true;
+                if (PAGED) {
+                    va = vref > 0.0f ? va / vref : 0.0f;
+                    vb = vref > 0.0f ? vb / vref : 0.0f;
+                }
+                // pass 2: P over S; its first half goes where scores already read were
+                const float z = m == -INFINITY ? 0.0f : -m;
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    uint32_t x[32];
+                    MRL_TC_LD32(x, s_col + h * 32);
+                    tc::wait_ld();
+                    const float k = h < 2 ? ka : kb, v = h < 2 ? va : vb;
+                    uint32_t y[16];
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        float e0 = ex2(fmaf(__uint_as_float(x[j]), k, z)), e1 = ex2(fmaf(__uint_as_float(x[j + 1]), k, z));
+                        if (!full) {
+                            const int key = key0 + h * 32 + j;
+                            const bool ok = there >> (h >> 1) & 1;
+                            if (!ok || !(key < span.head || (key >= span.lo && key < span.hi))) e0 = 0.0f;
+                            if (!ok || !(key + 1 < span.head || (key + 1 >= span.lo && key + 1 < span.hi))) e1 = 0.0f;
+                        }
+                        sum += e0 + e1;
+                        if (PAGED) e0 *= v, e1 *= v;
+                        y[j >> 1] = pack16<kBf>(e0, e1);
+                    }
+                    l += sum;
+                    TC_ST16(s_col + h * 16, y);
+                }
+                tc::wait_st();
+                tc::fence_before();
+                arrive(&p_full[buf]);
+                ++used;
+            }
+            // the next item's Q: this one's last S is done, nothing reads Q any more
+            const Item<TILES> done = it;
+            if (i + gridDim.x < items) {
+                it = item_at(i + gridDim.x);
+                if (it.st[tile].hi > 0) load_q(it);
+            }
+            const bool in = row_used && done.first + tile * tokens + tok < done.m;
+            const int t_row = done.row + done.first + tile * tokens + tok, h = done.head * group + qh;
+            T* dst = static_cast<T*>(a.out) + (int64_t)t_row * a.o_row + (int64_t)h * a.o_head;
+            float bad = 0.0f;
+            if (any) {
+                if (!wait(&o_full[tile], o_par, &failed)) break;
+                o_par ^= 1;
+                tc::fence_after();
+                const uint32_t o_col = tmem + lane_off + S::tmem_o + tile * D;
+                const float inv = l == 0.0f ? 0.0f : (PAGED ? vref : 1.0f) / l;
+#pragma unroll
+                for (int j = 0; j < D / 32; ++j) {
+                    uint32_t x[32];
+                    MRL_TC_LD32(x, o_col + j * 32);
+                    tc::wait_ld();
+                    if (j == D / 32 - 1) {
+                        tc::fence_before();
+                        arrive(&o_free[tile]);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 32; k += 8) {
+                        uint4 y;
+                        uint32_t* w = &y.x;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float u = __uint_as_float(x[k + 2 * e]), v = __uint_as_float(x[k + 2 * e + 1]);
+                            if (!PAGED) bad = fmaf(u, 0.0f, fmaf(v, 0.0f, bad));
+                            w[e] = pack16<!__is_same(T, __half)>(l == 0.0f ? 0.0f : u * inv, l == 0.0f ? 0.0f : v * inv);
+                        }
+                        if (in) *reinterpret_cast<uint4*>(dst + j * 32 + k) = y;
+                    }
+                }
+            } else if (in) {
+                for (int j = 0; j < D / 8; ++j) *reinterpret_cast<uint4*>(dst + j * 8) = make_uint4(0, 0, 0, 0);
+            }
+            if (in && a.lse) a.lse[(size_t)t_row * a.q_heads + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+            if (!PAGED) {
+                // not finite: a value the row sees, or one it does not (a later key, another sequence's row)
+                unsigned again = __ballot_sync(~0u, in && !(bad == 0.0f && l < INFINITY && m < INFINITY));
+                while (again) {
+                    const int who = __ffs((int)again) - 1;
+                    again &= again - 1;
+                    slow_row<T, D>(a, done.row, done.len, __shfl_sync(~0u, p, who), __shfl_sync(~0u, t_row, who), __shfl_sync(~0u, h, who), done.head, causal);
+                }
+            }
+        }
+    } else if (warp == 8) {
+        // ---- the products: one thread
+        if (lane == 0) {
+            constexpr uint32_t id_s = idesc_f16(kKeys, kBf, false), id_o = idesc_f16(D, kBf, !PAGED);
+            uint32_t q_par = 0, p_par = 0, free_par = 0;
+            int step_no = 0, used = 0;
+            bool ok = true;
+            auto product_s = [&](int tile, int buf, int stage) {
+                const uint32_t q_addr = tc::smem_u32(q_s + (size_t)tile * S::q_bytes), k_addr = tc::smem_u32(k_s + (size_t)stage * S::kv_bytes);
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint32_t off = (uint32_t)((k >> 2) * 16384 + (k & 3) * 32);
+                    mma_ss(tmem + S::tmem_s + buf * 128, desc_sw128(q_addr + off, 16, 1024), desc_sw128(k_addr + off, 16, 1024), id_s, k > 0);
+                }
+                tc::mma_commit(&s_full[buf]);
+            };
+            auto product_o = [&](int tile, int buf, int stage, bool first) {
+                const uint32_t v_addr = tc::smem_u32(v_s + (size_t)stage * S::kv_bytes);
+#pragma unroll
+                for (int k = 0; k < kKeys / 16; ++k) {
+                    const uint64_t b = PAGED ? desc_sw128(v_addr + (k >> 2) * (D * 128) + (k & 3) * 32, 16, 1024)
+                                             : desc_sw128(v_addr + k * 2048, 16384, 1024);
+                    mma_ts(tmem + S::tmem_o + tile * D, tmem + S::tmem_s + buf * 128 + k * 8, b, id_o, !(first && k == 0));
+                }
+            };
+            for (unsigned i = blockIdx.x; i < items && ok && !failed; i += gridDim.x) {
+                const Item<TILES> it = item_at(i);
+                bool q_here[TILES], begun[TILES];
+                int pend[TILES], pend_buf[TILES];  // step whose P is to come
+                for (int t = 0; t < TILES; ++t) q_here[t] = begun[t] = false, pend[t] = -1, pend_buf[t] = 0;
+                // O += P V of tile t's pending step
+                auto finish = [&](int t) {
+                    const int no = pend[t], stage = no % ST;
+                    if (!wait(&v_full[stage], (uint32_t)(no / ST) & 1, &failed)) return false;
+                    if (!begun[t]) {  // the previous item's O has been read
+                        if (!wait(&o_free[t], ((free_par >> t) & 1) ^ 1, &failed)) return false;
+                        free_par ^= 1u << t;
+                    }
+                    if (!wait(&p_full[pend_buf[t]], (p_par >> pend_buf[t]) & 1, &failed)) return false;
+                    p_par ^= 1u << pend_buf[t];
+                    tc::fence_after();
+                    product_o(t, pend_buf[t], stage, !begun[t]);
+                    if (SB == 2) tc::mma_commit(&pv_done[pend_buf[t]]);
+                    begun[t] = true;
+                    return true;
+                };
+                int prev = -1;  // the step before, whose V the tiles may still need
+                for (int s = it.begin(); s < it.all.hi && ok; s = it.next(s), ++step_no) {
+                    const int stage = step_no % ST;
+                    if (!wait(&k_full[stage], (uint32_t)(step_no / ST) & 1, &failed)) {
+                        ok = false;
+                        break;
+                    }
+                    tc::fence_after();
+                    for (int t = 0; t < TILES && ok; ++t) {
+                        const bool has = it.st[t].has(s);
+                        if (has && !q_here[t]) {
+                            ok = wait(&q_full[t], (q_par >> t) & 1, &failed);
+                            if (!ok) break;
+                            q_par ^= 1u << t;
+                            q_here[t] = true;
+                            tc::fence_after();
+                        }
+                        if (SB == 2) {
+                            // S of this step first: its buffer's last P went into O two steps ago
+                            const int buf = used & 1;
+                            product_s(t, buf, stage);
+                            tc::mma_commit(&k_empty[stage]);
+                            if (pend[t] >= 0) ok = finish(t);
+                            pend[t] = step_no;
+                            pend_buf[t] = buf;
+                            ++used;
+                        } else {
+                            if (pend[t] >= 0) {
+                                ok = finish(t);
+                                pend[t] = -1;
+                            }
+                            if (has && ok) {
+                                product_s(t, t, stage);
+                                pend[t] = step_no;
+                                pend_buf[t] = t;
+                            }
+                        }
+                    }
+                    if (!ok) break;
+                    if (SB == 1) tc::mma_commit(&k_empty[stage]);
+                    if (prev >= 0) tc::mma_commit(&v_empty[prev % ST]);
+                    prev = step_no;
+                }
+                if (!ok) break;
+                for (int t = 0; t < TILES && ok; ++t) {
+                    if (pend[t] >= 0) ok = finish(t);
+                    if (begun[t] && ok) tc::mma_commit(&o_full[t]);
+                }
+                if (prev >= 0 && ok) tc::mma_commit(&v_empty[prev % ST]);
+            }
+        }
+    } else if constexpr (!PAGED) {
+        // ---- K and V by TMA: boxes of 64 dims x 128 rows
+        if (warp == 9 && lane == 0) {
+            int step_no = 0;
+            bool ok = true;
+            for (unsigned i = blockIdx.x; i < items && ok && !failed; i += gridDim.x) {
+                const Item<TILES> it = item_at(i);
+                for (int s = it.begin(); s < it.all.hi && ok; s = it.next(s), ++step_no) {
+                    const int stage = step_no % ST;
+                    const uint32_t par = (uint32_t)(step_no / ST) & 1;
+                    const int row = it.row + s * kKeys;
+                    ok = wait(&k_empty[stage], par ^ 1, &failed);
+                    if (!ok) break;
+                    expect(&k_full[stage], S::kv_bytes);
+                    for (int d = 0; d < D / 64; ++d)
+                        tma3(tc::smem_u32(k_s + (size_t)stage * S::kv_bytes + d * 16384), &map_k, d * 64, pr.keys_inner & 1 ? row : it.head,
+                             pr.keys_inner & 1 ? it.head : row, &k_full[stage]);
+                    ok = wait(&v_empty[stage], par ^ 1, &failed);
+                    if (!ok) break;
+                    expect(&v_full[stage], S::kv_bytes);
+                    for (int d = 0; d < D / 64; ++d)
+                        tma3(tc::smem_u32(v_s + (size_t)stage * S::kv_bytes + d * 16384), &map_v, d * 64, pr.keys_inner & 2 ? row : it.head,
+                             pr.keys_inner & 2 ? it.head : row, &v_full[stage]);
+                }
+            }
+        }
+    } else if (warp >= 9) {
+        // ---- K and V from the cache: blocks of codes staged by bulk copies, widened into the operands
+        constexpr int kConv = S::conv_warps * 32;
+        const int ct = tid - 9 * 32;
+        const mrl_kv_cache& c = pr.c;
+        // Blocks in order: per step K of page 0 and 1, then V of page 0 and 1; block j of the run is staged in
+        // slot j % slots. Thread 0 looks them up and starts the copies, `slots` ahead.
+        struct Cursor {
+            unsigned i;
+            Item<TILES> it;
+            int s;
+        };
+        Cursor cur;
+        int queued = 0, q_step = 0;
+        __shared__ int there_s[PAGED ? S::slots : 1];
+        auto open = [&](Cursor& x) {  // the first item from x.i on that has steps
+            while (x.i < items) {
+                x.it = item_at(x.i);
+                x.s = x.it.begin();
+                if (x.s < x.it.all.hi) return true;
+                x.i += gridDim.x;
+            }
+            return false;
+        };
+        cur.i = blockIdx.x;
+        bool more = open(cur);
+        Cursor ahead = cur;
+        bool ahead_more = more;
+        int ahead_part = 0;
+        float sc[4] = {0, 0, 0, 0};
+        int pages[2] = {-1, -1};
+        auto queue = [&]() {  // thread 0: the next block's copy
+            if (!ahead_more) return;
+            const int slot = queued % S::slots;
+            if (ahead_part == 0) {
+                for (int k = 0; k < 2; ++k) {
+                    const int index = ahead.s * 2 + k;
+                    int page = -1;
+                    if (index * kPage < ahead.it.len) page = c.tables[(size_t)seq_s[ahead.it.b] * c.max_pages + index];
+                    pages[k] = page >= 0 && page < (int)c.pages ? page : -1;
+                }
+                for (int k = 0; k < 2; ++k)
+                    for (int w = 0; w < 2; ++w) sc[w * 2 + k] = pages[k] >= 0 ? c.scales[block_index(c, a.layer, pages[k], w, ahead.it.head)] : 0.0f;
+            }
+            const int page = pages[ahead_part & 1], which = ahead_part >> 1;
+            there_s[slot] = page >= 0;
+            if (page >= 0) {
+                expect(&code_full[slot], S::block);
+                bulk(tc::smem_u32(stage_s + (size_t)slot * S::block), c.codes + block_index(c, a.layer, page, which, ahead.it.head) * (size_t)S::block, S::block,
+                     &code_full[slot]);
+            } else {
+                arrive(&code_full[slot]);
+            }
+            if (ahead_part == 0) {
+                // steps of scales are read until their softmax is done, at most stages + 2 steps behind
+                scales_s[q_step & (kInfo - 1)] = make_float4(sc[0], sc[1], sc[2], sc[3]);
+                present_s[q_step & (kInfo - 1)] = (pages[0] >= 0 ? 1 : 0) | (pages[1] >= 0 ? 2 : 0);
+            }
+            ++queued;
+            if (++ahead_part == 4) {
+                ahead_part = 0;
+                ++q_step;
+                ahead.s = ahead.it.next(ahead.s);
+                if (ahead.s >= ahead.it.all.hi) {
+                    ahead.i += gridDim.x;
+                    ahead_more = open(ahead);
+                }
+            }
+        };
+        if (ct == 0)
+            for (int j = 0; j < S::slots; ++j) queue();
+        int step_no = 0, block = 0;
+        bool ok = true;
+        while (more && ok && !failed) {
+            const int stage = step_no % ST;
+            const uint32_t par = (uint32_t)(step_no / ST) & 1;
+            for (int part = 0; part < 4 && ok; ++part, ++block) {
+                const int slot = block % S::slots, half = part & 1;
+                const bool is_v = part >= 2;
+                if (half == 0) ok = wait(is_v ? &v_empty[stage] : &k_empty[stage], par ^ 1, &failed);
+                ok = ok && wait(&code_full[slot], (uint32_t)(block / S::slots) & 1, &failed);
+                if (!ok) break;
+                const bool have = there_s[slot] != 0;
+                const unsigned char* src = stage_s + (size_t)slot * S::block;
+                unsigned char* dst = is_v ? v_s + (size_t)stage * S::kv_bytes + half * (D * 128) : k_s + (size_t)stage * S::kv_bytes;
+                // 16 codes a thread and turn: row of 64 bytes -> 128-byte row, two 16-byte chunks
+#pragma unroll
+                for (int x = 0; x < S::block / 16 / kConv; ++x) {
+                    const int u = x * kConv + ct, line = u >> 2, quarter = u & 3;
+                    uint4 w = make_uint4(0x0u, 0x0u, 0x0u, 0x0u);
+                    if (have) w = *reinterpret_cast<const uint4*>(src + line * 64 + quarter * 16);
+                    uint4 e0, e1;
+                    widen4(w.x, e0.x, e0.y);
+                    widen4(w.y, e0.z, e0.w);
+                    widen4(w.z, e1.x, e1.y);
+                    widen4(w.w, e1.z, e1.w);
+                    // K: line = 64 block + token, to row 64 half + token of its block; V: line = dim
+                    const int at = is_v ? line * 128 : (line >> 6) * 16384 + (half * 64 + (line & 63)) * 128;
+                    const int sw = line & 7;
+                    *reinterpret_cast<uint4*>(dst + at + (((2 * quarter) ^ sw) << 4)) = e0;
+                    *reinterpret_cast<uint4*>(dst + at + (((2 * quarter + 1) ^ sw) << 4)) = e1;
+                }
+                tc::fence_proxy_async_smem();
+                asm volatile("bar.sync 1, %0;" ::"n"(kConv) : "memory");  // the staged block is read
+                if (half == 1 && lane == 0) arrive(is_v ? &v_full[stage] : &k_full[stage]);
+                if (ct == 0) queue();
+            }
+            ++step_no;
+            cur.s = cur.it.next(cur.s);
+            if (cur.s >= cur.it.all.hi) {
+                cur.i += gridDim.x;
+                more = open(cur);
+            }
+        }
+    }
+    __syncthreads();
+    if (warp == 8) tc::tmem_dealloc(tmem, 512);
+    if (tid == 0 && failed && pr.c.status) atomicOr(pr.c.status, MRL_KV_TIMEOUT);
+}
+
+using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                            const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+Encode encoder() {
+    static Encode f = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) != cudaSuccess) p = nullptr;
+        return reinterpret_cast<Encode>(p);
+    }();
+    return f;
+}
+
+// [rows][heads][D] 16-bit rows: dimensions D, then head and row in the order of their strides.
+bool make_map(CUtensorMap* map, const mrl_attn& a, const void* p, int64_t row, int64_t head, int d, int* keys_inner) {
+    const bool inner = a.n_tokens > 1 && (a.kv_heads == 1 ? false : row < head);
+    if (a.kv_heads == 1) head = d;
+    if (a.n_tokens == 1) row = (int64_t)a.kv_heads * d;
+    const cuuint64_t dims[3] = {(cuuint64_t)d, inner ? a.n_tokens : a.kv_heads, inner ? a.kv_heads : a.n_tokens};
+    const cuuint64_t strides[2] = {(cuuint64_t)(inner ? row : head) * 2, (cuuint64_t)(inner ? head : row) * 2};
+    const cuuint32_t box[3] = {64, inner ? (cuuint32_t)kKeys : 1u, inner ? 1u : (cuuint32_t)kKeys}, one[3] = {1, 1, 1};
+    *keys_inner = inner;
+    const Encode f = encoder();
+    return f && f(map, a.dtype == MRL_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p), dims, strides, box,
+                  one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <class T, int D, bool PAGED> int launch(TcParams p, int sms, cudaStream_t s) {
+    using S = Shape<D, PAGED>;
+    CUtensorMap mk = {}, mv = {};
+    if (!PAGED) {
+        int ik, iv;
+        if (!make_map(&mk, p.a, p.a.k, p.a.k_row, p.a.k_head, D, &ik) || !make_map(&mv, p.a, p.a.v, p.a.v_row, p.a.v_head, D, &iv)) return -1;
+        p.keys_inner = ik | iv << 1;
+    }
+    p.tokens = 128 / p.group;
+    if (const cudaError_t e = cudaFuncSetAttribute(tc_kernel<T, D, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::smem)) return (int)e;
+    const mrl_attn a = p.a;
+    for (uint32_t at = 0; at < a.n_seqs; at += S::seqs) {
+        p.a.n_seqs = a.n_seqs - at < (uint32_t)S::seqs ? a.n_seqs - at : (uint32_t)S::seqs;
+        p.a.seqs = a.seqs ? a.seqs + at : nullptr;
+        p.a.cu = a.cu + at;
+        // at most one part-filled item per sequence and head
+        const uint64_t most = ((uint64_t)a.n_tokens / (S::tiles * p.tokens) + p.a.n_seqs) * p.heads;
+        tc_kernel<T, D, PAGED><<<(unsigned)(most < (uint64_t)sms ? most : sms), S::threads, S::smem, s>>>(p, mk, mv);
+        if (const cudaError_t e = cudaGetLastError()) return (int)e;
+    }
+    return 0;
+}
+
+template <bool PAGED> int dispatch(const TcParams& p, uint32_t d, int sms, cudaStream_t s) {
+    if (p.a.dtype == MRL_F16)
+        return d == 64 ? launch<__half, 64, PAGED>(p, sms, s) : d == 128 ? launch<__half, 128, PAGED>(p, sms, s) : launch<__half, 256, PAGED>(p, sms, s);
+    return d == 64    ? launch<__nv_bfloat16, 64, PAGED>(p, sms, s)
+           : d == 128 ? launch<__nv_bfloat16, 128, PAGED>(p, sms, s)
+                      : launch<__nv_bfloat16, 256, PAGED>(p, sms, s);
+}
+
+}  // namespace
+}  // namespace kv
+
+int launch_attend_tc(const mrl_kv_cache* c, const mrl_attn& a, int sms, cudaStream_t s) {
+    kv::TcParams p;
+    p.c = c ? *c : mrl_kv_cache{};
+    p.a = a;
+    p.heads = (int)(c ? c->kv_heads : a.kv_heads);
+    p.group = (int)a.q_heads / p.heads;
+    p.causal = c ? 1 : (int)(a.causal != 0);
+    p.keys_inner = 0;
+    return c ? kv::dispatch<true>(p, c->head_dim, sms, s) : kv::dispatch<false>(p, a.head_dim, sms, s);
+}
+
+}  // namespace mrl

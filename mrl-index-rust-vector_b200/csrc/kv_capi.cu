@@ -211,6 +211,8 @@ int mrl_kv_attend(mrl_ctx* ctx, const mrl_kv_cache* kv, const mrl_attn* a) {
         if (a->layer >= kv->layers) return bad(ctx, "layer is not one of the cache's");
         if (int rc = check_attn(ctx, a, kv->kv_heads, kv->head_dim, true)) return rc;
         if (a->n_tokens == 0) return MRL_OK;
+        if (a->cu && a->max_rows * (a->q_heads / kv->kv_heads) > 64)
+            return done(ctx, mrl::launch_attend_tc(kv, *a, ctx->sms, ctx->stream), "mrl_kv_attend");
         // units of work of a launch are counted in 32 bits
         const uint64_t tiles = (uint64_t)a->n_tokens * (a->q_heads / kv->kv_heads) / 16 + std::min(a->n_seqs, mrl::kKvDecodeSeqs);
         if (tiles * kv->kv_heads * kv->max_pages >= (1ull << 32)) return bad(ctx, "too many rows x pages for one call");
@@ -226,7 +228,9 @@ int mrl_window_attention(mrl_ctx* ctx, const mrl_attn* a) {
         if (!a) return bad(ctx, "args are NULL");
         if (int rc = check_attn(ctx, a, a->kv_heads, a->head_dim, false)) return rc;
         if (a->n_tokens == 0) return MRL_OK;
-        return done(ctx, mrl::launch_attend_simple(nullptr, *a, ctx->stream), "mrl_window_attention");
+        const int rc = mrl::launch_attend_tc(nullptr, *a, ctx->sms, ctx->stream);
+        if (rc < 0) return bad(ctx, "k or v has strides that a tensor map cannot describe");
+        return done(ctx, rc, "mrl_window_attention");
     });
 }
 

@@ -22,7 +22,7 @@ namespace kv {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr uint32_t kPolls = 1u << 22;  // of a wait for a page, each up to the hardware's own time limit
+constexpr long long kWaitClocks = 4000000000ll;  // a wait for a page gives up after about two seconds
 
 // Warps per CTA: each holds one page's K and V block, 128 KiB in all, enough in flight per SM to cover the
 // latency of HBM.
@@ -69,7 +69,8 @@ __device__ __forceinline__ void load_block(uint32_t dst, const void* src, uint32
                  : "memory");
 }
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
-    for (uint32_t i = 0; i < kPolls; ++i) {
+    long long start = 0;
+    for (uint32_t i = 1;; ++i) {
         uint32_t ok;
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
@@ -79,8 +80,11 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
             : "r"(bar), "r"(parity)
             : "memory");
         if (ok) return true;
+        if (i % 16 == 0) {
+            if (start == 0) start = clock64();
+            else if (clock64() - start > kWaitClocks) return false;
+        }
     }
-    return false;
 }
 // A team is `threads` threads of consecutive warps; one warp needs no barrier resource.
 __device__ __forceinline__ void team_sync(int team, int threads) {
@@ -294,7 +298,7 @@ template <class T, int D> __global__ void __launch_bounds__(kWarps<D> * 32, 1) d
     };
 
     // ---- the page after the current one: found early, its K and V loaded as their slots come free
-    Segment ns;
+    Segment ns{};
     long long npos = pos;
     int ni = 0, npage = -1, nindex = 0;
     float nks = 0.0f, nvs = 0.0f;
