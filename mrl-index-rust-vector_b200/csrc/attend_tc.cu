@@ -13,10 +13,9 @@
 // at most 2^8, well inside f16, and its rounding is relative either way.
 //
 // Roles: warps 0-3 and 4-7 softmax and epilogue of the tiles (they also load their rows of Q), warp 8
-// issues the products, warp 9 loads K and V by TMA (16-bit rows) or, over the cache, warps 9-12 bring the
-// int8 blocks in by bulk copies and widen them to f16 (exact) into the operand layout; the blocks' scales
-// go to S and P, which are f32 there. Every wait is bounded; when one runs out the kernel records it and
-// ends.
+// issues the products, warp 9 loads K and V by TMA (16-bit rows) or stages the cache's int8 blocks by bulk
+// copies, which warps 12-15 widen to f16 (exact) into the operand layout; the blocks' scales go to S and
+// P, which are f32 there. Every wait is bounded; when one runs out the kernel records it and ends.
 //
 // Bound by the tensor core and the exponentials together: per 128 x 128 x D tile pair 2 x 2 x 128 x 128 x D
 // products against 2 x 16384 exponentials at 16 per clock and SM.
@@ -35,6 +34,7 @@ constexpr int kKeys = 128;        // keys per step
 constexpr float kSlack = 8.0f;    // log2 by which a row's maximum may lead the one it subtracts
 constexpr float kScaleSlack = 64.0f;  // the same for V's scales over the cache (a factor)
 constexpr int kInfo = 8;          // steps of scales kept
+constexpr int kPolyOf = 8;        // of so many pairs of exponentials `poly` go to the FMA units
 
 // What a template instance is: D, two tiles or one, stages of K and V, and its threads.
 template <int D, bool PAGED> struct Shape {
@@ -46,7 +46,11 @@ template <int D, bool PAGED> struct Shape {
     static constexpr int slots = PAGED ? (D == 64 ? 8 : D == 128 ? 3 : 2) : 0;  // staged blocks
     static constexpr int seqs = !PAGED || D == 64 ? 512 : D == 128 ? 384 : 64;  // sequences per launch (their table is in shared memory)
     static constexpr int conv_warps = PAGED ? 4 : 0;
-    static constexpr int threads = (9 + (PAGED ? conv_warps : 1)) * 32;
+    static constexpr int threads = (12 + conv_warps) * 32;
+    // Registers: launched with 168 (128 over the cache) a thread, of which the two softmax warpgroups take
+    // more and the others give up as many: 8 x 208 + 4 x 88 = 12 x 168, 8 x 168 + 8 x 88 = 16 x 128.
+    static constexpr int regs_softmax = PAGED ? 168 : 208, regs_other = 88;
+    static constexpr int poly = 2;
     static constexpr int tmem_s = 0;                           // S (and P) columns of tile or buffer i at 128 i
     static constexpr int tmem_o = 256;                         // O columns of tile i at 256 + D i
     static constexpr size_t smem = 1024 + (size_t)tiles * q_bytes + 2 * stages * kv_bytes + (size_t)slots * block;
@@ -125,6 +129,63 @@ __device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t lbo, uint
           "=r"((r)[25]), "=r"((r)[26]), "=r"((r)[27]), "=r"((r)[28]), "=r"((r)[29]), "=r"((r)[30]), "=r"((r)[31])                        \
         : "r"(taddr)                                                                                                                     \
         : "memory")
+
+#define MRL_TC_ST32(taddr, r)                                                                                                            \
+    asm volatile(                                                                                                                        \
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "     \
+        "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),                                      \
+        "r"((r)[0]), "r"((r)[1]), "r"((r)[2]), "r"((r)[3]), "r"((r)[4]), "r"((r)[5]), "r"((r)[6]), "r"((r)[7]), "r"((r)[8]),             \
+        "r"((r)[9]), "r"((r)[10]), "r"((r)[11]), "r"((r)[12]), "r"((r)[13]), "r"((r)[14]), "r"((r)[15]), "r"((r)[16]), "r"((r)[17]),     \
+        "r"((r)[18]), "r"((r)[19]), "r"((r)[20]), "r"((r)[21]), "r"((r)[22]), "r"((r)[23]), "r"((r)[24]), "r"((r)[25]), "r"((r)[26]),    \
+        "r"((r)[27]), "r"((r)[28]), "r"((r)[29]), "r"((r)[30]), "r"((r)[31])                                                             \
+        : "memory")
+// The values of loads that a wait has covered are used after it, not before.
+template <int N> __device__ __forceinline__ void pin(uint32_t (&x)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+r"(x[i]));
+}
+template <int REGS> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS)); }
+template <int REGS> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS)); }
+
+// Two f32 operations at once.
+__device__ __forceinline__ uint64_t two(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void split(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// 2^x of two values on the FMA units instead of the exponential unit: x = n + f with n whole, f in
+// [-1/2, 1/2], 2^f by the degree-5 polynomial with the least largest relative error there (7.5e-8, found by
+// exchange), n added to the exponent. x in [-125, 126].
+__device__ __forceinline__ void ex2_poly(uint64_t x, float& a, float& b) {
+    const float big = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number, kept in the low bits
+    float x0, x1;
+    split(x, x0, x1);
+    x = two(fmaxf(x0, -125.0f), fmaxf(x1, -125.0f));
+    const uint64_t t = add2(x, two(big, big)), n = add2(t, two(-big, -big));
+    const uint64_t f = fma2(n, two(-1.0f, -1.0f), x);
+    uint64_t p = two(1.3276472454890609e-3f, 1.3276472454890609e-3f);
+    p = fma2(p, f, two(9.675540961325169e-3f, 9.675540961325169e-3f));
+    p = fma2(p, f, two(5.550713092088699e-2f, 5.550713092088699e-2f));
+    p = fma2(p, f, two(0.24022120237350464f, 0.24022120237350464f));
+    p = fma2(p, f, two(0.6931469440460205f, 0.6931469440460205f));
+    p = fma2(p, f, two(1.0000001192092896f, 1.0000001192092896f));
+    float p0, p1, t0, t1;
+    split(p, p0, p1);
+    split(t, t0, t1);
+    a = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
+    b = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
+}
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -231,12 +292,14 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
     __shared__ SeqItem info[S::seqs];
     __shared__ int seq_s[PAGED ? S::seqs : 1];
     __shared__ unsigned scan_s[32];
+    constexpr int SL = PAGED ? S::slots : 1;
     __shared__ uint64_t q_full[TILES], k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], s_full[2], p_full[2], o_full[TILES], o_free[TILES],
-        pv_done[2], code_full[PAGED ? S::slots : 1];
+        pv_done[2], code_full[SL], code_empty[SL];
     __shared__ uint32_t tmem_s;
     __shared__ volatile int failed;
     __shared__ float4 scales_s[kInfo];  // over the cache: K scales of a step's two pages, V scales
     __shared__ int present_s[kInfo];    // bit i: page i of the step exists
+    __shared__ int there_s[SL];         // the staged block exists
 
     const mrl_attn& a = pr.a;
     const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -246,22 +309,25 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
     if (tid == 0) {
         failed = 0;
         for (int i = 0; i < TILES; ++i) {
-            tc::mbar_init(&q_full[i], 128);
+            tc::mbar_init(&q_full[i], 4);
             tc::mbar_init(&o_full[i], 1);
-            tc::mbar_init(&o_free[i], 128);
+            tc::mbar_init(&o_free[i], 4);
         }
         for (int i = 0; i < ST; ++i) {
-            tc::mbar_init(&k_full[i], PAGED ? S::conv_warps : 1);
+            tc::mbar_init(&k_full[i], PAGED ? 4 : 1);
             tc::mbar_init(&k_empty[i], 1);
-            tc::mbar_init(&v_full[i], PAGED ? S::conv_warps : 1);
+            tc::mbar_init(&v_full[i], PAGED ? 4 : 1);
             tc::mbar_init(&v_empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
             tc::mbar_init(&s_full[i], 1);
-            tc::mbar_init(&p_full[i], 128);
+            tc::mbar_init(&p_full[i], 4);
             tc::mbar_init(&pv_done[i], 1);
         }
-        for (int i = 0; i < (PAGED ? S::slots : 1); ++i) tc::mbar_init(&code_full[i], 1);
+        for (int i = 0; i < SL; ++i) {
+            tc::mbar_init(&code_full[i], 1);
+            tc::mbar_init(&code_empty[i], 4);
+        }
         tc::fence_mbar_init();
     }
     if (warp == 8) {
@@ -344,6 +410,8 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
         return it;
     };
 
+    if (warp >= 8) fewer_registers<S::regs_other>();
+    else if (warp < 4 * TILES) more_registers<S::regs_softmax>();
     if (warp < 4 * TILES) {
         // ---- softmax and epilogue of tile `tile`: thread = row
         const int tile = warp >> 2, r = tid & 127;
@@ -393,7 +461,8 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                 *reinterpret_cast<uint4*>(q_tile + (i >> 3) * 16384 + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = x;
             }
             tc::fence_proxy_async_smem();
-            arrive(&q_full[tile]);
+            __syncwarp();
+            if (lane == 0) arrive(&q_full[tile]);
         };
         Item<TILES> it;
         if (blockIdx.x < items) {
@@ -425,32 +494,35 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                 if (PAGED) {
                     const float4 x = scales_s[step_no & (kInfo - 1)];
                     there = present_s[step_no & (kInfo - 1)];
-                    ka *= x.x;
-                    kb *= x.y;
+                    ka = fmaxf(ka * x.x, 1e-37f);  // of a page of zeros: a masked score stays -inf
+                    kb = fmaxf(kb * x.y, 1e-37f);
                     va = x.z;
                     vb = x.w;
                     full = full && there == 3;
                 }
-                // pass 1: the largest score
-                float top = -INFINITY;
+                uint32_t x[128];
+                MRL_TC_LD32(x, s_col);
+                MRL_TC_LD32(x + 32, s_col + 32);
+                MRL_TC_LD32(x + 64, s_col + 64);
+                MRL_TC_LD32(x + 96, s_col + 96);
+                tc::wait_ld();
+                pin(x);
+                if (!full) {
+                    // visible keys of this row, relative to the step: [0, head) and [lo, hi)
+                    const int head = span.head - key0, lo = span.lo - key0, hi = span.hi - key0;
 #pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    uint32_t x[32];
-                    MRL_TC_LD32(x, s_col + h * 32);
-                    tc::wait_ld();
-                    float mx = -INFINITY;
-                    if (full) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) mx = fmaxf(mx, __uint_as_float(x[j]));
-                    } else if (there >> (h >> 1) & 1) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            const int key = key0 + h * 32 + j;
-                            if (key < span.head || (key >= span.lo && key < span.hi)) mx = fmaxf(mx, __uint_as_float(x[j]));
-                        }
-                    }
-                    top = fmaxf(top, mx * (h < 2 ? ka : kb));
+                    for (int j = 0; j < 128; ++j)
+                        if (!(j < head || (j >= lo && j < hi)) || (PAGED && !(there >> (j >> 6) & 1))) x[j] = 0xff800000u;
                 }
+                float mx[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) mx[j] = __uint_as_float(x[16 * j]);
+#pragma unroll
+                for (int i = 1; i < 16; ++i)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) mx[j] = fmaxf(mx[j], __uint_as_float(x[16 * j + i]));
+                const float top_a = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), top_b = fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7]));
+                const float top = fmaxf(top_a * ka, top_b * kb);
                 // the maximum that is subtracted, and V's scale unit, move rarely
                 float keep = 1.0f;
                 const float vmax = fmaxf(va, vb);
@@ -487,35 +559,42 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                     va = vref > 0.0f ? va / vref : 0.0f;
                     vb = vref > 0.0f ? vb / vref : 0.0f;
                 }
-                // pass 2: P over S; its first half goes where scores already read were
+                // P over S. A masked score is -inf. Over the cache P carries V's scale, put into the exponent and
+                // taken out of the sum again; below 2^-24 of the unit it would leave f16 anyway.
                 const float z = m == -INFINITY ? 0.0f : -m;
+                if (PAGED) {
+                    va = fmaxf(va, 5.9604645e-8f);
+                    vb = fmaxf(vb, 5.9604645e-8f);
+                }
 #pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    uint32_t x[32];
-                    MRL_TC_LD32(x, s_col + h * 32);
-                    tc::wait_ld();
-                    const float k = h < 2 ? ka : kb, v = h < 2 ? va : vb;
-                    uint32_t y[16];
-                    float sum = 0.0f;
+                for (int h = 0; h < 2; ++h) {
+                    const float k = h ? kb : ka, zz = PAGED ? z + __log2f(h ? vb : va) : z;
+                    const uint64_t k2 = two(k, k), z2 = two(zz, zz);
+                    uint64_t sum = 0;
+                    uint32_t y[32];
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        float e0 = ex2(fmaf(__uint_as_float(x[j]), k, z)), e1 = ex2(fmaf(__uint_as_float(x[j + 1]), k, z));
-                        if (!full) {
-                            const int key = key0 + h * 32 + j;
-                            const bool ok = there >> (h >> 1) & 1;
-                            if (!ok || !(key < span.head || (key >= span.lo && key < span.hi))) e0 = 0.0f;
-                            if (!ok || !(key + 1 < span.head || (key + 1 >= span.lo && key + 1 < span.hi))) e1 = 0.0f;
+                    for (int j = 0; j < 32; ++j) {
+                        const uint64_t e = fma2(two(__uint_as_float(x[64 * h + 2 * j]), __uint_as_float(x[64 * h + 2 * j + 1])), k2, z2);
+                        float e0, e1;
+                        if (full && j % kPolyOf < S::poly) {
+                            ex2_poly(e, e0, e1);
+                        } else {
+                            split(e, e0, e1);
+                            e0 = ex2(e0);
+                            e1 = ex2(e1);
                         }
-                        sum += e0 + e1;
-                        if (PAGED) e0 *= v, e1 *= v;
-                        y[j >> 1] = pack16<kBf>(e0, e1);
+                        sum = add2(sum, two(e0, e1));
+                        y[j] = pack16<kBf>(e0, e1);
                     }
-                    l += sum;
-                    TC_ST16(s_col + h * 16, y);
+                    float s0, s1;
+                    split(sum, s0, s1);
+                    l += PAGED ? (s0 + s1) / (h ? vb : va) : s0 + s1;
+                    MRL_TC_ST32(s_col + h * 32, y);
                 }
                 tc::wait_st();
                 tc::fence_before();
-                arrive(&p_full[buf]);
+                __syncwarp();
+                if (lane == 0) arrive(&p_full[buf]);
                 ++used;
             }
             // the next item's Q: this one's last S is done, nothing reads Q any more
@@ -541,7 +620,8 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                     tc::wait_ld();
                     if (j == D / 32 - 1) {
                         tc::fence_before();
-                        arrive(&o_free[tile]);
+                        __syncwarp();
+                        if (lane == 0) arrive(&o_free[tile]);
                     }
 #pragma unroll
                     for (int k = 0; k < 32; k += 8) {
@@ -693,118 +773,97 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                 }
             }
         }
-    } else if (warp >= 9) {
-        // ---- K and V from the cache: blocks of codes staged by bulk copies, widened into the operands
+    } else if (warp == 9) {
+        // ---- the cache's blocks in order, per step K of page 0 and 1, then V of page 0 and 1: block j goes to
+        // staging slot j % slots
+        if (lane == 0) {
+            const mrl_kv_cache& c = pr.c;
+            int block = 0, step_no = 0;
+            bool ok = true;
+            for (unsigned i = blockIdx.x; i < items && ok && !failed; i += gridDim.x) {
+                const Item<TILES> it = item_at(i);
+                const int32_t* table = c.tables + (size_t)seq_s[it.b] * c.max_pages;
+                auto page_of = [&](int index) {
+                    const int page = index * kPage < it.len ? table[index] : -1;
+                    return page >= 0 && page < (int)c.pages ? page : -1;
+                };
+                int s = it.begin();
+                int pages[2] = {-1, -1};
+                if (s < it.all.hi) pages[0] = page_of(2 * s), pages[1] = page_of(2 * s + 1);
+                for (; s < it.all.hi && ok; ++step_no) {
+                    const int p0 = pages[0], p1 = pages[1];
+                    s = it.next(s);
+                    if (s < it.all.hi) pages[0] = page_of(2 * s), pages[1] = page_of(2 * s + 1);  // read while this step's copies are queued
+                    float4 sc = make_float4(0, 0, 0, 0);
+                    const size_t b0 = block_index(c, a.layer, max(p0, 0), 0, it.head), b1 = block_index(c, a.layer, max(p1, 0), 0, it.head);
+                    if (p0 >= 0) sc.x = c.scales[b0], sc.z = c.scales[b0 + c.kv_heads];
+                    if (p1 >= 0) sc.y = c.scales[b1], sc.w = c.scales[b1 + c.kv_heads];
+                    for (int part = 0; part < 4; ++part, ++block) {
+                        const int slot = block % SL;
+                        ok = wait(&code_empty[slot], ((uint32_t)(block / SL) & 1) ^ 1, &failed);
+                        if (!ok) break;
+                        const bool have = (part & 1 ? p1 : p0) >= 0;
+                        there_s[slot] = have;
+                        if (part == 0) {
+                            // read by the softmax of a step at most stages + 2 steps behind this one
+                            scales_s[step_no & (kInfo - 1)] = sc;
+                            present_s[step_no & (kInfo - 1)] = (p0 >= 0 ? 1 : 0) | (p1 >= 0 ? 2 : 0);
+                        }
+                        if (have) {
+                            const size_t from = (part & 1 ? b1 : b0) + (part >> 1) * c.kv_heads;
+                            expect(&code_full[slot], S::block);
+                            bulk(tc::smem_u32(stage_s + (size_t)slot * S::block), c.codes + from * (size_t)S::block, S::block, &code_full[slot]);
+                        } else {
+                            arrive(&code_full[slot]);
+                        }
+                    }
+                }
+            }
+        }
+    } else if (warp >= 12) {
+        // ---- codes to f16 operands
         constexpr int kConv = S::conv_warps * 32;
-        const int ct = tid - 9 * 32;
-        const mrl_kv_cache& c = pr.c;
-        // Blocks in order: per step K of page 0 and 1, then V of page 0 and 1; block j of the run is staged in
-        // slot j % slots. Thread 0 looks them up and starts the copies, `slots` ahead.
-        struct Cursor {
-            unsigned i;
-            Item<TILES> it;
-            int s;
-        };
-        Cursor cur;
-        int queued = 0, q_step = 0;
-        __shared__ int there_s[PAGED ? S::slots : 1];
-        auto open = [&](Cursor& x) {  // the first item from x.i on that has steps
-            while (x.i < items) {
-                x.it = item_at(x.i);
-                x.s = x.it.begin();
-                if (x.s < x.it.all.hi) return true;
-                x.i += gridDim.x;
-            }
-            return false;
-        };
-        cur.i = blockIdx.x;
-        bool more = open(cur);
-        Cursor ahead = cur;
-        bool ahead_more = more;
-        int ahead_part = 0;
-        float sc[4] = {0, 0, 0, 0};
-        int pages[2] = {-1, -1};
-        auto queue = [&]() {  // thread 0: the next block's copy
-            if (!ahead_more) return;
-            const int slot = queued % S::slots;
-            if (ahead_part == 0) {
-                for (int k = 0; k < 2; ++k) {
-                    const int index = ahead.s * 2 + k;
-                    int page = -1;
-                    if (index * kPage < ahead.it.len) page = c.tables[(size_t)seq_s[ahead.it.b] * c.max_pages + index];
-                    pages[k] = page >= 0 && page < (int)c.pages ? page : -1;
-                }
-                for (int k = 0; k < 2; ++k)
-                    for (int w = 0; w < 2; ++w) sc[w * 2 + k] = pages[k] >= 0 ? c.scales[block_index(c, a.layer, pages[k], w, ahead.it.head)] : 0.0f;
-            }
-            const int page = pages[ahead_part & 1], which = ahead_part >> 1;
-            there_s[slot] = page >= 0;
-            if (page >= 0) {
-                expect(&code_full[slot], S::block);
-                bulk(tc::smem_u32(stage_s + (size_t)slot * S::block), c.codes + block_index(c, a.layer, page, which, ahead.it.head) * (size_t)S::block, S::block,
-                     &code_full[slot]);
-            } else {
-                arrive(&code_full[slot]);
-            }
-            if (ahead_part == 0) {
-                // steps of scales are read until their softmax is done, at most stages + 2 steps behind
-                scales_s[q_step & (kInfo - 1)] = make_float4(sc[0], sc[1], sc[2], sc[3]);
-                present_s[q_step & (kInfo - 1)] = (pages[0] >= 0 ? 1 : 0) | (pages[1] >= 0 ? 2 : 0);
-            }
-            ++queued;
-            if (++ahead_part == 4) {
-                ahead_part = 0;
-                ++q_step;
-                ahead.s = ahead.it.next(ahead.s);
-                if (ahead.s >= ahead.it.all.hi) {
-                    ahead.i += gridDim.x;
-                    ahead_more = open(ahead);
-                }
-            }
-        };
-        if (ct == 0)
-            for (int j = 0; j < S::slots; ++j) queue();
+        const int ct = tid - 12 * 32;
         int step_no = 0, block = 0;
         bool ok = true;
-        while (more && ok && !failed) {
-            const int stage = step_no % ST;
-            const uint32_t par = (uint32_t)(step_no / ST) & 1;
-            for (int part = 0; part < 4 && ok; ++part, ++block) {
-                const int slot = block % S::slots, half = part & 1;
-                const bool is_v = part >= 2;
-                if (half == 0) ok = wait(is_v ? &v_empty[stage] : &k_empty[stage], par ^ 1, &failed);
-                ok = ok && wait(&code_full[slot], (uint32_t)(block / S::slots) & 1, &failed);
-                if (!ok) break;
-                const bool have = there_s[slot] != 0;
-                const unsigned char* src = stage_s + (size_t)slot * S::block;
-                unsigned char* dst = is_v ? v_s + (size_t)stage * S::kv_bytes + half * (D * 128) : k_s + (size_t)stage * S::kv_bytes;
-                // 16 codes a thread and turn: row of 64 bytes -> 128-byte row, two 16-byte chunks
+        for (unsigned i = blockIdx.x; i < items && ok && !failed; i += gridDim.x) {
+            const Item<TILES> it = item_at(i);
+            for (int s = it.begin(); s < it.all.hi && ok; s = it.next(s), ++step_no) {
+                const int stage = step_no % ST;
+                const uint32_t par = (uint32_t)(step_no / ST) & 1;
+                for (int part = 0; part < 4 && ok; ++part, ++block) {
+                    const int slot = block % SL, half = part & 1;
+                    const bool is_v = part >= 2;
+                    if (half == 0) ok = wait(is_v ? &v_empty[stage] : &k_empty[stage], par ^ 1, &failed);
+                    ok = ok && wait(&code_full[slot], (uint32_t)(block / SL) & 1, &failed);
+                    if (!ok) break;
+                    const bool have = there_s[slot] != 0;
+                    const unsigned char* src = stage_s + (size_t)slot * S::block;
+                    unsigned char* dst = is_v ? v_s + (size_t)stage * S::kv_bytes + half * (D * 128) : k_s + (size_t)stage * S::kv_bytes;
+                    // 16 codes a thread and turn: row of 64 bytes -> 128-byte row, two 16-byte chunks
 #pragma unroll
-                for (int x = 0; x < S::block / 16 / kConv; ++x) {
-                    const int u = x * kConv + ct, line = u >> 2, quarter = u & 3;
-                    uint4 w = make_uint4(0x0u, 0x0u, 0x0u, 0x0u);
-                    if (have) w = *reinterpret_cast<const uint4*>(src + line * 64 + quarter * 16);
-                    uint4 e0, e1;
-                    widen4(w.x, e0.x, e0.y);
-                    widen4(w.y, e0.z, e0.w);
-                    widen4(w.z, e1.x, e1.y);
-                    widen4(w.w, e1.z, e1.w);
-                    // K: line = 64 block + token, to row 64 half + token of its block; V: line = dim
-                    const int at = is_v ? line * 128 : (line >> 6) * 16384 + (half * 64 + (line & 63)) * 128;
-                    const int sw = line & 7;
-                    *reinterpret_cast<uint4*>(dst + at + (((2 * quarter) ^ sw) << 4)) = e0;
-                    *reinterpret_cast<uint4*>(dst + at + (((2 * quarter + 1) ^ sw) << 4)) = e1;
+                    for (int x = 0; x < S::block / 16 / kConv; ++x) {
+                        const int u = x * kConv + ct, line = u >> 2, quarter = u & 3;
+                        uint4 w = make_uint4(0, 0, 0, 0);
+                        if (have) w = *reinterpret_cast<const uint4*>(src + line * 64 + quarter * 16);
+                        uint4 e0, e1;
+                        widen4(w.x, e0.x, e0.y);
+                        widen4(w.y, e0.z, e0.w);
+                        widen4(w.z, e1.x, e1.y);
+                        widen4(w.w, e1.z, e1.w);
+                        // K: line = 64 block + token, to row 64 half + token of its block; V: line = dim
+                        const int at = is_v ? line * 128 : (line >> 6) * 16384 + (half * 64 + (line & 63)) * 128;
+                        const int sw = line & 7;
+                        *reinterpret_cast<uint4*>(dst + at + (((2 * quarter) ^ sw) << 4)) = e0;
+                        *reinterpret_cast<uint4*>(dst + at + (((2 * quarter + 1) ^ sw) << 4)) = e1;
+                    }
+                    tc::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        arrive(&code_empty[slot]);
+                        if (half == 1) arrive(is_v ? &v_full[stage] : &k_full[stage]);
+                    }
                 }
-                tc::fence_proxy_async_smem();
-                asm volatile("bar.sync 1, %0;" ::"n"(kConv) : "memory");  // the staged block is read
-                if (half == 1 && lane == 0) arrive(is_v ? &v_full[stage] : &k_full[stage]);
-                if (ct == 0) queue();
-            }
-            ++step_no;
-            cur.s = cur.it.next(cur.s);
-            if (cur.s >= cur.it.all.hi) {
-                cur.i += gridDim.x;
-                more = open(cur);
             }
         }
     }
