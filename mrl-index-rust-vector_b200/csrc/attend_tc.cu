@@ -20,6 +20,7 @@
 // Bound by the tensor core and the exponentials together: per 128 x 128 x D tile pair 2 x 2 x 128 x 128 x D
 // products against 2 x 16384 exponentials at 16 per clock and SM.
 #include <cuda.h>
+#include <type_traits>
 
 #include "kv.cuh"
 #include "umma.cuh"
@@ -112,11 +113,17 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
 __host__ __device__ constexpr uint32_t idesc_f16(int n, bool bf, bool mn) {
     return (1u << 4) | ((bf ? 1u : 0u) << 7) | ((bf ? 1u : 0u) << 10) | ((mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
 }
-// 128-byte swizzle: 8 rows of 128 bytes per 1024-byte atom, atoms `sbo` apart along the rows, and for a
-// B that is N-major, 64-wide column blocks `lbo` apart.
-__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-    return (uint64_t)((addr >> 4) & 0x3FFFu) | (uint64_t)((lbo >> 4) & 0x3FFFu) << 16 | (uint64_t)((sbo >> 4) & 0x3FFFu) << 32 | (uint64_t)1 << 46 |
-           (uint64_t)2 << 61;
+// Shared-memory descriptor of a 128-byte-swizzled operand: 8 rows of 128 bytes per 1024-byte atom, atoms 1024
+// bytes apart along the rows, and for a B that is N-major, 64-wide column blocks `lbo` apart. The low word
+// holds the address, so stepping along an operand is an addition to it.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);  // atom stride, version, 128-byte swizzle
+__device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t lbo) { return ((addr >> 4) & 0x3FFFu) | (lbo >> 4) << 16; }
+__device__ __forceinline__ uint64_t desc(uint32_t low) { return (uint64_t)kDescHigh << 32 | low; }
+// The first active lane of a converged warp.
+__device__ __forceinline__ bool elect() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
 }
 
 #define MRL_TC_LD32(r, taddr)                                                                                                            \
@@ -566,31 +573,35 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                     va = fmaxf(va, 5.9604645e-8f);
                     vb = fmaxf(vb, 5.9604645e-8f);
                 }
+                auto make_p = [&](auto all) {  // all: no score is masked
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float k = h ? kb : ka, zz = PAGED ? z + __log2f(h ? vb : va) : z;
-                    const uint64_t k2 = two(k, k), z2 = two(zz, zz);
-                    uint64_t sum = 0;
-                    uint32_t y[32];
+                    for (int h = 0; h < 2; ++h) {
+                        const float k = h ? kb : ka, zz = PAGED ? z + __log2f(h ? vb : va) : z;
+                        const uint64_t k2 = two(k, k), z2 = two(zz, zz);
+                        uint64_t sum[4] = {0, 0, 0, 0};
+                        uint32_t y[32];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        const uint64_t e = fma2(two(__uint_as_float(x[64 * h + 2 * j]), __uint_as_float(x[64 * h + 2 * j + 1])), k2, z2);
-                        float e0, e1;
-                        if (full && j % kPolyOf < S::poly) {
-                            ex2_poly(e, e0, e1);
-                        } else {
-                            split(e, e0, e1);
-                            e0 = ex2(e0);
-                            e1 = ex2(e1);
+                        for (int j = 0; j < 32; ++j) {
+                            const uint64_t e = fma2(two(__uint_as_float(x[64 * h + 2 * j]), __uint_as_float(x[64 * h + 2 * j + 1])), k2, z2);
+                            float e0, e1;
+                            if (decltype(all)::value && j % kPolyOf < S::poly) {
+                                ex2_poly(e, e0, e1);
+                            } else {
+                                split(e, e0, e1);
+                                e0 = ex2(e0);
+                                e1 = ex2(e1);
+                            }
+                            sum[j & 3] = add2(sum[j & 3], two(e0, e1));
+                            y[j] = pack16<kBf>(e0, e1);
                         }
-                        sum = add2(sum, two(e0, e1));
-                        y[j] = pack16<kBf>(e0, e1);
+                        MRL_TC_ST32(s_col + h * 32, y);
+                        float s0, s1;
+                        split(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), s0, s1);
+                        l += PAGED ? (s0 + s1) / (h ? vb : va) : s0 + s1;
                     }
-                    float s0, s1;
-                    split(sum, s0, s1);
-                    l += PAGED ? (s0 + s1) / (h ? vb : va) : s0 + s1;
-                    MRL_TC_ST32(s_col + h * 32, y);
-                }
+                };
+                if (full) make_p(std::true_type{});
+                else make_p(std::false_type{});
                 tc::wait_st();
                 tc::fence_before();
                 __syncwarp();
@@ -651,29 +662,43 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
             }
         }
     } else if (warp == 8) {
-        // ---- the products: one thread
-        if (lane == 0) {
+        // ---- the products: the warp runs converged, so that what the instructions take sits in uniform registers,
+        // and one elected lane issues them
+        {
             constexpr uint32_t id_s = idesc_f16(kKeys, kBf, false), id_o = idesc_f16(D, kBf, !PAGED);
+            const uint32_t q_low = __shfl_sync(~0u, desc_low(tc::smem_u32(q_s), 16), 0), k_low = __shfl_sync(~0u, desc_low(tc::smem_u32(k_s), 16), 0),
+                           v_low = __shfl_sync(~0u, desc_low(tc::smem_u32(v_s), PAGED ? 16 : 16384), 0), tm = __shfl_sync(~0u, tmem, 0);
+            const bool leader = elect();
             uint32_t q_par = 0, p_par = 0, free_par = 0;
             int step_no = 0, used = 0;
             bool ok = true;
+            auto commit = [&](uint64_t* bar) {
+                if (leader) tc::mma_commit(bar);
+                __syncwarp();
+            };
             auto product_s = [&](int tile, int buf, int stage) {
-                const uint32_t q_addr = tc::smem_u32(q_s + (size_t)tile * S::q_bytes), k_addr = tc::smem_u32(k_s + (size_t)stage * S::kv_bytes);
+                const uint32_t q = q_low + (uint32_t)tile * (S::q_bytes >> 4), k = k_low + (uint32_t)stage * (S::kv_bytes >> 4),
+                               d = tm + S::tmem_s + (uint32_t)buf * 128;
+                if (leader) {
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const uint32_t off = (uint32_t)((k >> 2) * 16384 + (k & 3) * 32);
-                    mma_ss(tmem + S::tmem_s + buf * 128, desc_sw128(q_addr + off, 16, 1024), desc_sw128(k_addr + off, 16, 1024), id_s, k > 0);
+                    for (int i = 0; i < D / 16; ++i) {
+                        const uint32_t off = (uint32_t)((i >> 2) * 16384 + (i & 3) * 32) >> 4;
+                        mma_ss(d, desc(q + off), desc(k + off), id_s, i > 0);
+                    }
+                    tc::mma_commit(&s_full[buf]);
                 }
-                tc::mma_commit(&s_full[buf]);
+                __syncwarp();
             };
             auto product_o = [&](int tile, int buf, int stage, bool first) {
-                const uint32_t v_addr = tc::smem_u32(v_s + (size_t)stage * S::kv_bytes);
+                const uint32_t v = v_low + (uint32_t)stage * (S::kv_bytes >> 4), d = tm + S::tmem_o + (uint32_t)tile * D, p = tm + S::tmem_s + (uint32_t)buf * 128;
+                if (leader) {
 #pragma unroll
-                for (int k = 0; k < kKeys / 16; ++k) {
-                    const uint64_t b = PAGED ? desc_sw128(v_addr + (k >> 2) * (D * 128) + (k & 3) * 32, 16, 1024)
-                                             : desc_sw128(v_addr + k * 2048, 16384, 1024);
-                    mma_ts(tmem + S::tmem_o + tile * D, tmem + S::tmem_s + buf * 128 + k * 8, b, id_o, !(first && k == 0));
+                    for (int i = 0; i < kKeys / 16; ++i) {
+                        const uint32_t off = (uint32_t)(PAGED ? (i >> 2) * (D * 128) + (i & 3) * 32 : i * 2048) >> 4;
+                        mma_ts(d, p + i * 8, desc(v + off), id_o, !(first && i == 0));
+                    }
                 }
+                __syncwarp();
             };
             for (unsigned i = blockIdx.x; i < items && ok && !failed; i += gridDim.x) {
                 const Item<TILES> it = item_at(i);
@@ -692,7 +717,7 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                     p_par ^= 1u << pend_buf[t];
                     tc::fence_after();
                     product_o(t, pend_buf[t], stage, !begun[t]);
-                    if (SB == 2) tc::mma_commit(&pv_done[pend_buf[t]]);
+                    if (SB == 2) commit(&pv_done[pend_buf[t]]);
                     begun[t] = true;
                     return true;
                 };
@@ -717,7 +742,7 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                             // S of this step first: its buffer's last P went into O two steps ago
                             const int buf = used & 1;
                             product_s(t, buf, stage);
-                            tc::mma_commit(&k_empty[stage]);
+                            commit(&k_empty[stage]);
                             if (pend[t] >= 0) ok = finish(t);
                             pend[t] = step_no;
                             pend_buf[t] = buf;
@@ -735,16 +760,16 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                         }
                     }
                     if (!ok) break;
-                    if (SB == 1) tc::mma_commit(&k_empty[stage]);
-                    if (prev >= 0) tc::mma_commit(&v_empty[prev % ST]);
+                    if (SB == 1) commit(&k_empty[stage]);
+                    if (prev >= 0) commit(&v_empty[prev % ST]);
                     prev = step_no;
                 }
                 if (!ok) break;
                 for (int t = 0; t < TILES && ok; ++t) {
                     if (pend[t] >= 0) ok = finish(t);
-                    if (begun[t] && ok) tc::mma_commit(&o_full[t]);
+                    if (begun[t] && ok) commit(&o_full[t]);
                 }
-                if (prev >= 0 && ok) tc::mma_commit(&v_empty[prev % ST]);
+                if (prev >= 0 && ok) commit(&v_empty[prev % ST]);
             }
         }
     } else if constexpr (!PAGED) {
