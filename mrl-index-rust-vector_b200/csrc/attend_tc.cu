@@ -12,10 +12,10 @@
 // the sum l are kept relative to the stale one, which cancels in o = O / l, and O is rescaled rarely. P is
 // at most 2^8, well inside f16, and its rounding is relative either way.
 //
-// Roles: warps 0-3 and 4-7 softmax and epilogue of the tiles (they also load their rows of Q), warp 8
-// issues the products, warp 9 loads K and V by TMA (16-bit rows) or stages the cache's int8 blocks by bulk
-// copies, which warps 12-15 widen to f16 (exact) into the operand layout; the blocks' scales go to S and
-// P, which are f32 there. Every wait is bounded; when one runs out the kernel records it and ends.
+// Roles: warps 0-3 and 4-7 softmax and epilogue of the tiles, warp 8 issues the products, warp 9 loads Q, K
+// and V by TMA (16-bit rows) or stages the cache's int8 blocks by bulk copies, which warps 12-15 widen to
+// f16 (exact) into the operand layout (they also bring in Q, as f16); the blocks' scales go to S and P,
+// which are f32 there. Every wait is bounded; when one runs out the kernel records it and ends.
 //
 // Bound by the tensor core and the exponentials together: per 128 x 128 x D tile pair 2 x 2 x 128 x 128 x D
 // products against 2 x 16384 exponentials at 16 per clock and SM.
@@ -43,14 +43,16 @@ template <int D, bool PAGED> struct Shape {
     static constexpr int sbufs = D == 256 ? 2 : 1;
     static constexpr int stages = D == 64 ? 3 : D == 128 ? 2 : 1;
     static constexpr int q_bytes = 128 * D * 2, kv_bytes = kKeys * D * 2;
+    // A stage of K or V is handed over in pieces where there is only one: K by 64 dims, V by 64 keys.
+    static constexpr int k_parts = D == 256 ? 4 : 1, v_parts = D == 256 ? 2 : 1;
     static constexpr int block = kPage * D;  // codes of a page and head
     static constexpr int slots = PAGED ? (D == 64 ? 8 : D == 128 ? 3 : 2) : 0;  // staged blocks
-    static constexpr int seqs = !PAGED || D == 64 ? 512 : D == 128 ? 384 : 64;  // sequences per launch (their table is in shared memory)
+    static constexpr int seqs = !PAGED || D == 64 ? 512 : D == 128 ? 384 : 48;  // sequences per launch (their table is in shared memory)
     static constexpr int conv_warps = PAGED ? 4 : 0;
     static constexpr int threads = (12 + conv_warps) * 32;
     // Registers: launched with 168 (128 over the cache) a thread, of which the two softmax warpgroups take
-    // more and the others give up as many: 8 x 208 + 4 x 88 = 12 x 168, 8 x 168 + 8 x 88 = 16 x 128.
-    static constexpr int regs_softmax = PAGED ? 168 : 208, regs_other = 88;
+    // more and the others give up as many: 8 x 216 + 4 x 72 = 12 x 168, 8 x 184 + 8 x 72 = 16 x 128.
+    static constexpr int regs_softmax = PAGED ? 184 : 216, regs_other = 72;
     static constexpr int poly = 2;
     static constexpr int tmem_s = 0;                           // S (and P) columns of tile or buffer i at 128 i
     static constexpr int tmem_o = 256;                         // O columns of tile i at 256 + D i
@@ -66,7 +68,8 @@ struct TcParams {
     mrl_kv_cache c;
     mrl_attn a;
     int heads, group, tokens;  // kv heads, query heads per kv head, tokens per tile
-    int causal, keys_inner;    // keys_inner: the maps' second dimension is the row, not the head
+    int causal;
+    int inner_q, inner_k, inner_v;  // the map's second dimension is the row, not the head
 };
 
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
@@ -286,7 +289,8 @@ template <class T, int D> __device__ __noinline__ void slow_row(const mrl_attn& 
 
 template <class T, int D, bool PAGED>
 __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
-    tc_kernel(const __grid_constant__ TcParams pr, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
+    tc_kernel(const __grid_constant__ TcParams pr, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+              const __grid_constant__ CUtensorMap map_v) {
     using S = Shape<D, PAGED>;
     constexpr bool kBf = !PAGED && !__is_same(T, __half);  // operand type of the products
     constexpr int TILES = S::tiles, SB = S::sbufs, ST = S::stages;
@@ -300,13 +304,15 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
     __shared__ int seq_s[PAGED ? S::seqs : 1];
     __shared__ unsigned scan_s[32];
     constexpr int SL = PAGED ? S::slots : 1;
-    __shared__ uint64_t q_full[TILES], k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], s_full[2], p_full[2], o_full[TILES], o_free[TILES],
+    constexpr int KP = S::k_parts, VP = S::v_parts;
+    __shared__ uint64_t q_full[TILES], q_empty[TILES], k_full[ST * KP], k_empty[ST * KP], v_full[ST * VP], v_empty[ST * VP], s_full[2], p_full[2], o_full[TILES], o_free[TILES],
         pv_done[2], code_full[SL], code_empty[SL];
     __shared__ uint32_t tmem_s;
     __shared__ volatile int failed;
     __shared__ float4 scales_s[kInfo];  // over the cache: K scales of a step's two pages, V scales
     __shared__ int present_s[kInfo];    // bit i: page i of the step exists
     __shared__ int there_s[SL];         // the staged block exists
+    __shared__ uint8_t q_up_s[PAGED ? 2 * TILES * 128 : 1];  // over the cache: log2 + 127 of what each row of Q was divided by, of two items
 
     const mrl_attn& a = pr.a;
     const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -316,13 +322,16 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
     if (tid == 0) {
         failed = 0;
         for (int i = 0; i < TILES; ++i) {
-            tc::mbar_init(&q_full[i], 4);
+            tc::mbar_init(&q_full[i], PAGED ? 4 : 1);
+            tc::mbar_init(&q_empty[i], 1);
             tc::mbar_init(&o_full[i], 1);
             tc::mbar_init(&o_free[i], 4);
         }
-        for (int i = 0; i < ST; ++i) {
+        for (int i = 0; i < ST * KP; ++i) {
             tc::mbar_init(&k_full[i], PAGED ? 4 : 1);
             tc::mbar_init(&k_empty[i], 1);
+        }
+        for (int i = 0; i < ST * VP; ++i) {
             tc::mbar_init(&v_full[i], PAGED ? 4 : 1);
             tc::mbar_init(&v_empty[i], 1);
         }
@@ -423,61 +432,13 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
         // ---- softmax and epilogue of tile `tile`: thread = row
         const int tile = warp >> 2, r = tid & 127;
         const uint32_t lane_off = (uint32_t)(warp & 3) << 21;  // lane 32 (warp % 4) of tensor memory
-        unsigned char* q_tile = q_s + (size_t)tile * S::q_bytes;
-        const int tok = r / group, qh = r % group;
-        const bool row_used = tok < tokens;
+        const int tok = pr.inner_q ? r % tokens : r / group, qh = pr.inner_q ? r / tokens : r % group;
+        const bool row_used = r < tokens * group;
         uint32_t s_par = 0, o_par = 0;  // bit i: buffer i
-        int step_no = 0, used = 0;
-        float c0 = 0.0f;  // softmax scale in base 2 (over the cache with the row's power of two)
-        // This thread's row of Q for item `it` into shared memory.
-        auto load_q = [&](const Item<TILES>& it) {
-            const int f = it.first + tile * tokens + tok;
-            const bool in = row_used && f < it.m;
-            const T* p = static_cast<const T*>(a.q) + (int64_t)(it.row + f) * a.q_row + (int64_t)(it.head * group + qh) * a.q_head;
-            c0 = a.scale * kLog2e;
-            float down = 1.0f;
-            if (PAGED && !__is_same(T, __half)) {
-                // bf16 to f16 by way of [1, 2): see kv_decode.cu
-                float top = 0.0f;
-                if (in) {
-                    for (int i = 0; i < D / 8; ++i) {
-                        const uint4 x = *reinterpret_cast<const uint4*>(p + i * 8);
-                        const T* e = reinterpret_cast<const T*>(&x);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(to_f32<T>(e[j])));
-                    }
-                }
-                const uint32_t ex = __float_as_uint(top) >> 23;
-                if (ex > 0 && ex < 255) {
-                    const uint32_t up = min(ex, 253u);
-                    down = __uint_as_float((254u - up) << 23);
-                    c0 *= __uint_as_float(up << 23);
-                }
-            }
-#pragma unroll 4
-            for (int i = 0; i < D / 8; ++i) {
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (in) x = *reinterpret_cast<const uint4*>(p + i * 8);
-                if (PAGED && !__is_same(T, __half)) {
-                    const T* e = reinterpret_cast<const T*>(&x);
-                    uint32_t y[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) y[j] = pack16<false>(to_f32<T>(e[2 * j]) * down, to_f32<T>(e[2 * j + 1]) * down);
-                    x = make_uint4(y[0], y[1], y[2], y[3]);
-                }
-                *reinterpret_cast<uint4*>(q_tile + (i >> 3) * 16384 + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = x;
-            }
-            tc::fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) arrive(&q_full[tile]);
-        };
-        Item<TILES> it;
-        if (blockIdx.x < items) {
-            it = item_at(blockIdx.x);
-            if (it.st[tile].hi > 0) load_q(it);
-        }
+        int step_no = 0, used = 0, items_done = 0;
         for (unsigned i = blockIdx.x; i < items && !failed; i += gridDim.x) {
-            const float cur = c0;
+            const Item<TILES> it = item_at(i);
+            float cur = a.scale * kLog2e;
             const int f = it.first + tile * tokens, base = it.len - it.m;
             const Steps st = it.st[tile];
             const int p = base + f + tok;
@@ -494,6 +455,7 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                 tc::fence_after();
                 const uint32_t s_col = tmem + lane_off + S::tmem_s + buf * 128;
                 const int key0 = s * kKeys;
+                if (PAGED && !any) cur *= __uint_as_float((uint32_t)q_up_s[((items_done & 1) * TILES + tile) * 128 + r] << 23);
                 float ka = cur, kb = cur, va = 1.0f, vb = 1.0f;
                 bool full = key0 + kKeys <= it.len && (!causal || key0 + kKeys - 1 <= p_lo) &&
                             (window == 0 || key0 + kKeys <= sinks || (key0 > p_hi - window && (causal || key0 + kKeys - 1 < p_lo + window)));
@@ -517,9 +479,15 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                 if (!full) {
                     // visible keys of this row, relative to the step: [0, head) and [lo, hi)
                     const int head = span.head - key0, lo = span.lo - key0, hi = span.hi - key0;
+                    auto below = [](int k) { return k <= 0 ? 0u : k >= 32 ? ~0u : (1u << k) - 1u; };  // bits 0 .. k - 1
 #pragma unroll
-                    for (int j = 0; j < 128; ++j)
-                        if (!(j < head || (j >= lo && j < hi)) || (PAGED && !(there >> (j >> 6) & 1))) x[j] = 0xff800000u;
+                    for (int w = 0; w < 4; ++w) {
+                        uint32_t see = below(head - 32 * w) | (below(hi - 32 * w) & ~below(lo - 32 * w));
+                        if (PAGED && !(there >> (w >> 1) & 1)) see = 0;
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (!(see & (1u << j))) x[32 * w + j] = 0xff800000u;
+                    }
                 }
                 float mx[8];
 #pragma unroll
@@ -608,14 +576,9 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                 if (lane == 0) arrive(&p_full[buf]);
                 ++used;
             }
-            // the next item's Q: this one's last S is done, nothing reads Q any more
-            const Item<TILES> done = it;
-            if (i + gridDim.x < items) {
-                it = item_at(i + gridDim.x);
-                if (it.st[tile].hi > 0) load_q(it);
-            }
-            const bool in = row_used && done.first + tile * tokens + tok < done.m;
-            const int t_row = done.row + done.first + tile * tokens + tok, h = done.head * group + qh;
+            ++items_done;
+            const bool in = row_used && f + tok < it.m;
+            const int t_row = it.row + f + tok, h = it.head * group + qh;
             T* dst = static_cast<T*>(a.out) + (int64_t)t_row * a.o_row + (int64_t)h * a.o_head;
             float bad = 0.0f;
             if (any) {
@@ -657,7 +620,7 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                 while (again) {
                     const int who = __ffs((int)again) - 1;
                     again &= again - 1;
-                    slow_row<T, D>(a, done.row, done.len, __shfl_sync(~0u, p, who), __shfl_sync(~0u, t_row, who), __shfl_sync(~0u, h, who), done.head, causal);
+                    slow_row<T, D>(a, it.row, it.len, __shfl_sync(~0u, p, who), __shfl_sync(~0u, t_row, who), __shfl_sync(~0u, h, who), it.head, causal);
                 }
             }
         }
@@ -667,7 +630,7 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
         {
             constexpr uint32_t id_s = idesc_f16(kKeys, kBf, false), id_o = idesc_f16(D, kBf, !PAGED);
             const uint32_t q_low = __shfl_sync(~0u, desc_low(tc::smem_u32(q_s), 16), 0), k_low = __shfl_sync(~0u, desc_low(tc::smem_u32(k_s), 16), 0),
-                           v_low = __shfl_sync(~0u, desc_low(tc::smem_u32(v_s), PAGED ? 16 : 16384), 0), tm = __shfl_sync(~0u, tmem, 0);
+                           v_low = __shfl_sync(~0u, desc_low(tc::smem_u32(v_s), PAGED ? 16 : kKeys / VP * 128), 0), tm = __shfl_sync(~0u, tmem, 0);
             const bool leader = elect();
             uint32_t q_par = 0, p_par = 0, free_par = 0;
             int step_no = 0, used = 0;
@@ -676,29 +639,48 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                 if (leader) tc::mma_commit(bar);
                 __syncwarp();
             };
-            auto product_s = [&](int tile, int buf, int stage) {
+            auto product_s = [&](int tile, int buf, int stage, uint32_t k_par, bool last) {
                 const uint32_t q = q_low + (uint32_t)tile * (S::q_bytes >> 4), k = k_low + (uint32_t)stage * (S::kv_bytes >> 4),
                                d = tm + S::tmem_s + (uint32_t)buf * 128;
-                if (leader) {
+                constexpr int steps = D / 16 / KP;
 #pragma unroll
-                    for (int i = 0; i < D / 16; ++i) {
-                        const uint32_t off = (uint32_t)((i >> 2) * 16384 + (i & 3) * 32) >> 4;
-                        mma_ss(d, desc(q + off), desc(k + off), id_s, i > 0);
+                for (int part = 0; part < KP; ++part) {
+                    if (KP > 1) {
+                        if (!wait(&k_full[stage * KP + part], k_par, &failed)) return false;
+                        tc::fence_after();
                     }
-                    tc::mma_commit(&s_full[buf]);
+                    if (leader) {
+#pragma unroll
+                        for (int i = part * steps; i < (part + 1) * steps; ++i) {
+                            const uint32_t off = (uint32_t)((i >> 2) * 16384 + (i & 3) * 32) >> 4;
+                            mma_ss(d, desc(q + off), desc(k + off), id_s, i > 0);
+                        }
+                        if (KP > 1) tc::mma_commit(&k_empty[stage * KP + part]);
+                        if (part == KP - 1) tc::mma_commit(&s_full[buf]);
+                        if (part == KP - 1 && last) tc::mma_commit(&q_empty[tile]);
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
+                return true;
             };
-            auto product_o = [&](int tile, int buf, int stage, bool first) {
+            auto product_o = [&](int tile, int buf, int stage, uint32_t v_par, bool first) {
                 const uint32_t v = v_low + (uint32_t)stage * (S::kv_bytes >> 4), d = tm + S::tmem_o + (uint32_t)tile * D, p = tm + S::tmem_s + (uint32_t)buf * 128;
-                if (leader) {
+                constexpr int steps = kKeys / 16 / VP;
 #pragma unroll
-                    for (int i = 0; i < kKeys / 16; ++i) {
-                        const uint32_t off = (uint32_t)(PAGED ? (i >> 2) * (D * 128) + (i & 3) * 32 : i * 2048) >> 4;
-                        mma_ts(d, p + i * 8, desc(v + off), id_o, !(first && i == 0));
+                for (int part = 0; part < VP; ++part) {
+                    if (!wait(&v_full[stage * VP + part], v_par, &failed)) return false;
+                    tc::fence_after();
+                    if (leader) {
+#pragma unroll
+                        for (int i = part * steps; i < (part + 1) * steps; ++i) {
+                            const uint32_t off = (uint32_t)(PAGED ? (i >> 2) * (D * 128) + (i & 3) * 32 : part * (S::kv_bytes / VP) + (i % steps) * 2048) >> 4;
+                            mma_ts(d, p + i * 8, desc(v + off), id_o, !(first && i == 0));
+                        }
+                        if (VP > 1) tc::mma_commit(&v_empty[stage * VP + part]);
                     }
+                    __syncwarp();
                 }
-                __syncwarp();
+                return true;
             };
             for (unsigned i = blockIdx.x; i < items && ok && !failed; i += gridDim.x) {
                 const Item<TILES> it = item_at(i);
@@ -707,8 +689,7 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                 for (int t = 0; t < TILES; ++t) q_here[t] = begun[t] = false, pend[t] = -1, pend_buf[t] = 0;
                 // O += P V of tile t's pending step
                 auto finish = [&](int t) {
-                    const int no = pend[t], stage = no % ST;
-                    if (!wait(&v_full[stage], (uint32_t)(no / ST) & 1, &failed)) return false;
+                    const int no = pend[t];
                     if (!begun[t]) {  // the previous item's O has been read
                         if (!wait(&o_free[t], ((free_par >> t) & 1) ^ 1, &failed)) return false;
                         free_par ^= 1u << t;
@@ -716,7 +697,7 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                     if (!wait(&p_full[pend_buf[t]], (p_par >> pend_buf[t]) & 1, &failed)) return false;
                     p_par ^= 1u << pend_buf[t];
                     tc::fence_after();
-                    product_o(t, pend_buf[t], stage, !begun[t]);
+                    if (!product_o(t, pend_buf[t], no % ST, (uint32_t)(no / ST) & 1, !begun[t])) return false;
                     if (SB == 2) commit(&pv_done[pend_buf[t]]);
                     begun[t] = true;
                     return true;
@@ -724,11 +705,14 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                 int prev = -1;  // the step before, whose V the tiles may still need
                 for (int s = it.begin(); s < it.all.hi && ok; s = it.next(s), ++step_no) {
                     const int stage = step_no % ST;
-                    if (!wait(&k_full[stage], (uint32_t)(step_no / ST) & 1, &failed)) {
-                        ok = false;
-                        break;
+                    const uint32_t k_par = (uint32_t)(step_no / ST) & 1;
+                    if (KP == 1) {
+                        if (!wait(&k_full[stage], k_par, &failed)) {
+                            ok = false;
+                            break;
+                        }
+                        tc::fence_after();
                     }
-                    tc::fence_after();
                     for (int t = 0; t < TILES && ok; ++t) {
                         const bool has = it.st[t].has(s);
                         if (has && !q_here[t]) {
@@ -741,9 +725,8 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                         if (SB == 2) {
                             // S of this step first: its buffer's last P went into O two steps ago
                             const int buf = used & 1;
-                            product_s(t, buf, stage);
-                            commit(&k_empty[stage]);
-                            if (pend[t] >= 0) ok = finish(t);
+                            ok = product_s(t, buf, stage, k_par, s == it.st[t].hi - 1);
+                            if (ok && pend[t] >= 0) ok = finish(t);
                             pend[t] = step_no;
                             pend_buf[t] = buf;
                             ++used;
@@ -753,15 +736,15 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                                 pend[t] = -1;
                             }
                             if (has && ok) {
-                                product_s(t, t, stage);
+                                ok = product_s(t, t, stage, k_par, s == it.st[t].hi - 1);
                                 pend[t] = step_no;
                                 pend_buf[t] = t;
                             }
                         }
                     }
                     if (!ok) break;
-                    if (SB == 1) commit(&k_empty[stage]);
-                    if (prev >= 0) commit(&v_empty[prev % ST]);
+                    if (KP == 1) commit(&k_empty[stage]);
+                    if (VP == 1 && prev >= 0) commit(&v_empty[prev % ST]);
                     prev = step_no;
                 }
                 if (!ok) break;
@@ -769,32 +752,50 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                     if (pend[t] >= 0) ok = finish(t);
                     if (begun[t] && ok) commit(&o_full[t]);
                 }
-                if (prev >= 0 && ok) commit(&v_empty[prev % ST]);
+                if (VP == 1 && prev >= 0 && ok) commit(&v_empty[prev % ST]);
             }
         }
     } else if constexpr (!PAGED) {
-        // ---- K and V by TMA: boxes of 64 dims x 128 rows
+        // ---- Q, K and V by TMA: boxes of 64 dims x 128 rows (Q: a tile's tokens x heads, V: a part's keys)
         if (warp == 9 && lane == 0) {
             int step_no = 0;
+            uint32_t q_par = 0;
             bool ok = true;
             for (unsigned i = blockIdx.x; i < items && ok && !failed; i += gridDim.x) {
                 const Item<TILES> it = item_at(i);
+                for (int t = 0; t < TILES && ok; ++t) {
+                    if (it.st[t].hi == 0) continue;
+                    ok = wait(&q_empty[t], ((q_par >> t) & 1) ^ 1, &failed);
+                    if (!ok) break;
+                    q_par ^= 1u << t;
+                    expect(&q_full[t], (uint32_t)(tokens * group) * D * 2);
+                    const int row = it.row + it.first + t * tokens, h = it.head * group;
+                    for (int d = 0; d < D / 64; ++d)
+                        tma3(tc::smem_u32(q_s + (size_t)t * S::q_bytes + d * 16384), &map_q, d * 64, pr.inner_q ? row : h, pr.inner_q ? h : row, &q_full[t]);
+                }
                 for (int s = it.begin(); s < it.all.hi && ok; s = it.next(s), ++step_no) {
                     const int stage = step_no % ST;
                     const uint32_t par = (uint32_t)(step_no / ST) & 1;
                     const int row = it.row + s * kKeys;
-                    ok = wait(&k_empty[stage], par ^ 1, &failed);
-                    if (!ok) break;
-                    expect(&k_full[stage], S::kv_bytes);
-                    for (int d = 0; d < D / 64; ++d)
-                        tma3(tc::smem_u32(k_s + (size_t)stage * S::kv_bytes + d * 16384), &map_k, d * 64, pr.keys_inner & 1 ? row : it.head,
-                             pr.keys_inner & 1 ? it.head : row, &k_full[stage]);
-                    ok = wait(&v_empty[stage], par ^ 1, &failed);
-                    if (!ok) break;
-                    expect(&v_full[stage], S::kv_bytes);
-                    for (int d = 0; d < D / 64; ++d)
-                        tma3(tc::smem_u32(v_s + (size_t)stage * S::kv_bytes + d * 16384), &map_v, d * 64, pr.keys_inner & 2 ? row : it.head,
-                             pr.keys_inner & 2 ? it.head : row, &v_full[stage]);
+                    for (int part = 0; part < KP && ok; ++part) {
+                        uint64_t* bar = &k_full[stage * KP + part];
+                        ok = wait(&k_empty[stage * KP + part], par ^ 1, &failed);
+                        if (!ok) break;
+                        expect(bar, S::kv_bytes / KP);
+                        for (int d = part * (D / 64 / KP); d < (part + 1) * (D / 64 / KP); ++d)
+                            tma3(tc::smem_u32(k_s + (size_t)stage * S::kv_bytes + d * 16384), &map_k, d * 64, pr.inner_k ? row : it.head,
+                                 pr.inner_k ? it.head : row, bar);
+                    }
+                    for (int part = 0; part < VP && ok; ++part) {
+                        uint64_t* bar = &v_full[stage * VP + part];
+                        ok = wait(&v_empty[stage * VP + part], par ^ 1, &failed);
+                        if (!ok) break;
+                        expect(bar, S::kv_bytes / VP);
+                        const int v_row = row + part * (kKeys / VP);
+                        for (int d = 0; d < D / 64; ++d)
+                            tma3(tc::smem_u32(v_s + (size_t)stage * S::kv_bytes + part * (S::kv_bytes / VP) + d * (kKeys / VP * 128)), &map_v, d * 64,
+                                 pr.inner_v ? v_row : it.head, pr.inner_v ? it.head : v_row, bar);
+                    }
                 }
             }
         }
@@ -849,17 +850,63 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
         // ---- codes to f16 operands
         constexpr int kConv = S::conv_warps * 32;
         const int ct = tid - 12 * 32;
-        int step_no = 0, block = 0;
+        int step_no = 0, block = 0, items_done = 0;
+        uint32_t q_par = 0;
         bool ok = true;
-        for (unsigned i = blockIdx.x; i < items && ok && !failed; i += gridDim.x) {
+        for (unsigned i = blockIdx.x; i < items && ok && !failed; i += gridDim.x, ++items_done) {
             const Item<TILES> it = item_at(i);
+            for (int t = 0; t < TILES && ok; ++t) {
+                if (it.st[t].hi == 0) continue;
+                ok = wait(&q_empty[t], ((q_par >> t) & 1) ^ 1, &failed);
+                if (!ok) break;
+                q_par ^= 1u << t;
+                // D / 8 lanes to a row, 16 bytes each. bf16 has more range than f16: a row is brought to [1, 2) by a power
+                // of two, which goes to the softmax scale; what leaves f16's range below is 2^-24 of the row's largest.
+                constexpr int kLanes = D / 8, kRows = kConv / kLanes;
+#pragma unroll 4
+                for (int r0 = 0; r0 < 128; r0 += kRows) {
+                    const int r = r0 + ct / kLanes, col = ct % kLanes;
+                    const int f = it.first + t * tokens + r / group;
+                    const bool in = r < tokens * group && f < it.m;
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (in)
+                        x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (int64_t)(it.row + f) * a.q_row +
+                                                            (int64_t)(it.head * group + r % group) * a.q_head + col * 8);
+                    uint32_t up = 127;
+                    if (!__is_same(T, __half)) {
+                        const T* e = reinterpret_cast<const T*>(&x);
+                        float top = 0.0f, down = 1.0f;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(to_f32<T>(e[j])));
+#pragma unroll
+                        for (int d = kLanes / 2; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+                        const uint32_t ex = __float_as_uint(top) >> 23;
+                        if (ex > 0 && ex < 255) {
+                            up = min(ex, 253u);
+                            down = __uint_as_float((254u - up) << 23);
+                        }
+                        uint32_t y[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) y[j] = pack16<false>(to_f32<T>(e[2 * j]) * down, to_f32<T>(e[2 * j + 1]) * down);
+                        x = make_uint4(y[0], y[1], y[2], y[3]);
+                    }
+                    if (col == 0) q_up_s[((items_done & 1) * TILES + t) * 128 + r] = (uint8_t)up;
+                    *reinterpret_cast<uint4*>(q_s + (size_t)t * S::q_bytes + (col >> 3) * 16384 + r * 128 + (((col & 7) ^ (r & 7)) << 4)) = x;
+                }
+                tc::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) arrive(&q_full[t]);
+            }
             for (int s = it.begin(); s < it.all.hi && ok; s = it.next(s), ++step_no) {
                 const int stage = step_no % ST;
                 const uint32_t par = (uint32_t)(step_no / ST) & 1;
                 for (int part = 0; part < 4 && ok; ++part, ++block) {
                     const int slot = block % SL, half = part & 1;
                     const bool is_v = part >= 2;
-                    if (half == 0) ok = wait(is_v ? &v_empty[stage] : &k_empty[stage], par ^ 1, &failed);
+                    // a half of K lies in all of K's parts; V's parts, where there are two, are the halves
+                    if (!is_v && half == 0)
+                        for (int x = 0; x < KP; ++x) ok = ok && wait(&k_empty[stage * KP + x], par ^ 1, &failed);
+                    if (is_v && (VP == 2 || half == 0)) ok = ok && wait(&v_empty[stage * VP + (VP == 2 ? half : 0)], par ^ 1, &failed);
                     ok = ok && wait(&code_full[slot], (uint32_t)(block / SL) & 1, &failed);
                     if (!ok) break;
                     const bool have = there_s[slot] != 0;
@@ -886,7 +933,9 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                     __syncwarp();
                     if (lane == 0) {
                         arrive(&code_empty[slot]);
-                        if (half == 1) arrive(is_v ? &v_full[stage] : &k_full[stage]);
+                        if (!is_v && half == 1)
+                            for (int x = 0; x < KP; ++x) arrive(&k_full[stage * KP + x]);
+                        if (is_v && (VP == 2 || half == 1)) arrive(&v_full[stage * VP + (VP == 2 ? half : 0)]);
                     }
                 }
             }
@@ -910,15 +959,16 @@ Encode encoder() {
     return f;
 }
 
-// [rows][heads][D] 16-bit rows: dimensions D, then head and row in the order of their strides.
-bool make_map(CUtensorMap* map, const mrl_attn& a, const void* p, int64_t row, int64_t head, int d, int* keys_inner) {
-    const bool inner = a.n_tokens > 1 && (a.kv_heads == 1 ? false : row < head);
-    if (a.kv_heads == 1) head = d;
-    if (a.n_tokens == 1) row = (int64_t)a.kv_heads * d;
-    const cuuint64_t dims[3] = {(cuuint64_t)d, inner ? a.n_tokens : a.kv_heads, inner ? a.kv_heads : a.n_tokens};
-    const cuuint64_t strides[2] = {(cuuint64_t)(inner ? row : head) * 2, (cuuint64_t)(inner ? head : row) * 2};
-    const cuuint32_t box[3] = {64, inner ? (cuuint32_t)kKeys : 1u, inner ? 1u : (cuuint32_t)kKeys}, one[3] = {1, 1, 1};
-    *keys_inner = inner;
+// [rows][heads][D] 16-bit rows: dimensions D, then head and row in the order of their strides; boxes of 64
+// dims, `box_heads` heads and `box_rows` rows.
+bool make_map(CUtensorMap* map, const mrl_attn& a, const void* p, int64_t row, int64_t head, uint32_t heads, int d, int box_heads, int box_rows, int* inner) {
+    if (heads == 1) head = d;
+    if (a.n_tokens == 1) row = (int64_t)heads * head;
+    const bool in = heads > 1 && row < head;
+    const cuuint64_t dims[3] = {(cuuint64_t)d, in ? a.n_tokens : heads, in ? heads : a.n_tokens};
+    const cuuint64_t strides[2] = {(cuuint64_t)(in ? row : head) * 2, (cuuint64_t)(in ? head : row) * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)(in ? box_rows : box_heads), (cuuint32_t)(in ? box_heads : box_rows)}, one[3] = {1, 1, 1};
+    *inner = in;
     const Encode f = encoder();
     return f && f(map, a.dtype == MRL_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p), dims, strides, box,
                   one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -927,12 +977,11 @@ bool make_map(CUtensorMap* map, const mrl_attn& a, const void* p, int64_t row, i
 
 template <class T, int D, bool PAGED> int launch(TcParams p, int sms, cudaStream_t s) {
     using S = Shape<D, PAGED>;
-    CUtensorMap mk = {}, mv = {};
-    if (!PAGED) {
-        int ik, iv;
-        if (!make_map(&mk, p.a, p.a.k, p.a.k_row, p.a.k_head, D, &ik) || !make_map(&mv, p.a, p.a.v, p.a.v_row, p.a.v_head, D, &iv)) return -1;
-        p.keys_inner = ik | iv << 1;
-    }
+    CUtensorMap mq = {}, mk = {}, mv = {};
+    if (!PAGED && (!make_map(&mq, p.a, p.a.q, p.a.q_row, p.a.q_head, p.a.q_heads, D, p.group, 128 / p.group, &p.inner_q) ||
+                   !make_map(&mk, p.a, p.a.k, p.a.k_row, p.a.k_head, p.a.kv_heads, D, 1, kKeys, &p.inner_k) ||
+                   !make_map(&mv, p.a, p.a.v, p.a.v_row, p.a.v_head, p.a.kv_heads, D, 1, kKeys / S::v_parts, &p.inner_v)))
+        return -1;
     p.tokens = 128 / p.group;
     if (const cudaError_t e = cudaFuncSetAttribute(tc_kernel<T, D, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::smem)) return (int)e;
     const mrl_attn a = p.a;
@@ -942,7 +991,7 @@ template <class T, int D, bool PAGED> int launch(TcParams p, int sms, cudaStream
         p.a.cu = a.cu + at;
         // at most one part-filled item per sequence and head
         const uint64_t most = ((uint64_t)a.n_tokens / (S::tiles * p.tokens) + p.a.n_seqs) * p.heads;
-        tc_kernel<T, D, PAGED><<<(unsigned)(most < (uint64_t)sms ? most : sms), S::threads, S::smem, s>>>(p, mk, mv);
+        tc_kernel<T, D, PAGED><<<(unsigned)(most < (uint64_t)sms ? most : sms), S::threads, S::smem, s>>>(p, mq, mk, mv);
         if (const cudaError_t e = cudaGetLastError()) return (int)e;
     }
     return 0;
@@ -966,7 +1015,7 @@ int launch_attend_tc(const mrl_kv_cache* c, const mrl_attn& a, int sms, cudaStre
     p.heads = (int)(c ? c->kv_heads : a.kv_heads);
     p.group = (int)a.q_heads / p.heads;
     p.causal = c ? 1 : (int)(a.causal != 0);
-    p.keys_inner = 0;
+    p.inner_q = p.inner_k = p.inner_v = 0;
     return c ? kv::dispatch<true>(p, c->head_dim, sms, s) : kv::dispatch<false>(p, a.head_dim, sms, s);
 }
 
