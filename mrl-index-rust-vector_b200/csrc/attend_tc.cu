@@ -13,14 +13,13 @@
 // at most 2^8, well inside f16, and its rounding is relative either way.
 //
 // Roles: warps 0-3 and 4-7 softmax and epilogue of the tiles, warp 8 issues the products, warp 9 loads Q, K
-// and V by TMA (16-bit rows) or stages the cache's int8 blocks by bulk copies, which warps 12-15 widen to
-// f16 (exact) into the operand layout (they also bring in Q, as f16); the blocks' scales go to S and P,
-// which are f32 there. Every wait is bounded; when one runs out the kernel records it and ends.
+// and V by TMA (16-bit rows); over the cache warp 9 copies blocks of codes that
+// a first launch has widened to f16 (exact) in the operand layout, once for all the tiles that read them, and
+// warps 10 and 11 bring in Q as f16; the blocks' scales go to S and P, which are f32 there. Every wait is bounded; when one runs out the kernel records it and ends.
 //
 // Bound by the tensor core and the exponentials together: per 128 x 128 x D tile pair 2 x 2 x 128 x 128 x D
 // products against 2 x 16384 exponentials at 16 per clock and SM.
 #include <cuda.h>
-#include <type_traits>
 
 #include "kv.cuh"
 #include "umma.cuh"
@@ -35,7 +34,6 @@ constexpr int kKeys = 128;        // keys per step
 constexpr float kSlack = 8.0f;    // log2 by which a row's maximum may lead the one it subtracts
 constexpr float kScaleSlack = 64.0f;  // the same for V's scales over the cache (a factor)
 constexpr int kInfo = 8;          // steps of scales kept
-constexpr int kPolyOf = 8;        // of so many pairs of exponentials `poly` go to the FMA units
 
 // What a template instance is: D, two tiles or one, stages of K and V, and its threads.
 template <int D, bool PAGED> struct Shape {
@@ -45,18 +43,15 @@ template <int D, bool PAGED> struct Shape {
     static constexpr int q_bytes = 128 * D * 2, kv_bytes = kKeys * D * 2;
     // A stage of K or V is handed over in pieces where there is only one: K by 64 dims, V by 64 keys.
     static constexpr int k_parts = D == 256 ? 4 : 1, v_parts = D == 256 ? 2 : 1;
-    static constexpr int block = kPage * D;  // codes of a page and head
-    static constexpr int slots = PAGED ? (D == 64 ? 8 : D == 128 ? 3 : 2) : 0;  // staged blocks
-    static constexpr int seqs = !PAGED || D == 64 ? 512 : D == 128 ? 384 : 48;  // sequences per launch (their table is in shared memory)
-    static constexpr int conv_warps = PAGED ? 4 : 0;
-    static constexpr int threads = (12 + conv_warps) * 32;
-    // Registers: launched with 168 (128 over the cache) a thread, of which the two softmax warpgroups take
-    // more and the others give up as many: 8 x 216 + 4 x 72 = 12 x 168, 8 x 184 + 8 x 72 = 16 x 128.
-    static constexpr int regs_softmax = PAGED ? 184 : 216, regs_other = 72;
-    static constexpr int poly = 2;
+    static constexpr int wide = kPage * D * 2;  // bytes of a page and head's K or V as f16
+    static constexpr int seqs = 512;  // sequences per launch (their table is in shared memory)
+    static constexpr int threads = 12 * 32;
+    // Registers: launched with 168 a thread, of which the two softmax warpgroups take more and the other gives up
+    // as many: 8 x 216 + 4 x 72 = 12 x 168.
+    static constexpr int regs_softmax = 216, regs_other = 72;
     static constexpr int tmem_s = 0;                           // S (and P) columns of tile or buffer i at 128 i
     static constexpr int tmem_o = 256;                         // O columns of tile i at 256 + D i
-    static constexpr size_t smem = 1024 + (size_t)tiles * q_bytes + 2 * stages * kv_bytes + (size_t)slots * block;
+    static constexpr size_t smem = 1024 + (size_t)tiles * q_bytes + 2 * stages * kv_bytes;
 };
 
 struct SeqItem {
@@ -70,6 +65,9 @@ struct TcParams {
     int heads, group, tokens;  // kv heads, query heads per kv head, tokens per tile
     int causal;
     int inner_q, inner_k, inner_v;  // the map's second dimension is the row, not the head
+    // over the cache: f16 image of the layer's pool, [pages][2][kv heads][wide], and a block of zeros. The image only
+    // ever holds codes, so pages of it that a step touches but no row sees are finite.
+    const unsigned char *wide, *zero;
 };
 
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
@@ -174,33 +172,15 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-// 2^x of two values on the FMA units instead of the exponential unit: x = n + f with n whole, f in
-// [-1/2, 1/2], 2^f by the degree-5 polynomial with the least largest relative error there (7.5e-8, found by
-// exchange), n added to the exponent. x in [-125, 126].
-__device__ __forceinline__ void ex2_poly(uint64_t x, float& a, float& b) {
-    const float big = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number, kept in the low bits
-    float x0, x1;
-    split(x, x0, x1);
-    x = two(fmaxf(x0, -125.0f), fmaxf(x1, -125.0f));
-    const uint64_t t = add2(x, two(big, big)), n = add2(t, two(-big, -big));
-    const uint64_t f = fma2(n, two(-1.0f, -1.0f), x);
-    uint64_t p = two(1.3276472454890609e-3f, 1.3276472454890609e-3f);
-    p = fma2(p, f, two(9.675540961325169e-3f, 9.675540961325169e-3f));
-    p = fma2(p, f, two(5.550713092088699e-2f, 5.550713092088699e-2f));
-    p = fma2(p, f, two(0.24022120237350464f, 0.24022120237350464f));
-    p = fma2(p, f, two(0.6931469440460205f, 0.6931469440460205f));
-    p = fma2(p, f, two(1.0000001192092896f, 1.0000001192092896f));
-    float p0, p1, t0, t1;
-    split(p, p0, p1);
-    split(t, t0, t1);
-    a = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
-    b = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
-}
-
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 template <bool BF> __device__ __forceinline__ uint32_t pack16(float a, float b) {
     uint32_t r;
@@ -299,19 +279,16 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
     unsigned char* q_s = smem;                                  // per tile [D/64][128 rows][128 B], swizzled
     unsigned char* k_s = q_s + (size_t)TILES * S::q_bytes;      // per stage [D/64][128 keys][128 B]
     unsigned char* v_s = k_s + (size_t)ST * S::kv_bytes;        // per stage the same, over the cache [2 pages][D][128 B]
-    unsigned char* stage_s = v_s + (size_t)ST * S::kv_bytes;    // codes
     __shared__ SeqItem info[S::seqs];
     __shared__ int seq_s[PAGED ? S::seqs : 1];
     __shared__ unsigned scan_s[32];
-    constexpr int SL = PAGED ? S::slots : 1;
     constexpr int KP = S::k_parts, VP = S::v_parts;
     __shared__ uint64_t q_full[TILES], q_empty[TILES], k_full[ST * KP], k_empty[ST * KP], v_full[ST * VP], v_empty[ST * VP], s_full[2], p_full[2], o_full[TILES], o_free[TILES],
-        pv_done[2], code_full[SL], code_empty[SL];
+        pv_done[2];
     __shared__ uint32_t tmem_s;
     __shared__ volatile int failed;
     __shared__ float4 scales_s[kInfo];  // over the cache: K scales of a step's two pages, V scales
     __shared__ int present_s[kInfo];    // bit i: page i of the step exists
-    __shared__ int there_s[SL];         // the staged block exists
     __shared__ uint8_t q_up_s[PAGED ? 2 * TILES * 128 : 1];  // over the cache: log2 + 127 of what each row of Q was divided by, of two items
 
     const mrl_attn& a = pr.a;
@@ -322,27 +299,23 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
     if (tid == 0) {
         failed = 0;
         for (int i = 0; i < TILES; ++i) {
-            tc::mbar_init(&q_full[i], PAGED ? 4 : 1);
+            tc::mbar_init(&q_full[i], PAGED ? 2 : 1);
             tc::mbar_init(&q_empty[i], 1);
             tc::mbar_init(&o_full[i], 1);
             tc::mbar_init(&o_free[i], 4);
         }
         for (int i = 0; i < ST * KP; ++i) {
-            tc::mbar_init(&k_full[i], PAGED ? 4 : 1);
+            tc::mbar_init(&k_full[i], 1);
             tc::mbar_init(&k_empty[i], 1);
         }
         for (int i = 0; i < ST * VP; ++i) {
-            tc::mbar_init(&v_full[i], PAGED ? 4 : 1);
+            tc::mbar_init(&v_full[i], 1);
             tc::mbar_init(&v_empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
             tc::mbar_init(&s_full[i], 1);
             tc::mbar_init(&p_full[i], 4);
             tc::mbar_init(&pv_done[i], 1);
-        }
-        for (int i = 0; i < SL; ++i) {
-            tc::mbar_init(&code_full[i], 1);
-            tc::mbar_init(&code_empty[i], 4);
         }
         tc::fence_mbar_init();
     }
@@ -455,7 +428,7 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                 tc::fence_after();
                 const uint32_t s_col = tmem + lane_off + S::tmem_s + buf * 128;
                 const int key0 = s * kKeys;
-                if (PAGED && !any) cur *= __uint_as_float((uint32_t)q_up_s[((items_done & 1) * TILES + tile) * 128 + r] << 23);
+                if (PAGED && !__is_same(T, __half) && !any) cur *= __uint_as_float((uint32_t)q_up_s[((items_done & 1) * TILES + tile) * 128 + r] << 23);
                 float ka = cur, kb = cur, va = 1.0f, vb = 1.0f;
                 bool full = key0 + kKeys <= it.len && (!causal || key0 + kKeys - 1 <= p_lo) &&
                             (window == 0 || key0 + kKeys <= sinks || (key0 > p_hi - window && (causal || key0 + kKeys - 1 < p_lo + window)));
@@ -493,9 +466,11 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) mx[j] = __uint_as_float(x[16 * j]);
 #pragma unroll
-                for (int i = 1; i < 16; ++i)
+                for (int i = 1; i < 15; i += 2)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) mx[j] = fmaxf(mx[j], __uint_as_float(x[16 * j + i]));
+                    for (int j = 0; j < 8; ++j) mx[j] = max3(mx[j], __uint_as_float(x[16 * j + i]), __uint_as_float(x[16 * j + i + 1]));
+#pragma unroll
+                for (int j = 0; j < 8; ++j) mx[j] = fmaxf(mx[j], __uint_as_float(x[16 * j + 15]));
                 const float top_a = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), top_b = fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7]));
                 const float top = fmaxf(top_a * ka, top_b * kb);
                 // the maximum that is subtracted, and V's scale unit, move rarely
@@ -541,35 +516,26 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                     va = fmaxf(va, 5.9604645e-8f);
                     vb = fmaxf(vb, 5.9604645e-8f);
                 }
-                auto make_p = [&](auto all) {  // all: no score is masked
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float k = h ? kb : ka, zz = PAGED ? z + __log2f(h ? vb : va) : z;
-                        const uint64_t k2 = two(k, k), z2 = two(zz, zz);
-                        uint64_t sum[4] = {0, 0, 0, 0};
-                        uint32_t y[32];
+                for (int h = 0; h < 2; ++h) {
+                    const float k = h ? kb : ka, zz = PAGED ? z + __log2f(h ? vb : va) : z;
+                    const uint64_t k2 = two(k, k), z2 = two(zz, zz);
+                    uint64_t sum[4] = {0, 0, 0, 0};
+                    uint32_t y[32];
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            const uint64_t e = fma2(two(__uint_as_float(x[64 * h + 2 * j]), __uint_as_float(x[64 * h + 2 * j + 1])), k2, z2);
-                            float e0, e1;
-                            if (decltype(all)::value && j % kPolyOf < S::poly) {
-                                ex2_poly(e, e0, e1);
-                            } else {
-                                split(e, e0, e1);
-                                e0 = ex2(e0);
-                                e1 = ex2(e1);
-                            }
-                            sum[j & 3] = add2(sum[j & 3], two(e0, e1));
-                            y[j] = pack16<kBf>(e0, e1);
-                        }
-                        MRL_TC_ST32(s_col + h * 32, y);
-                        float s0, s1;
-                        split(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), s0, s1);
-                        l += PAGED ? (s0 + s1) / (h ? vb : va) : s0 + s1;
+                    for (int j = 0; j < 32; ++j) {
+                        float e0, e1;
+                        split(fma2(two(__uint_as_float(x[64 * h + 2 * j]), __uint_as_float(x[64 * h + 2 * j + 1])), k2, z2), e0, e1);
+                        e0 = ex2(e0);
+                        e1 = ex2(e1);
+                        sum[j & 3] = add2(sum[j & 3], two(e0, e1));
+                        y[j] = pack16<kBf>(e0, e1);
                     }
-                };
-                if (full) make_p(std::true_type{});
-                else make_p(std::false_type{});
+                    MRL_TC_ST32(s_col + h * 32, y);
+                    float s0, s1;
+                    split(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), s0, s1);
+                    l += PAGED ? (s0 + s1) / (h ? vb : va) : s0 + s1;
+                }
                 tc::wait_st();
                 tc::fence_before();
                 __syncwarp();
@@ -685,8 +651,9 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
             for (unsigned i = blockIdx.x; i < items && ok && !failed; i += gridDim.x) {
                 const Item<TILES> it = item_at(i);
                 bool q_here[TILES], begun[TILES];
-                int pend[TILES], pend_buf[TILES];  // step whose P is to come
-                for (int t = 0; t < TILES; ++t) q_here[t] = begun[t] = false, pend[t] = -1, pend_buf[t] = 0;
+                int pend[TILES], pend_buf[TILES];  // step whose P is to come, -1: none
+#pragma unroll
+                for (int t = 0; t < TILES; ++t) q_here[t] = begun[t] = false, pend[t] = -1, pend_buf[t] = t;
                 // O += P V of tile t's pending step
                 auto finish = [&](int t) {
                     const int no = pend[t];
@@ -700,6 +667,15 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                     if (!product_o(t, pend_buf[t], no % ST, (uint32_t)(no / ST) & 1, !begun[t])) return false;
                     if (SB == 2) commit(&pv_done[pend_buf[t]]);
                     begun[t] = true;
+                    pend[t] = -1;
+                    return true;
+                };
+                auto begin_q = [&](int t) {
+                    if (q_here[t]) return true;
+                    if (!wait(&q_full[t], (q_par >> t) & 1, &failed)) return false;
+                    q_par ^= 1u << t;
+                    q_here[t] = true;
+                    tc::fence_after();
                     return true;
                 };
                 int prev = -1;  // the step before, whose V the tiles may still need
@@ -713,33 +689,23 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                         }
                         tc::fence_after();
                     }
-                    for (int t = 0; t < TILES && ok; ++t) {
-                        const bool has = it.st[t].has(s);
-                        if (has && !q_here[t]) {
-                            ok = wait(&q_full[t], (q_par >> t) & 1, &failed);
-                            if (!ok) break;
-                            q_par ^= 1u << t;
-                            q_here[t] = true;
-                            tc::fence_after();
-                        }
+#pragma unroll
+                    for (int t = 0; t < TILES; ++t) {
+                        if (!ok) continue;
+                        const bool has = it.st[t].has(s), last = s == it.st[t].hi - 1;
                         if (SB == 2) {
                             // S of this step first: its buffer's last P went into O two steps ago
                             const int buf = used & 1;
-                            ok = product_s(t, buf, stage, k_par, s == it.st[t].hi - 1);
+                            ok = begin_q(t) && product_s(t, buf, stage, k_par, last);
                             if (ok && pend[t] >= 0) ok = finish(t);
                             pend[t] = step_no;
                             pend_buf[t] = buf;
                             ++used;
                         } else {
-                            if (pend[t] >= 0) {
-                                ok = finish(t);
-                                pend[t] = -1;
-                            }
-                            if (has && ok) {
-                                ok = product_s(t, t, stage, k_par, s == it.st[t].hi - 1);
-                                pend[t] = step_no;
-                                pend_buf[t] = t;
-                            }
+                            if (pend[t] >= 0) ok = finish(t);
+                            if (!has || !ok) continue;
+                            ok = begin_q(t) && product_s(t, t, stage, k_par, last);
+                            pend[t] = step_no;
                         }
                     }
                     if (!ok) break;
@@ -748,8 +714,9 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                     prev = step_no;
                 }
                 if (!ok) break;
-                for (int t = 0; t < TILES && ok; ++t) {
-                    if (pend[t] >= 0) ok = finish(t);
+#pragma unroll
+                for (int t = 0; t < TILES; ++t) {
+                    if (pend[t] >= 0 && ok) ok = finish(t);
                     if (begun[t] && ok) commit(&o_full[t]);
                 }
                 if (VP == 1 && prev >= 0 && ok) commit(&v_empty[prev % ST]);
@@ -800,11 +767,10 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
             }
         }
     } else if (warp == 9) {
-        // ---- the cache's blocks in order, per step K of page 0 and 1, then V of page 0 and 1: block j goes to
-        // staging slot j % slots
+        // ---- K and V from the cache's f16 image, scales beside them
         if (lane == 0) {
             const mrl_kv_cache& c = pr.c;
-            int block = 0, step_no = 0;
+            int step_no = 0;
             bool ok = true;
             for (unsigned i = blockIdx.x; i < items && ok && !failed; i += gridDim.x) {
                 const Item<TILES> it = item_at(i);
@@ -813,137 +779,206 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                     const int page = index * kPage < it.len ? table[index] : -1;
                     return page >= 0 && page < (int)c.pages ? page : -1;
                 };
-                int s = it.begin();
-                int pages[2] = {-1, -1};
-                if (s < it.all.hi) pages[0] = page_of(2 * s), pages[1] = page_of(2 * s + 1);
+                auto scale_of = [&](int page, int which) { return page >= 0 ? c.scales[block_index(c, a.layer, page, which, it.head)] : 0.0f; };
+                // page numbers are looked up two steps early and scales one, so that neither is waited for
+                int s = it.begin(), s1 = it.next(s);
+                int p0 = -1, p1 = -1, n0 = -1, n1 = -1;
+                if (s < it.all.hi) p0 = page_of(2 * s), p1 = page_of(2 * s + 1);
+                if (s1 < it.all.hi) n0 = page_of(2 * s1), n1 = page_of(2 * s1 + 1);
+                float4 sc = make_float4(scale_of(p0, 0), scale_of(p1, 0), scale_of(p0, 1), scale_of(p1, 1));
                 for (; s < it.all.hi && ok; ++step_no) {
-                    const int p0 = pages[0], p1 = pages[1];
-                    s = it.next(s);
-                    if (s < it.all.hi) pages[0] = page_of(2 * s), pages[1] = page_of(2 * s + 1);  // read while this step's copies are queued
-                    float4 sc = make_float4(0, 0, 0, 0);
-                    const size_t b0 = block_index(c, a.layer, max(p0, 0), 0, it.head), b1 = block_index(c, a.layer, max(p1, 0), 0, it.head);
-                    if (p0 >= 0) sc.x = c.scales[b0], sc.z = c.scales[b0 + c.kv_heads];
-                    if (p1 >= 0) sc.y = c.scales[b1], sc.w = c.scales[b1 + c.kv_heads];
-                    for (int part = 0; part < 4; ++part, ++block) {
-                        const int slot = block % SL;
-                        ok = wait(&code_empty[slot], ((uint32_t)(block / SL) & 1) ^ 1, &failed);
+                    const int stage = step_no % ST;
+                    const uint32_t par = (uint32_t)(step_no / ST) & 1;
+                    auto image = [&](int page, int which) {
+                        return page >= 0 ? pr.wide + (((size_t)page * 2 + which) * c.kv_heads + it.head) * S::wide : pr.zero;
+                    };
+                    const unsigned char *w0 = image(p0, 0), *w1 = image(p1, 0);
+                    // read by the softmax of a step at most stages + 1 behind this one
+                    scales_s[step_no & (kInfo - 1)] = sc;
+                    present_s[step_no & (kInfo - 1)] = (p0 >= 0 ? 1 : 0) | (p1 >= 0 ? 2 : 0);
+                    for (int part = 0; part < KP && ok; ++part) {
+                        uint64_t* bar = &k_full[stage * KP + part];
+                        ok = wait(&k_empty[stage * KP + part], par ^ 1, &failed);
                         if (!ok) break;
-                        const bool have = (part & 1 ? p1 : p0) >= 0;
-                        there_s[slot] = have;
-                        if (part == 0) {
-                            // read by the softmax of a step at most stages + 2 steps behind this one
-                            scales_s[step_no & (kInfo - 1)] = sc;
-                            present_s[step_no & (kInfo - 1)] = (p0 >= 0 ? 1 : 0) | (p1 >= 0 ? 2 : 0);
-                        }
-                        if (have) {
-                            const size_t from = (part & 1 ? b1 : b0) + (part >> 1) * c.kv_heads;
-                            expect(&code_full[slot], S::block);
-                            bulk(tc::smem_u32(stage_s + (size_t)slot * S::block), c.codes + from * (size_t)S::block, S::block, &code_full[slot]);
-                        } else {
-                            arrive(&code_full[slot]);
+                        expect(bar, S::kv_bytes / KP);
+                        for (int d = part * (D / 64 / KP); d < (part + 1) * (D / 64 / KP); ++d) {
+                            const uint32_t to = tc::smem_u32(k_s + (size_t)stage * S::kv_bytes + d * 16384);
+                            bulk(to, w0 + d * 8192, 8192, bar);
+                            bulk(to + 8192, w1 + d * 8192, 8192, bar);
                         }
                     }
+                    for (int part = 0; part < VP && ok; ++part) {
+                        uint64_t* bar = &v_full[stage * VP + part];
+                        ok = wait(&v_empty[stage * VP + part], par ^ 1, &failed);
+                        if (!ok) break;
+                        expect(bar, S::kv_bytes / VP);
+                        const uint32_t to = tc::smem_u32(v_s + (size_t)stage * S::kv_bytes);
+                        if (part == 0) bulk(to, image(p0, 1), S::wide, bar);
+                        if (part == VP - 1) bulk(to + S::wide, image(p1, 1), S::wide, bar);
+                    }
+                    s = s1;
+                    s1 = it.next(s);
+                    p0 = n0;
+                    p1 = n1;
+                    sc = make_float4(scale_of(p0, 0), scale_of(p1, 0), scale_of(p0, 1), scale_of(p1, 1));
+                    n0 = n1 = -1;
+                    if (s1 < it.all.hi) n0 = page_of(2 * s1), n1 = page_of(2 * s1 + 1);
                 }
             }
         }
-    } else if (warp >= 12) {
-        // ---- codes to f16 operands
-        constexpr int kConv = S::conv_warps * 32;
-        const int ct = tid - 12 * 32;
-        int step_no = 0, block = 0, items_done = 0;
+    } else if (warp >= 10) {
+        // ---- Q of the cache's attention, as f16
+        constexpr int kConv = 64;
+        const int ct = tid - 10 * 32;
+        int items_done = 0;
         uint32_t q_par = 0;
         bool ok = true;
         for (unsigned i = blockIdx.x; i < items && ok && !failed; i += gridDim.x, ++items_done) {
             const Item<TILES> it = item_at(i);
-            for (int t = 0; t < TILES && ok; ++t) {
-                if (it.st[t].hi == 0) continue;
-                ok = wait(&q_empty[t], ((q_par >> t) & 1) ^ 1, &failed);
-                if (!ok) break;
-                q_par ^= 1u << t;
-                // D / 8 lanes to a row, 16 bytes each. bf16 has more range than f16: a row is brought to [1, 2) by a power
-                // of two, which goes to the softmax scale; what leaves f16's range below is 2^-24 of the row's largest.
-                constexpr int kLanes = D / 8, kRows = kConv / kLanes;
+            // D / 8 lanes to a row, 16 bytes each, copied to where the operand wants them, and bf16 made f16 there by
+            // the thread that copied it. bf16 has more range than f16: a row is brought to [1, 2) by a power of two,
+            // which goes to the softmax scale; what leaves f16's range below is 2^-24 of the row's largest.
+            constexpr int kLanes = D / 8, kRows = kConv / kLanes;
+            const int q_row = ct / kLanes, q_col = ct % kLanes;
+            auto q_at = [&](int t, int r) { return q_s + (size_t)t * S::q_bytes + (q_col >> 3) * 16384 + r * 128 + (((q_col & 7) ^ (r & 7)) << 4); };
+            auto copy_q = [&](int t) {
 #pragma unroll 4
-                for (int r0 = 0; r0 < 128; r0 += kRows) {
-                    const int r = r0 + ct / kLanes, col = ct % kLanes;
+                for (int r = q_row; r < 128; r += kRows) {
                     const int f = it.first + t * tokens + r / group;
                     const bool in = r < tokens * group && f < it.m;
-                    uint4 x = make_uint4(0, 0, 0, 0);
-                    if (in)
-                        x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (int64_t)(it.row + f) * a.q_row +
-                                                            (int64_t)(it.head * group + r % group) * a.q_head + col * 8);
+                    const T* from = static_cast<const T*>(a.q);
+                    if (in) from += (int64_t)(it.row + f) * a.q_row + (int64_t)(it.head * group + r % group) * a.q_head + q_col * 8;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tc::smem_u32(q_at(t, r))), "l"(from), "r"(in ? 16 : 0) : "memory");
+                }
+            };
+            auto finish_q = [&](int t) {
+#pragma unroll 2
+                for (int r = q_row; r < 128 && !__is_same(T, __half); r += kRows) {
+                    uint4* at = reinterpret_cast<uint4*>(q_at(t, r));
+                    uint4 x = *at;
+                    const T* e = reinterpret_cast<const T*>(&x);
+                    float top = 0.0f, down = 1.0f;
                     uint32_t up = 127;
-                    if (!__is_same(T, __half)) {
-                        const T* e = reinterpret_cast<const T*>(&x);
-                        float top = 0.0f, down = 1.0f;
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(to_f32<T>(e[j])));
+                    for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(to_f32<T>(e[j])));
 #pragma unroll
-                        for (int d = kLanes / 2; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-                        const uint32_t ex = __float_as_uint(top) >> 23;
-                        if (ex > 0 && ex < 255) {
-                            up = min(ex, 253u);
-                            down = __uint_as_float((254u - up) << 23);
-                        }
-                        uint32_t y[4];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) y[j] = pack16<false>(to_f32<T>(e[2 * j]) * down, to_f32<T>(e[2 * j + 1]) * down);
-                        x = make_uint4(y[0], y[1], y[2], y[3]);
+                    for (int d = kLanes / 2; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+                    const uint32_t ex = __float_as_uint(top) >> 23;
+                    if (ex > 0 && ex < 255) {
+                        up = min(ex, 253u);
+                        down = __uint_as_float((254u - up) << 23);
                     }
-                    if (col == 0) q_up_s[((items_done & 1) * TILES + t) * 128 + r] = (uint8_t)up;
-                    *reinterpret_cast<uint4*>(q_s + (size_t)t * S::q_bytes + (col >> 3) * 16384 + r * 128 + (((col & 7) ^ (r & 7)) << 4)) = x;
+                    uint32_t y[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) y[j] = pack16<false>(to_f32<T>(e[2 * j]) * down, to_f32<T>(e[2 * j + 1]) * down);
+                    *at = make_uint4(y[0], y[1], y[2], y[3]);
+                    if (q_col == 0) q_up_s[((items_done & 1) * TILES + t) * 128 + r] = (uint8_t)up;
                 }
                 tc::fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) arrive(&q_full[t]);
+            };
+            for (int t = 0; t < TILES && ok; ++t) {
+                if (it.st[t].hi == 0) continue;
+                ok = wait(&q_empty[t], ((q_par >> t) & 1) ^ 1, &failed);
+                q_par ^= 1u << t;
+                if (ok) copy_q(t);
             }
-            for (int s = it.begin(); s < it.all.hi && ok; s = it.next(s), ++step_no) {
-                const int stage = step_no % ST;
-                const uint32_t par = (uint32_t)(step_no / ST) & 1;
-                for (int part = 0; part < 4 && ok; ++part, ++block) {
-                    const int slot = block % SL, half = part & 1;
-                    const bool is_v = part >= 2;
-                    // a half of K lies in all of K's parts; V's parts, where there are two, are the halves
-                    if (!is_v && half == 0)
-                        for (int x = 0; x < KP; ++x) ok = ok && wait(&k_empty[stage * KP + x], par ^ 1, &failed);
-                    if (is_v && (VP == 2 || half == 0)) ok = ok && wait(&v_empty[stage * VP + (VP == 2 ? half : 0)], par ^ 1, &failed);
-                    ok = ok && wait(&code_full[slot], (uint32_t)(block / SL) & 1, &failed);
-                    if (!ok) break;
-                    const bool have = there_s[slot] != 0;
-                    const unsigned char* src = stage_s + (size_t)slot * S::block;
-                    unsigned char* dst = is_v ? v_s + (size_t)stage * S::kv_bytes + half * (D * 128) : k_s + (size_t)stage * S::kv_bytes;
-                    // 16 codes a thread and turn: row of 64 bytes -> 128-byte row, two 16-byte chunks
-#pragma unroll
-                    for (int x = 0; x < S::block / 16 / kConv; ++x) {
-                        const int u = x * kConv + ct, line = u >> 2, quarter = u & 3;
-                        uint4 w = make_uint4(0, 0, 0, 0);
-                        if (have) w = *reinterpret_cast<const uint4*>(src + line * 64 + quarter * 16);
-                        uint4 e0, e1;
-                        widen4(w.x, e0.x, e0.y);
-                        widen4(w.y, e0.z, e0.w);
-                        widen4(w.z, e1.x, e1.y);
-                        widen4(w.w, e1.z, e1.w);
-                        // K: line = 64 block + token, to row 64 half + token of its block; V: line = dim
-                        const int at = is_v ? line * 128 : (line >> 6) * 16384 + (half * 64 + (line & 63)) * 128;
-                        const int sw = line & 7;
-                        *reinterpret_cast<uint4*>(dst + at + (((2 * quarter) ^ sw) << 4)) = e0;
-                        *reinterpret_cast<uint4*>(dst + at + (((2 * quarter + 1) ^ sw) << 4)) = e1;
-                    }
-                    tc::fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) {
-                        arrive(&code_empty[slot]);
-                        if (!is_v && half == 1)
-                            for (int x = 0; x < KP; ++x) arrive(&k_full[stage * KP + x]);
-                        if (is_v && (VP == 2 || half == 1)) arrive(&v_full[stage * VP + (VP == 2 ? half : 0)]);
-                    }
-                }
-            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            for (int t = 0; t < TILES && ok; ++t)
+                if (it.st[t].hi > 0) finish_q(t);
         }
     }
     __syncthreads();
     if (warp == 8) tc::tmem_dealloc(tmem, 512);
     if (tid == 0 && failed && pr.c.status) atomicOr(pr.c.status, MRL_KV_TIMEOUT);
+}
+
+// The pages that the call's sequences see, codes to f16 in the operands' layout: every 64 codes of K (a
+// token's dims 64 i ..) or V (a dim's tokens) become a swizzled row of 128 bytes. A page that several
+// sequences share lies at the same index of their tables after a fork: the first of them widens it.
+// Bound by HBM: 1 byte read, 2 written per code.
+constexpr int kWidenThreads = 256, kWidenSeqs = 1024;
+template <int D> __global__ void __launch_bounds__(kWidenThreads) widen_kernel(mrl_kv_cache c, mrl_attn a, unsigned char* wide) {
+    __shared__ unsigned start[kWidenSeqs];
+    __shared__ unsigned scan_s[kWidenThreads / 32];
+    __shared__ int skip_s;
+    const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5, n = (int)a.n_seqs, window = (int)a.window, sinks = (int)a.sinks;
+    const Rows rows{a.seqs, a.cu, n, (int)a.n_tokens};
+    struct Seen {
+        int seq, head, lo, n;  // visible pages [0, head) and [lo, lo + n - head)
+    };
+    auto seen = [&](int b) {
+        const int seq = a.seqs[b], m = rows.end(b) - rows.begin(b);
+        Seen s{seq, 0, 0, 0};
+        if (seq < 0 || seq >= (int)c.max_seqs || m <= 0) return s;
+        const int len = min(max(c.lens[seq], 0), (int)c.max_pages * kPage);
+        const Span v = visible(max(len - m, 0), len, 1, window, sinks);  // the first row sees the earliest
+        s.lo = min(v.lo, len) / kPage;
+        s.head = min(pages_of(min(sinks, v.lo)), s.lo);
+        s.n = s.head + pages_of(len) - s.lo;
+        return s;
+    };
+    unsigned carry = 0;
+    for (int at = 0; at < n; at += kWidenThreads) {
+        const int b = at + tid;
+        const unsigned v = b < n ? (unsigned)seen(b).n : 0;
+        unsigned x = v;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const unsigned y = __shfl_up_sync(~0u, x, d);
+            if (lane >= d) x += y;
+        }
+        if (lane == 31) scan_s[warp] = x;
+        __syncthreads();
+        unsigned before = carry;
+        for (int w = 0; w < kWidenThreads / 32; ++w) {
+            if (w < warp) before += scan_s[w];
+            carry += scan_s[w];
+        }
+        if (b < n) start[b] = before + x - v;
+        __syncthreads();
+    }
+    const unsigned heads = 2 * c.kv_heads, units = carry * heads;  // one block of 64 x D codes each
+    for (unsigned u = blockIdx.x; u < units; u += gridDim.x) {
+        const unsigned p = u / heads, block = u % heads;
+        int lo = 0, hi = n;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (start[mid] <= p) lo = mid;
+            else hi = mid;
+        }
+        const Seen s = seen(lo);
+        const int i = (int)(p - start[lo]), index = i < s.head ? i : s.lo + i - s.head;
+        const int page = c.tables[(size_t)s.seq * c.max_pages + index];
+        if (page < 0 || page >= (int)c.pages) continue;
+        if (c.refs[page] > 1) {
+            __syncthreads();
+            if (tid == 0) skip_s = 0;
+            __syncthreads();
+            for (int b = tid; b < lo; b += kWidenThreads) {
+                const Seen o = seen(b);
+                const bool has = index < o.head || (index >= o.lo && index < o.lo + o.n - o.head);
+                if (has && c.tables[(size_t)o.seq * c.max_pages + index] == page) skip_s = 1;
+            }
+            __syncthreads();
+            if (skip_s) continue;
+        }
+        const uint4* src = reinterpret_cast<const uint4*>(c.codes + (block_index(c, a.layer, page, 0, 0) + block) * (size_t)(kPage * D));
+        unsigned char* dst = wide + ((size_t)page * heads + block) * (kPage * D * 2);
+#pragma unroll
+        for (int x = 0; x < kPage * D / 16 / kWidenThreads; ++x) {
+            const int k = x * kWidenThreads + tid, line = k >> 2, quarter = k & 3, sw = line & 7;
+            const uint4 w = src[k];
+            uint4 e0, e1;
+            widen4(w.x, e0.x, e0.y);
+            widen4(w.y, e0.z, e0.w);
+            widen4(w.z, e1.x, e1.y);
+            widen4(w.w, e1.z, e1.w);
+            *reinterpret_cast<uint4*>(dst + line * 128 + (((2 * quarter) ^ sw) << 4)) = e0;
+            *reinterpret_cast<uint4*>(dst + line * 128 + (((2 * quarter + 1) ^ sw) << 4)) = e1;
+        }
+    }
 }
 
 using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -989,6 +1024,10 @@ template <class T, int D, bool PAGED> int launch(TcParams p, int sms, cudaStream
         p.a.n_seqs = a.n_seqs - at < (uint32_t)S::seqs ? a.n_seqs - at : (uint32_t)S::seqs;
         p.a.seqs = a.seqs ? a.seqs + at : nullptr;
         p.a.cu = a.cu + at;
+        if (PAGED) {
+            widen_kernel<D><<<(unsigned)sms * 8, kWidenThreads, 0, s>>>(p.c, p.a, const_cast<unsigned char*>(p.wide));
+            if (const cudaError_t e = cudaGetLastError()) return (int)e;
+        }
         // at most one part-filled item per sequence and head
         const uint64_t most = ((uint64_t)a.n_tokens / (S::tiles * p.tokens) + p.a.n_seqs) * p.heads;
         tc_kernel<T, D, PAGED><<<(unsigned)(most < (uint64_t)sms ? most : sms), S::threads, S::smem, s>>>(p, mq, mk, mv);
@@ -1008,8 +1047,12 @@ template <bool PAGED> int dispatch(const TcParams& p, uint32_t d, int sms, cudaS
 }  // namespace
 }  // namespace kv
 
-int launch_attend_tc(const mrl_kv_cache* c, const mrl_attn& a, int sms, cudaStream_t s) {
+size_t kv_wide_bytes(const mrl_kv_cache& c) { return kKvZeroBytes + (size_t)c.pages * 2 * kv::page_bytes(c); }
+
+int launch_attend_tc(const mrl_kv_cache* c, const mrl_attn& a, int sms, void* wide, cudaStream_t s) {
     kv::TcParams p;
+    p.zero = static_cast<const unsigned char*>(wide);
+    p.wide = p.zero + kKvZeroBytes;
     p.c = c ? *c : mrl_kv_cache{};
     p.a = a;
     p.heads = (int)(c ? c->kv_heads : a.kv_heads);

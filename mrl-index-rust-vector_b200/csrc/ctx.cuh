@@ -11,8 +11,10 @@
 // different streams never share a buffer.
 struct mrl_kv_scratch {
     cudaStream_t stream = nullptr;
-    void* buf = nullptr;
+    void* buf = nullptr;    // working memory
     size_t bytes = 0;
+    void* image = nullptr;  // 16-bit image of a layer's pool
+    size_t image_bytes = 0;
     bool used = false;
 };
 

@@ -137,7 +137,9 @@ int launch_kv_read(const mrl_kv_cache& c, uint32_t layer, uint32_t dtype, void* 
 constexpr uint32_t kKvDecodeSeqs = 1024;
 size_t kv_decode_bytes(uint32_t head_dim, int sms);
 int launch_kv_decode(const mrl_kv_cache& c, const mrl_attn& a, int sms, void* scratch, unsigned* counters, cudaStream_t s);
-// Tensor-core attention: over the cache (c) or over the call's own k and v. -1: strides that a TMA map
-// cannot describe.
-int launch_attend_tc(const mrl_kv_cache* c, const mrl_attn& a, int sms, cudaStream_t s);
+// Tensor-core attention: over the cache (c; `wide` is kKvZeroBytes of zeros and room for a 16-bit image of one
+// layer's pool) or over the call's own k and v. -1: strides that a TMA map cannot describe.
+constexpr size_t kKvZeroBytes = 64 * 256 * 2;
+size_t kv_wide_bytes(const mrl_kv_cache& c);
+int launch_attend_tc(const mrl_kv_cache* c, const mrl_attn& a, int sms, void* wide, cudaStream_t s);
 }  // namespace mrl

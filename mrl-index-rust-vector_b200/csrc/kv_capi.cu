@@ -58,28 +58,47 @@ int check_rows16(mrl_ctx* ctx, const char* name, const void* p, int64_t row, int
     return MRL_OK;
 }
 
-// The scratch buffer of the context's current stream: counters in the first kCounterBytes (zero when a
-// buffer is made, and left zero by the kernels that use them), then at least `bytes` for the call.
-constexpr size_t kCounterBytes = 65536;
-int kv_scratch(mrl_ctx* ctx, size_t bytes, void** out, unsigned** counters = nullptr) {
-    bytes += kCounterBytes;
+// The scratch of the context's current stream.
+int kv_scratch_slot(mrl_ctx* ctx, mrl_kv_scratch** out) {
     mrl_kv_scratch* k = nullptr;
     for (mrl_kv_scratch& x : ctx->kv)
         if (x.used && x.stream == ctx->stream) k = &x;
     if (!k) {
         k = &ctx->kv[ctx->kv_next];
-        if (k->used) MRL_CUDA_TRY(ctx, cudaDeviceSynchronize());  // its old stream may still use the buffer
+        if (k->used) MRL_CUDA_TRY(ctx, cudaDeviceSynchronize());  // its old stream may still use the buffers
         ctx->kv_next = (ctx->kv_next + 1) % mrl_ctx::kKvStreams;
         k->stream = ctx->stream;
         k->used = true;
     }
-    if (k->bytes < bytes) {
-        size_t want = (bytes + (size_t)0xfffff) & ~(size_t)0xfffff;
-        if (int rc = ensure_buf(ctx, &k->buf, &k->bytes, want)) return rc;
-        MRL_CUDA_TRY(ctx, cudaMemsetAsync(k->buf, 0, k->bytes, ctx->stream));
-    }
+    *out = k;
+    return MRL_OK;
+}
+
+// A buffer of the scratch, at least `bytes` long and zero when it is made.
+int kv_grow(mrl_ctx* ctx, void** buf, size_t* have, size_t bytes) {
+    if (*have >= bytes) return MRL_OK;
+    if (int rc = ensure_buf(ctx, buf, have, (bytes + (size_t)0xfffff) & ~(size_t)0xfffff)) return rc;
+    MRL_CUDA_TRY(ctx, cudaMemsetAsync(*buf, 0, *have, ctx->stream));
+    return MRL_OK;
+}
+
+// `bytes` of working memory, and counters before it (zero; the kernels that use them leave them zero).
+constexpr size_t kCounterBytes = 65536;
+int kv_scratch(mrl_ctx* ctx, size_t bytes, void** out, unsigned** counters = nullptr) {
+    mrl_kv_scratch* k;
+    if (int rc = kv_scratch_slot(ctx, &k)) return rc;
+    if (int rc = kv_grow(ctx, &k->buf, &k->bytes, bytes + kCounterBytes)) return rc;
     *out = static_cast<char*>(k->buf) + kCounterBytes;
     if (counters) *counters = static_cast<unsigned*>(k->buf);
+    return MRL_OK;
+}
+
+// Room for a layer's pool as f16 (launch_attend_tc).
+int kv_image(mrl_ctx* ctx, size_t bytes, void** out) {
+    mrl_kv_scratch* k;
+    if (int rc = kv_scratch_slot(ctx, &k)) return rc;
+    if (int rc = kv_grow(ctx, &k->image, &k->image_bytes, bytes)) return rc;
+    *out = k->image;
     return MRL_OK;
 }
 
@@ -211,8 +230,11 @@ int mrl_kv_attend(mrl_ctx* ctx, const mrl_kv_cache* kv, const mrl_attn* a) {
         if (a->layer >= kv->layers) return bad(ctx, "layer is not one of the cache's");
         if (int rc = check_attn(ctx, a, kv->kv_heads, kv->head_dim, true)) return rc;
         if (a->n_tokens == 0) return MRL_OK;
-        if (a->cu && a->max_rows * (a->q_heads / kv->kv_heads) > 64)
-            return done(ctx, mrl::launch_attend_tc(kv, *a, ctx->sms, ctx->stream), "mrl_kv_attend");
+        if (a->cu && (uint64_t)a->max_rows * (a->q_heads / kv->kv_heads) > 64) {
+            void* wide;
+            if (int rc = kv_image(ctx, mrl::kv_wide_bytes(*kv), &wide)) return rc;
+            return done(ctx, mrl::launch_attend_tc(kv, *a, ctx->sms, wide, ctx->stream), "mrl_kv_attend");
+        }
         // units of work of a launch are counted in 32 bits
         const uint64_t tiles = (uint64_t)a->n_tokens * (a->q_heads / kv->kv_heads) / 16 + std::min(a->n_seqs, mrl::kKvDecodeSeqs);
         if (tiles * kv->kv_heads * kv->max_pages >= (1ull << 32)) return bad(ctx, "too many rows x pages for one call");
@@ -228,7 +250,7 @@ int mrl_window_attention(mrl_ctx* ctx, const mrl_attn* a) {
         if (!a) return bad(ctx, "args are NULL");
         if (int rc = check_attn(ctx, a, a->kv_heads, a->head_dim, false)) return rc;
         if (a->n_tokens == 0) return MRL_OK;
-        const int rc = mrl::launch_attend_tc(nullptr, *a, ctx->sms, ctx->stream);
+        const int rc = mrl::launch_attend_tc(nullptr, *a, ctx->sms, nullptr, ctx->stream);
         if (rc < 0) return bad(ctx, "k or v has strides that a tensor map cannot describe");
         return done(ctx, rc, "mrl_window_attention");
     });
