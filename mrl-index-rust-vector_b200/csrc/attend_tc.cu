@@ -35,6 +35,7 @@ constexpr float kSlack = 8.0f;    // log2 by which a row's maximum may lead the 
 constexpr float kScaleSlack = 64.0f;  // the same for V's scales over the cache (a factor)
 constexpr int kInfo = 8;          // steps of scales kept
 
+template <int D> constexpr int kWide = kPage * D * 2;  // bytes of a page and head's K or V as f16
 // What a template instance is: D, two tiles or one, stages of K and V, and its threads.
 template <int D, bool PAGED> struct Shape {
     static constexpr int tiles = D == 256 ? 1 : 2;
@@ -43,7 +44,6 @@ template <int D, bool PAGED> struct Shape {
     static constexpr int q_bytes = 128 * D * 2, kv_bytes = kKeys * D * 2;
     // A stage of K or V is handed over in pieces where there is only one: K by 64 dims, V by 64 keys.
     static constexpr int k_parts = D == 256 ? 4 : 1, v_parts = D == 256 ? 2 : 1;
-    static constexpr int wide = kPage * D * 2;  // bytes of a page and head's K or V as f16
     static constexpr int seqs = 512;  // sequences per launch (their table is in shared memory)
     static constexpr int threads = 12 * 32;
     // Registers: launched with 168 a thread, of which the two softmax warpgroups take more and the other gives up
@@ -790,7 +790,7 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                     const int stage = step_no % ST;
                     const uint32_t par = (uint32_t)(step_no / ST) & 1;
                     auto image = [&](int page, int which) {
-                        return page >= 0 ? pr.wide + (((size_t)page * 2 + which) * c.kv_heads + it.head) * S::wide : pr.zero;
+                        return page >= 0 ? pr.wide + (((size_t)page * 2 + which) * c.kv_heads + it.head) * kWide<D> : pr.zero;
                     };
                     const unsigned char *w0 = image(p0, 0), *w1 = image(p1, 0);
                     // read by the softmax of a step at most stages + 1 behind this one
@@ -813,8 +813,8 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                         if (!ok) break;
                         expect(bar, S::kv_bytes / VP);
                         const uint32_t to = tc::smem_u32(v_s + (size_t)stage * S::kv_bytes);
-                        if (part == 0) bulk(to, image(p0, 1), S::wide, bar);
-                        if (part == VP - 1) bulk(to + S::wide, image(p1, 1), S::wide, bar);
+                        if (part == 0) bulk(to, image(p0, 1), kWide<D>, bar);
+                        if (part == VP - 1) bulk(to + kWide<D>, image(p1, 1), kWide<D>, bar);
                     }
                     s = s1;
                     s1 = it.next(s);
@@ -1018,7 +1018,7 @@ template <class T, int D, bool PAGED> int launch(TcParams p, int sms, cudaStream
                    !make_map(&mv, p.a, p.a.v, p.a.v_row, p.a.v_head, p.a.kv_heads, D, 1, kKeys / S::v_parts, &p.inner_v)))
         return -1;
     p.tokens = 128 / p.group;
-    if (const cudaError_t e = cudaFuncSetAttribute(tc_kernel<T, D, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::smem)) return (int)e;
+    if (const cudaError_t e = allow_smem<tc_kernel<T, D, PAGED>>((int)S::smem)) return (int)e;
     const mrl_attn a = p.a;
     for (uint32_t at = 0; at < a.n_seqs; at += S::seqs) {
         p.a.n_seqs = a.n_seqs - at < (uint32_t)S::seqs ? a.n_seqs - at : (uint32_t)S::seqs;

@@ -115,6 +115,17 @@ __host__ __device__ __forceinline__ Span visible(int p, int n, int causal, int w
     return s;
 }
 
+// Dynamic shared memory a kernel may be launched with, set once per kernel and device.
+template <auto kernel> cudaError_t allow_smem(int bytes) {
+    static bool set[64] = {};
+    int device = 0;
+    if (const cudaError_t e = cudaGetDevice(&device)) return e;
+    if (device < 64 && set[device]) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && device < 64) set[device] = true;
+    return e;
+}
+
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_go() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -24,9 +24,10 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr long long kWaitClocks = 4000000000ll;  // a wait for a page gives up after about two seconds
 
-// Warps per CTA: each holds one page's K and V block, 128 KiB in all, enough in flight per SM to cover the
-// latency of HBM.
-template <int D> constexpr int kWarps = 1024 / D;
+// Warps per CTA: each holds one page's K and V block, 96 to 128 KiB in all, enough in flight per SM to cover
+// the latency of HBM, and few enough that a warp's tiles stay in registers.
+template <int D> constexpr int kWarps = D == 64 ? 12 : 1024 / D;
+template <int D> constexpr int kWidest = D == 64 ? 4 : kWarps<D>;  // warps of the widest team
 template <int D> constexpr int kAccStride = D + 8;  // f32 per row of a joined tile: rows 8 banks apart
 
 struct SeqInfo {
@@ -128,7 +129,6 @@ __device__ __forceinline__ float quad_sum(float x) {
 // How the launch's pages are dealt out to its teams.
 struct Plan {
     unsigned units;  // pages of all items
-    unsigned jobs;   // short: pieces of items, each at most one page per warp of a team
     int teams, width;  // teams of the launch, warps per team
     bool few;        // short launch: jobs instead of equal shares of the units
 };
@@ -204,7 +204,7 @@ template <class T, int D> __global__ void __launch_bounds__(kWarps<D> * 32, 1) d
     if (pl.units == 0) return;
     // Warps per team: an item's share of the launch's warps, so that an item is in few pieces, none of
     // them joined by fewer threads than it has to (few items: whole CTAs; many: each warp on its own).
-    pl.width = NW;
+    pl.width = kWidest<D>;
     while (pl.width > 1 && items * pl.width > gridDim.x * (unsigned)NW) pl.width >>= 1;
     const int per_cta = NW / pl.width;
     pl.teams = (int)gridDim.x * per_cta;
@@ -212,14 +212,17 @@ template <class T, int D> __global__ void __launch_bounds__(kWarps<D> * 32, 1) d
     // at a team's border; beyond that every team takes an equal run of pages.
     pl.few = pl.units <= (unsigned)(pl.teams * pl.width);
     __syncthreads();  // scan_s is read
-    // Exclusive sums over the sequences of their units, or of their jobs.
+    // An item costs its pages and a fixed part (Q, joining, writing: about 1.5 pages' time of a warp), so equal
+    // shares are of pages + `fixed` per item. A share that would begin in an item's fixed part begins with the item.
+    const unsigned fixed = pl.few ? 0 : (unsigned)(3 * pl.width + 1) / 2;
+    // Exclusive sums over the sequences of their items' cost, or of their jobs.
     unsigned carry = 0;
     for (int at = 0; at < n; at += kThreads) {
         const int b = at + tid;
         unsigned v = 0;
         if (b < n && info[b].m > 0) {
             const int np = max(1, page_span(info[b].len, info[b].m, window, sinks).n);
-            v = (unsigned)((info[b].m * group + 15) / 16) * c.kv_heads * (unsigned)(pl.few ? (np + pl.width - 1) / pl.width : np);
+            v = (unsigned)((info[b].m * group + 15) / 16) * c.kv_heads * (pl.few ? (unsigned)((np + pl.width - 1) / pl.width) : np + fixed);
         }
         unsigned x = v;
 #pragma unroll
@@ -238,88 +241,140 @@ template <class T, int D> __global__ void __launch_bounds__(kWarps<D> * 32, 1) d
         if (b < n) info[b].start = before + x - v;
         __syncthreads();
     }
-    pl.jobs = carry;
+    const unsigned total = carry;  // cost of the launch, or its jobs
 
-    // ---- this team's run
+    // ---- this team's share
     const int team = warp / pl.width, w_in = warp % pl.width, threads = pl.width * 32, t_in = w_in * 32 + lane;
-    const long long t_all = (long long)blockIdx.x + (long long)team * gridDim.x;  // neighbours in work on different SMs
-    long long pos = pl.few ? t_all : (long long)pl.units * t_all / pl.teams;
-    const long long stop = pl.few ? (long long)pl.jobs : (long long)pl.units * (t_all + 1) / pl.teams;
-
-    // The segment at unit (or job) x; *next is where the following one starts.
-    auto segment_at = [&](long long x, long long* next) {
-        Segment s;
-        int lo = 0, hi = n;  // last sequence that starts at or before x: those without work are passed over
+    const unsigned t_all = blockIdx.x + (unsigned)team * gridDim.x;  // neighbours in work on different SMs
+    // Sequence of position x: the last one that starts at or before it, which passes over those without work.
+    auto seq_at = [&](unsigned x) {
+        int lo = 0, hi = n;
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if ((long long)info[mid].start <= x) lo = mid;
+            if (info[mid].start <= x) lo = mid;
             else hi = mid;
         }
-        s.b = lo;
-        const SeqInfo q = info[lo];
-        const int np = max(1, page_span(q.len, q.m, window, sinks).n), tiles = (q.m * group + 15) / 16;
-        const unsigned local = (unsigned)(x - q.start);
+        return lo;
+    };
+    // A place in the work: page p of item `item` (heads of tiles) of sequence b, or a job. A walk goes from the
+    // share's begin to its end.
+    struct Place {
+        int b, item, p;
+    };
+    auto place_at = [&](unsigned x) {
+        Place q;
+        if (x >= total) return Place{n, 0, 0};
+        q.b = seq_at(x);
+        const unsigned local = x - info[q.b].start, cost = max(1, page_span(info[q.b].len, info[q.b].m, window, sinks).n) + fixed;
+        q.item = (int)(local / cost);
+        const unsigned o = local % cost;
+        q.p = o > fixed ? (int)(o - fixed) : 0;
+        return q;
+    };
+    struct Walk {
+        Place at;          // the next segment
+        unsigned job;      // few: the next job
+        int np, tiles, items;  // of the sequence at.b
+    };
+    const Place stop = pl.few ? Place{n, 0, 0} : place_at((unsigned)((unsigned long long)total * (t_all + 1) / (unsigned)pl.teams));
+    auto enter = [&](Walk& w) {  // sequence w.at.b, or the next one that has work
+        while (w.at.b < n && info[w.at.b].m <= 0) ++w.at.b;
+        if (w.at.b >= n) return;
+        const SeqInfo& q = info[w.at.b];
+        w.np = max(1, page_span(q.len, q.m, window, sinks).n);
+        w.tiles = (q.m * group + 15) / 16;
+        w.items = w.tiles * (int)c.kv_heads;
+    };
+    Walk walk;
+    walk.job = t_all;
+    walk.at = pl.few ? Place{0, 0, 0} : place_at((unsigned)((unsigned long long)total * t_all / (unsigned)pl.teams));
+    enter(walk);
+    // The next segment of a walk; false at its end.
+    auto next_segment = [&](Walk& w, Segment& s) {
         if (pl.few) {
-            const int k = (np + pl.width - 1) / pl.width;
+            if (w.job >= total) return false;
+            w.at.b = seq_at(w.job);
+            enter(w);
+            const int k = (w.np + pl.width - 1) / pl.width;
+            const unsigned local = w.job - info[w.at.b].start;
             const int item = (int)(local / (unsigned)k), piece = (int)(local % (unsigned)k);
-            s.head = item / tiles;
-            s.tile = item % tiles;
-            s.p0 = (int)((long long)piece * np / k);
-            s.p1 = (int)((long long)(piece + 1) * np / k);
+            s.b = w.at.b;
+            s.head = item / w.tiles;
+            s.tile = item % w.tiles;
+            s.p0 = (int)((unsigned)(piece * w.np) / (unsigned)k);
+            s.p1 = (int)((unsigned)((piece + 1) * w.np) / (unsigned)k);
             s.parts = k;
             s.part = piece;
-            s.first = (int)(x - piece);
-            *next = x + pl.teams;
-        } else {
-            const int item = (int)(local / (unsigned)np);
-            s.p0 = (int)(local % (unsigned)np);
-            const long long begin = x - s.p0, end = begin + np;
-            s.p1 = (int)(min(end, stop) - begin);
-            s.head = item / tiles;
-            s.tile = item % tiles;
-            const long long t0 = ((begin + 1) * pl.teams - 1) / pl.units, t1 = (end * pl.teams - 1) / pl.units;
+            s.first = (int)w.job - piece;
+            w.job += (unsigned)pl.teams;
+            return true;
+        }
+        if (w.at.b >= n || (w.at.b == stop.b && w.at.item == stop.item && w.at.p >= stop.p)) return false;
+        if (w.at.b > stop.b || (w.at.b == stop.b && w.at.item > stop.item)) return false;
+        s.b = w.at.b;
+        s.head = w.tiles == 1 ? w.at.item : w.at.item / w.tiles;
+        s.tile = w.tiles == 1 ? 0 : w.at.item % w.tiles;
+        s.p0 = w.at.p;
+        s.p1 = w.at.b == stop.b && w.at.item == stop.item ? stop.p : w.np;
+        s.parts = 1;
+        s.part = 0;
+        s.first = 0;
+        if (s.p0 > 0 || s.p1 < w.np) {
+            const unsigned long long begin = info[w.at.b].start + (unsigned long long)w.at.item * (w.np + fixed), teams = (unsigned)pl.teams;
+            const unsigned t0 = (unsigned)(((begin + fixed + 1) * teams - 1) / total), t1 = (unsigned)(((begin + fixed + w.np) * teams - 1) / total);
             s.parts = (int)(t1 - t0) + 1;
             s.part = (int)(t_all - t0);
             s.first = (int)t0;
-            *next = begin + s.p1;
         }
-        return s;
+        w.at.p = 0;
+        if (++w.at.item == w.items) {
+            w.at.item = 0;
+            ++w.at.b;
+            enter(w);
+        }
+        return true;
     };
     auto slot_of = [&](const Segment& s, int part) { return pl.few ? s.first + part : (s.first + part) * 2 + (part == 0 ? 1 : 0); };
-    // Page of the pool holding the i-th visible page of a segment's sequence, -1: none; *index its page of
-    // the sequence.
-    auto page_at = [&](const Segment& s, int i, int* index) {
-        const SeqInfo q = info[s.b];
-        const PageSpan sp = page_span(q.len, q.m, window, sinks);
-        *index = i < sp.head ? i : sp.lo + i - sp.head;
-        if (i >= sp.n) return -1;
-        const int page = c.tables[(size_t)seq_s[s.b] * c.max_pages + *index];
-        return page >= 0 && page < (int)c.pages ? page : -1;
-    };
 
-    // ---- the page after the current one: found early, its K and V loaded as their slots come free
-    Segment ns{};
-    long long npos = pos;
-    int ni = 0, npage = -1, nindex = 0;
+    // ---- pages ahead of the current one: the one after it is known, its K and V loaded as their slots come free; the
+    // table is read for the one after that
+    Segment as{};         // segment of the page looked up
+    Walk awalk = walk;
+    int ai = 0;           // its number in the segment's item
+    bool more = true;
+    int raw_page = -1, raw_index = 0, raw_head = 0;  // looked up: entry as read, page of the sequence, kv head
+    int npage = -1, nindex = 0, nhead = 0;           // known
     float nks = 0.0f, nvs = 0.0f;
     uint32_t parity = 0;
     bool fine = true;  // no wait has run out
-    auto advance = [&](bool start) {
-        if (!start) ni += pl.width;
-        while (start || ni >= ns.p1) {
-            start = false;
-            if (npos >= stop) {
-                npage = -1;
+    bool fresh = true;
+    auto look_up = [&]() {
+        raw_page = -1;
+        if (!more) return;
+        if (!fresh) ai += pl.width;
+        while (fresh || ai >= as.p1) {
+            fresh = false;
+            if (!next_segment(awalk, as)) {
+                more = false;
                 return;
             }
-            ns = segment_at(npos, &npos);
-            ni = ns.p0 + w_in;
+            ai = as.p0 + w_in;
         }
-        npage = page_at(ns, ni, &nindex);
+        const SeqInfo& q = info[as.b];
+        const PageSpan sp = page_span(q.len, q.m, window, sinks);
+        raw_index = ai < sp.head ? ai : sp.lo + ai - sp.head;
+        raw_head = as.head;
+        if (ai < sp.n) raw_page = __ldg(c.tables + (size_t)seq_s[as.b] * c.max_pages + raw_index);
+    };
+    auto advance = [&]() {
+        npage = raw_page >= 0 && raw_page < (int)c.pages ? raw_page : -1;
+        nindex = raw_index;
+        nhead = raw_head;
+        look_up();
     };
     auto fetch = [&](int which) {
         if (npage < 0 || !fine) return;
-        const size_t block = block_index(c, a.layer, npage, which, ns.head);
+        const size_t block = block_index(c, a.layer, npage, which, nhead);
         if (which == 0) {
             nks = c.scales[block];
             nvs = c.scales[block + c.kv_heads];
@@ -327,22 +382,26 @@ template <class T, int D> __global__ void __launch_bounds__(kWarps<D> * 32, 1) d
         if (lane == 0)
             load_block(smem_addr(ring + (size_t)(warp * 2 + which) * kBlock), c.codes + block * (size_t)kBlock, kBlock, which ? bar_v : bar_k);
     };
-    advance(true);
+    look_up();
+    advance();
     fetch(0);
     fetch(1);
 
     const int g = lane >> 2, t = lane & 3;
     const unsigned char* kb = ring + (size_t)(warp * 2) * kBlock;
     const unsigned char* vb = kb + kBlock;
-    while (pos < stop) {
-        const Segment s = segment_at(pos, &pos);
+    Segment s{};
+    while (next_segment(walk, s)) {
         const SeqInfo q = info[s.b];
         // Rows of this lane: r, token of the sequence r / group, query head r % group.
         const int r0 = s.tile * 16 + g, r1 = r0 + 8, rows_all = q.m * group;
         const int first = q.len - q.m;
         const Span v0 = visible(first + r0 / group, q.len, 1, window, sinks), v1 = visible(first + r1 / group, q.len, 1, window, sinks);
         const int low_pos = first + s.tile * 16 / group, high_pos = first + min(rows_all - 1, s.tile * 16 + 15) / group;
-        uint32_t qf[D / 16][4];
+        // head_dim 256 keeps Q where the joined tile goes at the end of the segment: registers hold O
+        constexpr bool kQApart = D == 256;
+        uint32_t qf[kQApart ? 1 : D / 16][4];
+        uint4* const q_s = reinterpret_cast<uint4*>(acc_s + warp * 16 * kAccStride<D>) + lane;
         float c0 = a.scale * kLog2e, c1 = c0;
         {
             const T* base = static_cast<const T*>(a.q);
@@ -374,8 +433,14 @@ template <class T, int D> __global__ void __launch_bounds__(kWarps<D> * 32, 1) d
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i) {  // k-step i: block i / 4, word i % 4 of the lane's 16 dims
                     const T* x = e + (i >> 2) * 16 + (i & 3) * 4;
-                    qf[i][h] = pack_half(to_f32<T>(x[0]) * down, to_f32<T>(x[1]) * down);
-                    qf[i][2 + h] = pack_half(to_f32<T>(x[2]) * down, to_f32<T>(x[3]) * down);
+                    const uint32_t y0 = pack_half(to_f32<T>(x[0]) * down, to_f32<T>(x[1]) * down), y1 = pack_half(to_f32<T>(x[2]) * down, to_f32<T>(x[3]) * down);
+                    if (kQApart) {
+                        reinterpret_cast<uint32_t*>(q_s + i * 32)[h] = y0;
+                        reinterpret_cast<uint32_t*>(q_s + i * 32)[2 + h] = y1;
+                    } else {
+                        qf[i][h] = y0;
+                        qf[i][2 + h] = y1;
+                    }
                 }
             }
         }
@@ -387,7 +452,7 @@ template <class T, int D> __global__ void __launch_bounds__(kWarps<D> * 32, 1) d
         for (int i = s.p0 + w_in; i < s.p1; i += pl.width) {
             const int page = npage, index = nindex;
             const float ks = nks, vs = nvs;
-            advance(false);
+            advance();
             if (page < 0) {  // nothing of it was loaded
                 fetch(0);
                 fetch(1);
@@ -400,18 +465,28 @@ template <class T, int D> __global__ void __launch_bounds__(kWarps<D> * 32, 1) d
             if (fine) {
 #pragma unroll
                 for (int db = 0; db < D / 64; ++db) {
+                    uint32_t qd[4][4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (kQApart) {
+                            *reinterpret_cast<uint4*>(qd[i]) = q_s[(db * 4 + i) * 32];
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) qd[i][e] = qf[db * 4 + i][e];
+                        }
+                    }
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const uint4 w = *reinterpret_cast<const uint4*>(kb + db * 4096 + (16 * (g >> 1) + 2 * j + (g & 1)) * 64 + 16 * t);
                         uint32_t b0, b1;
                         widen4(w.x, b0, b1);
-                        mma16816(sc[j], qf[db * 4 + 0], b0, b1);
+                        mma16816(sc[j], qd[0], b0, b1);
                         widen4(w.y, b0, b1);
-                        mma16816(sc[j], qf[db * 4 + 1], b0, b1);
+                        mma16816(sc[j], qd[1], b0, b1);
                         widen4(w.z, b0, b1);
-                        mma16816(sc[j], qf[db * 4 + 2], b0, b1);
+                        mma16816(sc[j], qd[2], b0, b1);
                         widen4(w.w, b0, b1);
-                        mma16816(sc[j], qf[db * 4 + 3], b0, b1);
+                        mma16816(sc[j], qd[3], b0, b1);
                     }
                 }
             }
@@ -510,8 +585,10 @@ template <class T, int D> __global__ void __launch_bounds__(kWarps<D> * 32, 1) d
         float* mine = acc_s + warp * 16 * kAccStride<D>;
 #pragma unroll
         for (int x = 0; x < D / 8; ++x) {
-            *reinterpret_cast<float2*>(mine + g * kAccStride<D> + 8 * x + 2 * t) = make_float2(o[x][0] * vref, o[x][1] * vref);
-            *reinterpret_cast<float2*>(mine + (g + 8) * kAccStride<D> + 8 * x + 2 * t) = make_float2(o[x][2] * vref, o[x][3] * vref);
+            if (r0 < rows_all)
+                *reinterpret_cast<float2*>(mine + g * kAccStride<D> + 8 * x + 2 * t) = make_float2(o[x][0] * vref, o[x][1] * vref);
+            if (r1 < rows_all)
+                *reinterpret_cast<float2*>(mine + (g + 8) * kAccStride<D> + 8 * x + 2 * t) = make_float2(o[x][2] * vref, o[x][3] * vref);
         }
         if (t == 0) {
             *reinterpret_cast<float2*>(ml_s + (warp * 16 + g) * 2) = make_float2(m0, l0);
@@ -597,7 +674,7 @@ template <class T, int D> cudaError_t launch(const Params& p, int sms, cudaStrea
     constexpr int NW = kWarps<D>;
     const size_t smem = (size_t)NW * 2 * kPage * D + sizeof(float) * NW * 16 * kAccStride<D> + sizeof(float) * NW * 32 + 16 * NW +
                         (sizeof(SeqInfo) + sizeof(int)) * p.a.n_seqs;
-    if (const cudaError_t e = cudaFuncSetAttribute(decode_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return e;
+    if (const cudaError_t e = allow_smem<decode_kernel<T, D>>(232448 - 2048)) return e;
     decode_kernel<T, D><<<sms, NW * 32, smem, s>>>(p);
     return cudaGetLastError();
 }
@@ -606,7 +683,7 @@ template <class T, int D> cudaError_t launch(const Params& p, int sms, cudaStrea
 }  // namespace kv
 
 // Pieces: one per job or two per team, jobs at most pages / width + items <= 2 warps of the launch.
-static int decode_slots(uint32_t head_dim, int sms) { return 2 * sms * (int)(1024 / head_dim) + 2; }
+static int decode_slots(uint32_t head_dim, int sms) { return 2 * sms * (int)(1024 / head_dim) + 2; }  // at most 1024 / head_dim warps an SM
 size_t kv_decode_bytes(uint32_t head_dim, int sms) { return (size_t)decode_slots(head_dim, sms) * 16 * (head_dim + 2) * sizeof(float); }
 
 int launch_kv_decode(const mrl_kv_cache& c, const mrl_attn& a, int sms, void* scratch, unsigned* counters, cudaStream_t s) {
