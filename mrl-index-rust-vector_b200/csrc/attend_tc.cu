@@ -55,8 +55,7 @@ template <int D, bool PAGED> struct Shape {
 };
 
 struct SeqItem {
-    unsigned start;  // first item of the sequence
-    int len, row, m;
+    int len, row, m;  // tokens, first row of the call, rows
 };
 
 struct TcParams {
@@ -280,6 +279,8 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
     unsigned char* k_s = q_s + (size_t)TILES * S::q_bytes;      // per stage [D/64][128 keys][128 B]
     unsigned char* v_s = k_s + (size_t)ST * S::kv_bytes;        // per stage the same, over the cache [2 pages][D][128 B]
     __shared__ SeqItem info[S::seqs];
+    __shared__ unsigned start_s[S::seqs];  // first item of the i-th sequence in order
+    __shared__ uint16_t order_s[S::seqs];  // that sequence
     __shared__ int seq_s[PAGED ? S::seqs : 1];
     __shared__ unsigned scan_s[32];
     constexpr int KP = S::k_parts, VP = S::v_parts;
@@ -323,24 +324,38 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
         tc::tmem_alloc(&tmem_s, 512);
         tc::tmem_relinquish();
     }
-    // ---- the call's sequences and their items
+    // ---- the call's sequences, longest first where there are few, so that the last items are short ones
+    for (int b = tid; b < n; b += S::threads) {
+        const Rows r{a.seqs, a.cu, n, (int)a.n_tokens};
+        SeqItem q{0, r.begin(b), 0};
+        q.m = r.end(b) - q.row;
+        q.len = q.m;
+        if (PAGED) {
+            const int seq = a.seqs[b];
+            const bool known = seq >= 0 && seq < (int)pr.c.max_seqs;
+            seq_s[b] = known ? seq : 0;
+            q.len = known ? min(max(pr.c.lens[seq], 0), (int)pr.c.max_pages * kPage) : 0;
+        }
+        info[b] = q;
+    }
+    __syncthreads();
+    for (int b = tid; b < n; b += S::threads) {
+        int rank = b;
+        if (n <= 128) {
+            rank = 0;
+            for (int x = 0; x < n; ++x) rank += info[x].len > info[b].len || (info[x].len == info[b].len && x < b);
+        }
+        order_s[rank] = (uint16_t)b;
+    }
+    __syncthreads();
+    // ---- their items
     unsigned carry = 0;
     for (int at = 0; at < n; at += S::threads) {
         const int b = at + tid;
         unsigned v = 0;
-        SeqItem q{0, 0, 0, 0};
         if (b < n) {
-            const Rows r{a.seqs, a.cu, n, (int)a.n_tokens};
-            q.row = r.begin(b);
-            q.m = r.end(b) - q.row;
-            q.len = q.m;
-            if (PAGED) {
-                const int seq = a.seqs[b];
-                const bool known = seq >= 0 && seq < (int)pr.c.max_seqs;
-                seq_s[b] = known ? seq : 0;
-                q.len = known ? min(max(pr.c.lens[seq], 0), (int)pr.c.max_pages * kPage) : 0;
-            }
-            v = q.m > 0 ? (unsigned)((q.m + TILES * tokens - 1) / (TILES * tokens)) * (unsigned)pr.heads : 0;
+            const int m = info[order_s[b]].m;
+            v = m > 0 ? (unsigned)((m + TILES * tokens - 1) / (TILES * tokens)) * (unsigned)pr.heads : 0;
         }
         unsigned x = v;
 #pragma unroll
@@ -355,8 +370,7 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
             if (w < warp) before += scan_s[w];
             carry += scan_s[w];
         }
-        q.start = before + x - v;
-        if (b < n) info[b] = q;
+        if (b < n) start_s[b] = before + x - v;
         __syncthreads();
     }
     const unsigned items = carry;
@@ -371,12 +385,13 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
         int lo = 0, hi = n;
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if (info[mid].start <= i) lo = mid;
+            if (start_s[mid] <= i) lo = mid;
             else hi = mid;
         }
+        const unsigned local = i - start_s[lo];
+        lo = order_s[lo];
         const SeqItem q = info[lo];
         const int count = (q.m + TILES * tokens - 1) / (TILES * tokens);
-        const unsigned local = i - q.start;
         it.b = lo;
         it.head = (int)(local % (unsigned)pr.heads);
         it.first = (count - 1 - (int)(local / (unsigned)pr.heads)) * TILES * tokens;
@@ -399,6 +414,10 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
         return it;
     };
 
+    // The CTA's item in round r: there and back over the CTAs, so that a long one is followed by a short one.
+    const unsigned grid = gridDim.x;
+    auto item_no = [&](unsigned r) { return r & 1 ? (r + 1) * grid - 1 - blockIdx.x : r * grid + blockIdx.x; };
+
     if (warp >= 8) fewer_registers<S::regs_other>();
     else if (warp < 4 * TILES) more_registers<S::regs_softmax>();
     if (warp < 4 * TILES) {
@@ -409,7 +428,9 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
         const bool row_used = r < tokens * group;
         uint32_t s_par = 0, o_par = 0;  // bit i: buffer i
         int step_no = 0, used = 0, items_done = 0;
-        for (unsigned i = blockIdx.x; i < items && !failed; i += gridDim.x) {
+        for (unsigned r_no = 0; r_no * grid < items && !failed; ++r_no) {
+            const unsigned i = item_no(r_no);
+            if (i >= items) break;
             const Item<TILES> it = item_at(i);
             float cur = a.scale * kLog2e;
             const int f = it.first + tile * tokens, base = it.len - it.m;
@@ -506,8 +527,9 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                 }
                 any = true;
                 if (PAGED) {
-                    va = vref > 0.0f ? va / vref : 0.0f;
-                    vb = vref > 0.0f ? vb / vref : 0.0f;
+                    const float per = vref > 0.0f ? __fdividef(1.0f, vref) : 0.0f;
+                    va *= per;
+                    vb *= per;
                 }
                 // P over S. A masked score is -inf. Over the cache P carries V's scale, put into the exponent and
                 // taken out of the sum again; below 2^-24 of the unit it would leave f16 anyway.
@@ -534,7 +556,7 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                     MRL_TC_ST32(s_col + h * 32, y);
                     float s0, s1;
                     split(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), s0, s1);
-                    l += PAGED ? (s0 + s1) / (h ? vb : va) : s0 + s1;
+                    l += PAGED ? __fdividef(s0 + s1, h ? vb : va) : s0 + s1;
                 }
                 tc::wait_st();
                 tc::fence_before();
@@ -648,7 +670,9 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                 }
                 return true;
             };
-            for (unsigned i = blockIdx.x; i < items && ok && !failed; i += gridDim.x) {
+            for (unsigned r_no = 0; r_no * grid < items && ok && !failed; ++r_no) {
+                const unsigned i = item_no(r_no);
+                if (i >= items) break;
                 const Item<TILES> it = item_at(i);
                 bool q_here[TILES], begun[TILES];
                 int pend[TILES], pend_buf[TILES];  // step whose P is to come, -1: none
@@ -728,7 +752,9 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
             int step_no = 0;
             uint32_t q_par = 0;
             bool ok = true;
-            for (unsigned i = blockIdx.x; i < items && ok && !failed; i += gridDim.x) {
+            for (unsigned r_no = 0; r_no * grid < items && ok && !failed; ++r_no) {
+                const unsigned i = item_no(r_no);
+                if (i >= items) break;
                 const Item<TILES> it = item_at(i);
                 for (int t = 0; t < TILES && ok; ++t) {
                     if (it.st[t].hi == 0) continue;
@@ -772,7 +798,9 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
             const mrl_kv_cache& c = pr.c;
             int step_no = 0;
             bool ok = true;
-            for (unsigned i = blockIdx.x; i < items && ok && !failed; i += gridDim.x) {
+            for (unsigned r_no = 0; r_no * grid < items && ok && !failed; ++r_no) {
+                const unsigned i = item_no(r_no);
+                if (i >= items) break;
                 const Item<TILES> it = item_at(i);
                 const int32_t* table = c.tables + (size_t)seq_s[it.b] * c.max_pages;
                 auto page_of = [&](int index) {
@@ -833,7 +861,9 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
         int items_done = 0;
         uint32_t q_par = 0;
         bool ok = true;
-        for (unsigned i = blockIdx.x; i < items && ok && !failed; i += gridDim.x, ++items_done) {
+        for (unsigned r_no = 0; r_no * grid < items && ok && !failed; ++r_no, ++items_done) {
+            const unsigned i = item_no(r_no);
+            if (i >= items) break;
             const Item<TILES> it = item_at(i);
             // D / 8 lanes to a row, 16 bytes each, copied to where the operand wants them, and bf16 made f16 there by
             // the thread that copied it. bf16 has more range than f16: a row is brought to [1, 2) by a power of two,
@@ -852,27 +882,40 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                 }
             };
             auto finish_q = [&](int t) {
-#pragma unroll 2
-                for (int r = q_row; r < 128 && !__is_same(T, __half); r += kRows) {
-                    uint4* at = reinterpret_cast<uint4*>(q_at(t, r));
-                    uint4 x = *at;
-                    const T* e = reinterpret_cast<const T*>(&x);
-                    float top = 0.0f, down = 1.0f;
-                    uint32_t up = 127;
+                constexpr int kTurn = 8;  // rows of a thread in flight
+                for (int r0 = q_row; r0 < 128 && !__is_same(T, __half); r0 += kTurn * kRows) {
+                    uint4 x[kTurn];
+                    float top[kTurn];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(to_f32<T>(e[j])));
+                    for (int i = 0; i < kTurn; ++i) x[i] = *reinterpret_cast<const uint4*>(q_at(t, r0 + i * kRows));
 #pragma unroll
-                    for (int d = kLanes / 2; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-                    const uint32_t ex = __float_as_uint(top) >> 23;
-                    if (ex > 0 && ex < 255) {
-                        up = min(ex, 253u);
-                        down = __uint_as_float((254u - up) << 23);
+                    for (int i = 0; i < kTurn; ++i) {
+                        const T* e = reinterpret_cast<const T*>(&x[i]);
+                        top[i] = 0.0f;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) top[i] = fmaxf(top[i], fabsf(to_f32<T>(e[j])));
                     }
-                    uint32_t y[4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) y[j] = pack16<false>(to_f32<T>(e[2 * j]) * down, to_f32<T>(e[2 * j + 1]) * down);
-                    *at = make_uint4(y[0], y[1], y[2], y[3]);
-                    if (q_col == 0) q_up_s[((items_done & 1) * TILES + t) * 128 + r] = (uint8_t)up;
+                    for (int d = kLanes / 2; d; d >>= 1)
+#pragma unroll
+                        for (int i = 0; i < kTurn; ++i) top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], d));
+#pragma unroll
+                    for (int i = 0; i < kTurn; ++i) {
+                        const T* e = reinterpret_cast<const T*>(&x[i]);
+                        const int r = r0 + i * kRows;
+                        float down = 1.0f;
+                        uint32_t up = 127;
+                        const uint32_t ex = __float_as_uint(top[i]) >> 23;
+                        if (ex > 0 && ex < 255) {
+                            up = min(ex, 253u);
+                            down = __uint_as_float((254u - up) << 23);
+                        }
+                        uint32_t y[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) y[j] = pack16<false>(to_f32<T>(e[2 * j]) * down, to_f32<T>(e[2 * j + 1]) * down);
+                        *reinterpret_cast<uint4*>(q_at(t, r)) = make_uint4(y[0], y[1], y[2], y[3]);
+                        if (q_col == 0) q_up_s[((items_done & 1) * TILES + t) * 128 + r] = (uint8_t)up;
+                    }
                 }
                 tc::fence_proxy_async_smem();
                 __syncwarp();
