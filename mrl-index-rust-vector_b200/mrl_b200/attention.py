@@ -25,7 +25,7 @@ from ._capi import AttnC, KvCacheC, check
 from .api import Device, default_device
 
 PAGE_TOKENS = 64  # MRL_KV_PAGE
-KV_NO_PAGES, KV_ROW_FULL, KV_BAD_INDEX, KV_NONFINITE = 1, 2, 4, 8
+KV_NO_PAGES, KV_ROW_FULL, KV_BAD_INDEX, KV_NONFINITE, KV_TIMEOUT = 1, 2, 4, 8, 16
 HEAD_DIMS = (64, 128, 256)
 
 _ATTN = struct.Struct("@7P8q10IfI")
