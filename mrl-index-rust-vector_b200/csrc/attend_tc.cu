@@ -934,7 +934,8 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
     }
     __syncthreads();
     if (warp == 8) tc::tmem_dealloc(tmem, 512);
-    if (tid == 0 && failed && pr.c.status) atomicOr(pr.c.status, MRL_KV_TIMEOUT);
+    uint32_t* const status = PAGED ? pr.c.status : a.status;
+    if (tid == 0 && failed && status) atomicOr(status, MRL_KV_TIMEOUT);
 }
 
 // The pages that the call's sequences see, codes to f16 in the operands' layout: every 64 codes of K (a

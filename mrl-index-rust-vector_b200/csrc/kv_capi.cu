@@ -102,6 +102,14 @@ int kv_image(mrl_ctx* ctx, size_t bytes, void** out) {
     return MRL_OK;
 }
 
+// Windows and sinks beyond any sequence (2^28 rows) all mean the same; cut, sums with positions stay in an int.
+mrl_attn cut(const mrl_attn& a) {
+    mrl_attn b = a;
+    b.window = std::min(b.window, 1u << 30);
+    b.sinks = std::min(b.sinks, 1u << 30);
+    return b;
+}
+
 int check_attn(mrl_ctx* ctx, const mrl_attn* a, uint32_t kv_heads, uint32_t head_dim, bool paged) {
     if (a->dtype != MRL_F16 && a->dtype != MRL_BF16) return bad(ctx, "dtype must be MRL_F16 or MRL_BF16");
     if (head_dim != 64 && head_dim != 128 && head_dim != 256) return bad(ctx, "head_dim must be 64, 128 or 256");
@@ -167,7 +175,7 @@ int mrl_kv_trim(mrl_ctx* ctx, const mrl_kv_cache* kv, const int32_t* d_seqs, uin
         if (n > kMaxSeqs) return bad(ctx, "n must be at most 65535");
         if (n == 0) return MRL_OK;
         if (!d_seqs) return bad(ctx, "seqs is NULL");
-        return done(ctx, mrl::launch_kv_release(*kv, d_seqs, n, 1, window, sinks, ctx->stream), "mrl_kv_trim");
+        return done(ctx, mrl::launch_kv_release(*kv, d_seqs, n, 1, std::min(window, 1u << 30), std::min(sinks, 1u << 30), ctx->stream), "mrl_kv_trim");
     });
 }
 
@@ -233,15 +241,16 @@ int mrl_kv_attend(mrl_ctx* ctx, const mrl_kv_cache* kv, const mrl_attn* a) {
         if (a->cu && (uint64_t)a->max_rows * (a->q_heads / kv->kv_heads) > 64) {
             void* wide;
             if (int rc = kv_image(ctx, mrl::kv_wide_bytes(*kv), &wide)) return rc;
-            return done(ctx, mrl::launch_attend_tc(kv, *a, ctx->sms, wide, ctx->stream), "mrl_kv_attend");
+            return done(ctx, mrl::launch_attend_tc(kv, cut(*a), ctx->sms, wide, ctx->stream), "mrl_kv_attend");
         }
-        // units of work of a launch are counted in 32 bits
-        const uint64_t tiles = (uint64_t)a->n_tokens * (a->q_heads / kv->kv_heads) / 16 + std::min(a->n_seqs, mrl::kKvDecodeSeqs);
-        if (tiles * kv->kv_heads * kv->max_pages >= (1ull << 32)) return bad(ctx, "too many rows x pages for one call");
+        // the cost of a launch's items (pages and a fixed part of at most 16 each) is summed in 32 bits
+        const uint64_t group = a->q_heads / kv->kv_heads, per_launch = std::min(a->n_seqs, mrl::kKvDecodeSeqs);
+        const uint64_t tiles = a->cu ? a->n_tokens * group / 16 + per_launch : per_launch * ((group + 15) / 16);
+        if (tiles * kv->kv_heads * (kv->max_pages + 16ull) >= (1ull << 32)) return bad(ctx, "rows x kv_heads x max_pages is too large for one call");
         void* scratch;
         unsigned* counters;
         if (int rc = kv_scratch(ctx, mrl::kv_decode_bytes(kv->head_dim, ctx->sms), &scratch, &counters)) return rc;
-        return done(ctx, mrl::launch_kv_decode(*kv, *a, ctx->sms, scratch, counters, ctx->stream), "mrl_kv_attend");
+        return done(ctx, mrl::launch_kv_decode(*kv, cut(*a), ctx->sms, scratch, counters, ctx->stream), "mrl_kv_attend");
     });
 }
 
@@ -250,7 +259,7 @@ int mrl_window_attention(mrl_ctx* ctx, const mrl_attn* a) {
         if (!a) return bad(ctx, "args are NULL");
         if (int rc = check_attn(ctx, a, a->kv_heads, a->head_dim, false)) return rc;
         if (a->n_tokens == 0) return MRL_OK;
-        const int rc = mrl::launch_attend_tc(nullptr, *a, ctx->sms, nullptr, ctx->stream);
+        const int rc = mrl::launch_attend_tc(nullptr, cut(*a), ctx->sms, nullptr, ctx->stream);
         if (rc < 0) return bad(ctx, "k or v has strides that a tensor map cannot describe");
         return done(ctx, rc, "mrl_window_attention");
     });

@@ -696,7 +696,7 @@ int launch_kv_decode(const mrl_kv_cache& c, const mrl_attn& a, int sms, void* sc
     p.row0 = 0;
     const bool half = a.dtype == MRL_F16;
     for (uint32_t at = 0; at < a.n_seqs; at += kKvDecodeSeqs) {
-        p.a.n_seqs = a.n_seqs - at < kKvDecodeSeqs ? a.n_seqs - at : kKvDecodeSeqs;
+        p.a.n_seqs = a.n_seqs - at < kKvDecodeSeqs ? a.n_seqs - at : kKvDecodeSeqs;  // at most so many have their table in shared memory
         p.a.seqs = a.seqs + at;
         p.a.cu = a.cu ? a.cu + at : nullptr;
         p.row0 = (int)at;

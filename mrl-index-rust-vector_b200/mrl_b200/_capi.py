@@ -73,7 +73,7 @@ class KvCacheC(C.Structure):
 class AttnC(C.Structure):
     """struct mrl_attn of include/mrl_kv.h."""
 
-    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "out", "lse", "seqs", "cu")] + [
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "out", "lse", "seqs", "cu", "status")] + [
         (n, C.c_int64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head", "o_row", "o_head")] + [
         (n, C.c_uint32) for n in ("n_seqs", "n_tokens", "max_rows", "q_heads", "kv_heads", "head_dim", "dtype", "causal",
                                   "window", "sinks")] + [("scale", C.c_float), ("layer", C.c_uint32)]

@@ -211,6 +211,7 @@ class Device:
             raise MrlError(rc, f"cannot create a context on CUDA device {index} (needs an sm_100 GPU)")
         self.index = index
         self.torch_stream = None  # the stream set by set_stream (None: the context's own)
+        self.attention_status = None  # status word of window_attention (a CUDA tensor, made by its first call)
 
     def close(self) -> None:
         if self.ptr:

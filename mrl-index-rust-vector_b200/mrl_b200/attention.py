@@ -28,7 +28,7 @@ PAGE_TOKENS = 64  # MRL_KV_PAGE
 KV_NO_PAGES, KV_ROW_FULL, KV_BAD_INDEX, KV_NONFINITE, KV_TIMEOUT = 1, 2, 4, 8, 16
 HEAD_DIMS = (64, 128, 256)
 
-_ATTN = struct.Struct("@7P8q10IfI")
+_ATTN = struct.Struct("@8P8q10IfI")
 assert _ATTN.size == C.sizeof(AttnC)
 
 
@@ -248,12 +248,19 @@ class KvCache:
         out, o_row, o_head = _out(out, q, dev)
         lse = _torch_module.empty(t, heads, dtype=_torch_module.float32, device=q.device) if return_lse else None
         _ATTN.pack_into(self._args, 0, q.data_ptr(), 0, 0, out.data_ptr(), lse.data_ptr() if return_lse else 0,
-                        seqs.data_ptr(), cu_ptr or 0, q_row, q_head, 0, 0, 0, 0, o_row, o_head, n, t, _count(max_q, "max_q"), heads,
+                        seqs.data_ptr(), cu_ptr or 0, 0, q_row, q_head, 0, 0, 0, 0, o_row, o_head, n, t, _count(max_q, "max_q"), heads,
                         self.kv_heads, self.head_dim, _dtype_codes[q.dtype], 1, _count(window, "window"),
                         _count(sinks, "sinks"), self._scale if scale is None else scale, _count(layer, "layer"))
         with self._ordered:
             check(dev.ptr, dev.lib.mrl_kv_attend(dev.ptr, self._p, self._args_p))
         return (out, lse) if return_lse else out
+
+
+def _status(dev: Device, like):
+    """The device's status word for calls without a cache (Device.attention_status): KV_TIMEOUT or 0."""
+    if dev.attention_status is None:
+        dev.attention_status = _torch_module.zeros(1, dtype=_torch_module.int32, device=like.device)
+    return dev.attention_status
 
 
 def _count(x, name: str) -> int:
@@ -288,6 +295,7 @@ def window_attention(q, k, v, cu, max_len: int, causal: bool = True, window: int
     out, o_row, o_head = _out(out, q, dev)
     lse = torch.empty(t, heads, dtype=torch.float32, device=q.device) if return_lse else None
     a = AttnC(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0, 0, cu.data_ptr(),
+              _status(dev, q).data_ptr(),
               q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, cu.shape[0] - 1, t, _count(max_len, "max_len"), heads,
               k.shape[1], d, _dtype_codes[q.dtype], int(bool(causal)), _count(window, "window"), _count(sinks, "sinks"),
               1.0 / math.sqrt(d) if scale is None else scale, 0)
