@@ -276,7 +276,13 @@ template <class T, int D> __global__ void __launch_bounds__(kWarps<D> * 32, 1) d
         unsigned job;      // few: the next job
         int np, tiles, items;  // of the sequence at.b
     };
-    const Place stop = pl.few ? Place{n, 0, 0} : place_at((unsigned)((unsigned long long)total * (t_all + 1) / (unsigned)pl.teams));
+    // begin and end of the share, by the even and the odd lanes at once
+    Place edge{0, 0, 0}, stop{n, 0, 0};
+    if (!pl.few) {
+        const Place q = place_at((unsigned)((unsigned long long)total * (t_all + (lane & 1)) / (unsigned)pl.teams));
+        edge = Place{__shfl_sync(~0u, q.b, 0), __shfl_sync(~0u, q.item, 0), __shfl_sync(~0u, q.p, 0)};
+        stop = Place{__shfl_sync(~0u, q.b, 1), __shfl_sync(~0u, q.item, 1), __shfl_sync(~0u, q.p, 1)};
+    }
     auto enter = [&](Walk& w) {  // sequence w.at.b, or the next one that has work
         while (w.at.b < n && info[w.at.b].m <= 0) ++w.at.b;
         if (w.at.b >= n) return;
@@ -287,7 +293,7 @@ template <class T, int D> __global__ void __launch_bounds__(kWarps<D> * 32, 1) d
     };
     Walk walk;
     walk.job = t_all;
-    walk.at = pl.few ? Place{0, 0, 0} : place_at((unsigned)((unsigned long long)total * t_all / (unsigned)pl.teams));
+    walk.at = edge;
     enter(walk);
     // The next segment of a walk; false at its end.
     auto next_segment = [&](Walk& w, Segment& s) {
@@ -632,34 +638,47 @@ template <class T, int D> __global__ void __launch_bounds__(kWarps<D> * 32, 1) d
             }
         }
         if (s.parts > 1) {
-            __threadfence();
-            team_sync(team, threads);
+            team_sync(team, threads);  // the team's stores come before its arrival, and the others' before the last one's reads
             if (t_in == 0) {
+                __threadfence();
                 const unsigned before = atomicAdd(&pr.counters[s.first], 1u);
                 if (before + 1 == (unsigned)s.parts) pr.counters[s.first] = 0;
+                __threadfence();
                 arrived_s[warp] = before + 1;
             }
             team_sync(team, threads);
             if (arrived_s[w0] == (unsigned)s.parts) {
-                __threadfence();
                 for (int i = t_in; i < tile_rows * (D / 4); i += threads) {
                     const int r = i / (D / 4), d = i % (D / 4) * 4;
-                    float m = -INFINITY;
-                    for (int k = 0; k < s.parts; ++k) m = fmaxf(m, __ldcg(ml_g + ((size_t)slot_of(s, k) * 16 + r) * 2));
-                    const float z = m == -INFINITY ? 0.0f : m;
-                    float l = 0.0f;
+                    float m = -INFINITY, l = 0.0f;
                     float4 x = make_float4(0, 0, 0, 0);
-#pragma unroll 4
-                    for (int k = 0; k < s.parts; ++k) {
-                        const size_t slot = (size_t)slot_of(s, k);
-                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(ml_g + (slot * 16 + r) * 2));
-                        const float4 y = __ldcg(reinterpret_cast<const float4*>(pr.part + (slot * 16 + r) * D + d));
-                        const float e = ex2(ml.x - z);
-                        l = fmaf(e, ml.y, l);
-                        x.x = fmaf(e, y.x, x.x);
-                        x.y = fmaf(e, y.y, x.y);
-                        x.z = fmaf(e, y.z, x.z);
-                        x.w = fmaf(e, y.w, x.w);
+                    for (int k0 = 0; k0 < s.parts; k0 += 4) {  // four pieces' loads at once
+                        float2 ml[4];
+                        float4 y[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            ml[k] = make_float2(-INFINITY, 0.0f);
+                            y[k] = make_float4(0, 0, 0, 0);
+                            if (k0 + k < s.parts) {
+                                const size_t slot = (size_t)slot_of(s, k0 + k);
+                                ml[k] = __ldcg(reinterpret_cast<const float2*>(ml_g + (slot * 16 + r) * 2));
+                                y[k] = __ldcg(reinterpret_cast<const float4*>(pr.part + (slot * 16 + r) * D + d));
+                            }
+                        }
+                        const float top = fmaxf(fmaxf(m, fmaxf(ml[0].x, ml[1].x)), fmaxf(ml[2].x, ml[3].x)), z = top == -INFINITY ? 0.0f : top;
+                        const float keep = ex2(m - z);
+                        l *= keep;
+                        x = make_float4(x.x * keep, x.y * keep, x.z * keep, x.w * keep);
+                        m = top;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const float e = ex2(ml[k].x - z);
+                            l = fmaf(e, ml[k].y, l);
+                            x.x = fmaf(e, y[k].x, x.x);
+                            x.y = fmaf(e, y[k].y, x.y);
+                            x.z = fmaf(e, y[k].z, x.z);
+                            x.w = fmaf(e, y[k].w, x.w);
+                        }
                     }
                     emit(r, d, x, m, l);
                 }
