@@ -212,6 +212,7 @@ class Device:
         self.index = index
         self.torch_stream = None  # the stream set by set_stream (None: the context's own)
         self.attention_status = None  # status word of window_attention (a CUDA tensor, made by its first call)
+        self.attention_call = None
 
     def close(self) -> None:
         if self.ptr:

@@ -49,22 +49,17 @@ def _torch():
     return _torch_module
 
 
-class _Ordered:
-    """The context's work of the block after torch's current stream, and that stream after it."""
-
-    __slots__ = ("dev", "stream")
-
-    def __init__(self, dev: Device):
-        self.dev = dev
-
-    def __enter__(self):
-        self.stream = _raw_stream(self.dev.index) or 1
-        if self.stream != self.dev.torch_stream:
-            check(self.dev.ptr, self.dev.lib.mrl_ctx_join(self.dev.ptr, self.stream, 1))
-
-    def __exit__(self, *exc):
-        if self.stream != self.dev.torch_stream:
-            check(self.dev.ptr, self.dev.lib.mrl_ctx_join(self.dev.ptr, self.stream, 0))
+def _call(dev: Device, fn, *args) -> None:
+    """One entry point of the library, its work after torch's current stream and that stream after it."""
+    stream = _raw_stream(dev.index) or 1
+    if stream == dev.torch_stream:
+        rc = fn(dev.ptr, *args)
+    else:
+        check(dev.ptr, dev.lib.mrl_ctx_join(dev.ptr, stream, 1))
+        rc = fn(dev.ptr, *args)
+        check(dev.ptr, dev.lib.mrl_ctx_join(dev.ptr, stream, 0))
+    if rc:
+        check(dev.ptr, rc)
 
 
 def _index(x, name: str, dev: Device, n: Optional[int] = None):
@@ -81,9 +76,10 @@ def _index(x, name: str, dev: Device, n: Optional[int] = None):
 
 def _rows(x, name: str, dev: Device, heads=None, dims=None, dtype=None, tokens=None):
     """A [tokens, heads, dims] 16-bit tensor whose dims are contiguous; (row stride, head stride)."""
-    if x.dim() != 3 or x.get_device() != dev.index or _dtype_codes.get(x.dtype, 2) == 2:
+    shape = x.shape
+    if len(shape) != 3 or x.get_device() != dev.index or _dtype_codes.get(x.dtype, 2) == 2:
         raise ValueError(f"{name} must be a [tokens, heads, head_dim] float16 or bfloat16 tensor on cuda:{dev.index}")
-    t, h, d = x.shape
+    t, h, d = shape
     if (heads is not None and h != heads) or (dims is not None and d != dims) or (tokens is not None and t != tokens):
         raise ValueError(f"{name} has shape {tuple(x.shape)}; expected [{tokens if tokens is not None else 'tokens'}, "
                          f"{heads if heads is not None else 'heads'}, {dims if dims is not None else 'head_dim'}]")
@@ -127,7 +123,6 @@ class KvCache:
         self._p = C.addressof(self._c)
         self._args = bytearray(_ATTN.size)
         self._args_p = C.addressof((C.c_char * _ATTN.size).from_buffer(self._args))
-        self._ordered = _Ordered(dev)
         self._scale = 1.0 / math.sqrt(self.head_dim)
 
     @staticmethod
@@ -154,45 +149,38 @@ class KvCache:
         dev = self.dev
         _index(seqs, "seqs", dev)
         _index(tokens, "tokens", dev, seqs.shape[0])
-        with self._ordered:
-            check(dev.ptr, dev.lib.mrl_kv_reserve(dev.ptr, self._p, seqs.data_ptr(), tokens.data_ptr(), seqs.shape[0]))
+        _call(dev, dev.lib.mrl_kv_reserve, self._p, seqs.data_ptr(), tokens.data_ptr(), seqs.shape[0])
 
     def fork(self, parents, children) -> None:
         """children[i] (empty) becomes a copy of parents[i] that shares its full pages (mrl_kv_fork)."""
         dev = self.dev
         _index(parents, "parents", dev)
         _index(children, "children", dev, parents.shape[0])
-        with self._ordered:
-            check(dev.ptr, dev.lib.mrl_kv_fork(dev.ptr, self._p, parents.data_ptr(), children.data_ptr(), parents.shape[0]))
+        _call(dev, dev.lib.mrl_kv_fork, self._p, parents.data_ptr(), children.data_ptr(), parents.shape[0])
 
     def release(self, seqs) -> None:
         """Drop the sequences and give their pages back (mrl_kv_release)."""
         dev = self.dev
         _index(seqs, "seqs", dev)
-        with self._ordered:
-            check(dev.ptr, dev.lib.mrl_kv_release(dev.ptr, self._p, seqs.data_ptr(), seqs.shape[0]))
+        _call(dev, dev.lib.mrl_kv_release, self._p, seqs.data_ptr(), seqs.shape[0])
 
     def trim(self, seqs, window: int, sinks: int = 0) -> None:
         """Give back the pages that no later query sees through the window and the sinks (mrl_kv_trim)."""
         dev = self.dev
         _index(seqs, "seqs", dev)
-        with self._ordered:
-            check(dev.ptr, dev.lib.mrl_kv_trim(dev.ptr, self._p, seqs.data_ptr(), seqs.shape[0], _count(window, "window"),
-                                               _count(sinks, "sinks")))
+        _call(dev, dev.lib.mrl_kv_trim, self._p, seqs.data_ptr(), seqs.shape[0], _count(window, "window"), _count(sinks, "sinks"))
 
     def compact(self) -> None:
         """Move the held pages to the front of the pool (mrl_kv_compact)."""
         dev = self.dev
-        with self._ordered:
-            check(dev.ptr, dev.lib.mrl_kv_compact(dev.ptr, self._p))
+        _call(dev, dev.lib.mrl_kv_compact, self._p)
 
     def copy_pages(self, src, dst) -> None:
         """Copy the contents of page src[i] to page dst[i], all layers (mrl_kv_copy_pages)."""
         dev = self.dev
         _index(src, "src", dev)
         _index(dst, "dst", dev, src.shape[0])
-        with self._ordered:
-            check(dev.ptr, dev.lib.mrl_kv_copy_pages(dev.ptr, self._p, src.data_ptr(), dst.data_ptr(), src.shape[0]))
+        _call(dev, dev.lib.mrl_kv_copy_pages, self._p, src.data_ptr(), dst.data_ptr(), src.shape[0])
 
     # -- tokens --
 
@@ -212,9 +200,7 @@ class KvCache:
         _index(seqs, "seqs", dev)
         n, t = seqs.shape[0], k.shape[0]
         cu_ptr = self._cu(cu, n, t)
-        with self._ordered:
-            check(dev.ptr, dev.lib.mrl_kv_append(dev.ptr, self._p, layer, _dtype_codes[k.dtype], k.data_ptr(), k_row, k_head,
-                                                 v.data_ptr(), v_row, v_head, seqs.data_ptr(), cu_ptr, n, t))
+        _call(dev, dev.lib.mrl_kv_append, self._p, layer, _dtype_codes[k.dtype], k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head, seqs.data_ptr(), cu_ptr, n, t)
 
     def read(self, layer: int, seqs, cu=None, tokens: Optional[int] = None, dtype=None):
         """(k, v), [tokens, kv_heads, head_dim]: the values held for the same rows as append's
@@ -227,11 +213,9 @@ class KvCache:
         dtype = dtype or torch.float32
         if dtype not in _dtype_codes:
             raise ValueError("dtype must be float32, float16 or bfloat16")
-        kv = torch.empty(2, t, self.kv_heads, self.head_dim, dtype=dtype, device=seqs.device)
+        kv = seqs.new_empty((2, t, self.kv_heads, self.head_dim), dtype=dtype)
         k, v = kv[0], kv[1]
-        with self._ordered:
-            check(dev.ptr, dev.lib.mrl_kv_read(dev.ptr, self._p, layer, _dtype_codes[dtype], k.data_ptr(), v.data_ptr(),
-                                               seqs.data_ptr(), cu_ptr, n, t))
+        _call(dev, dev.lib.mrl_kv_read, self._p, layer, _dtype_codes[dtype], k.data_ptr(), v.data_ptr(), seqs.data_ptr(), cu_ptr, n, t)
         return k, v
 
     def attend(self, layer: int, q, seqs, cu=None, max_q: int = 1, window: int = 0, sinks: int = 0,
@@ -246,33 +230,35 @@ class KvCache:
         n, (t, heads, _) = seqs.shape[0], q.shape
         cu_ptr = self._cu(cu, n, t)  # cu itself stays referenced: what is allocated below must not take its memory
         out, o_row, o_head = _out(out, q, dev)
-        lse = _torch_module.empty(t, heads, dtype=_torch_module.float32, device=q.device) if return_lse else None
+        lse = q.new_empty((t, heads), dtype=_torch_module.float32) if return_lse else None
         _ATTN.pack_into(self._args, 0, q.data_ptr(), 0, 0, out.data_ptr(), lse.data_ptr() if return_lse else 0,
                         seqs.data_ptr(), cu_ptr or 0, 0, q_row, q_head, 0, 0, 0, 0, o_row, o_head, n, t, _count(max_q, "max_q"), heads,
                         self.kv_heads, self.head_dim, _dtype_codes[q.dtype], 1, _count(window, "window"),
                         _count(sinks, "sinks"), self._scale if scale is None else scale, _count(layer, "layer"))
-        with self._ordered:
-            check(dev.ptr, dev.lib.mrl_kv_attend(dev.ptr, self._p, self._args_p))
+        _call(dev, dev.lib.mrl_kv_attend, self._p, self._args_p)
         return (out, lse) if return_lse else out
 
 
-def _status(dev: Device, like):
-    """The device's status word for calls without a cache (Device.attention_status): KV_TIMEOUT or 0."""
-    if dev.attention_status is None:
-        dev.attention_status = _torch_module.zeros(1, dtype=_torch_module.int32, device=like.device)
-    return dev.attention_status
+def _call_buffer(dev: Device, like):
+    """What a device's calls without a cache keep: the argument struct, its address, and the status
+    word (Device.attention_status: KV_TIMEOUT or 0)."""
+    dev.attention_status = _torch_module.zeros(1, dtype=_torch_module.int32, device=like.device)
+    buf = bytearray(_ATTN.size)
+    dev.attention_call = (buf, C.addressof((C.c_char * _ATTN.size).from_buffer(buf)), dev.attention_status)
+    return dev.attention_call
 
 
 def _count(x, name: str) -> int:
-    x = int(x)
-    if not 0 <= x < 1 << 31:
+    if type(x) is not int:
+        x = int(x)
+    if not 0 <= x < 2147483648:
         raise ValueError(f"{name} must be in [0, 2^31)")
     return x
 
 
 def _out(out, q, dev: Device):
     if out is None:
-        out = _torch_module.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(q.shape)
         return out, q.shape[1] * q.shape[2], q.shape[2]
     return (out, *_rows(out, "out", dev, q.shape[1], q.shape[2], q.dtype, q.shape[0]))
 
@@ -293,12 +279,11 @@ def window_attention(q, k, v, cu, max_len: int, causal: bool = True, window: int
     if cu.shape[0] < 1:
         raise ValueError("cu must have one entry more than there are sequences")
     out, o_row, o_head = _out(out, q, dev)
-    lse = torch.empty(t, heads, dtype=torch.float32, device=q.device) if return_lse else None
-    a = AttnC(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0, 0, cu.data_ptr(),
-              _status(dev, q).data_ptr(),
-              q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, cu.shape[0] - 1, t, _count(max_len, "max_len"), heads,
-              k.shape[1], d, _dtype_codes[q.dtype], int(bool(causal)), _count(window, "window"), _count(sinks, "sinks"),
-              1.0 / math.sqrt(d) if scale is None else scale, 0)
-    with _Ordered(dev):
-        check(dev.ptr, dev.lib.mrl_window_attention(dev.ptr, C.byref(a)))
+    lse = q.new_empty((t, heads), dtype=torch.float32) if return_lse else None
+    buf, ptr, status = dev.attention_call or _call_buffer(dev, q)
+    _ATTN.pack_into(buf, 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0, 0,
+                    cu.data_ptr(), status.data_ptr(), q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head,
+                    cu.shape[0] - 1, t, _count(max_len, "max_len"), heads, k.shape[1], d, _dtype_codes[q.dtype], 1 if causal else 0,
+                    _count(window, "window"), _count(sinks, "sinks"), 1.0 / math.sqrt(d) if scale is None else scale, 0)
+    _call(dev, dev.lib.mrl_window_attention, ptr)
     return (out, lse) if return_lse else out
