@@ -21,6 +21,8 @@
 // products against 2 x 16384 exponentials at 16 per clock and SM.
 #include <cuda.h>
 
+#include <algorithm>
+
 #include "kv.cuh"
 #include "umma.cuh"
 
@@ -1073,7 +1075,8 @@ template <class T, int D, bool PAGED> int launch(TcParams p, int sms, cudaStream
             if (const cudaError_t e = cudaGetLastError()) return (int)e;
         }
         // at most one part-filled item per sequence and head
-        const uint64_t most = ((uint64_t)a.n_tokens / (S::tiles * p.tokens) + p.a.n_seqs) * p.heads;
+        const uint64_t span = (uint64_t)S::tiles * p.tokens, each = (a.max_rows + span - 1) / span;
+        const uint64_t most = std::min(a.n_tokens / span + p.a.n_seqs, p.a.n_seqs * each) * p.heads;
         tc_kernel<T, D, PAGED><<<(unsigned)(most < (uint64_t)sms ? most : sms), S::threads, S::smem, s>>>(p, mq, mk, mv);
         if (const cudaError_t e = cudaGetLastError()) return (int)e;
     }

@@ -102,6 +102,24 @@ int kv_image(mrl_ctx* ctx, size_t bytes, void** out) {
     return MRL_OK;
 }
 
+// Whether mrl_kv_attend widens the pages and runs 128-row tiles (attend_tc.cu) instead of 16-row items on the codes
+// (kv_decode.cu). A sequence whose rows are one item reads its pages once either way: always the latter. Else
+// the smaller estimate, in ns per 128 keys of every sequence: an item pays for each of its pages, all SMs
+// together; a tile pair (a tile, head_dim 256) for each step on its SM, and widening each page once. Measured us,
+// items / tiles, 8 kv heads of 128, group 4: 8 sequences of 8,000 with 64 rows 116 / 220, with 128 204 / 224, with
+// 256 372 / 246, with 512 706 / 249; one of 30,000 with 512 rows 332 / 549. 64 sequences of 1,000, 8 heads of 64,
+// group 2: 64 rows 75 / 135, 128 135 / 137, 256 260 / 164. 8 of 4,000, 2 heads of 256, group 4: 128 rows 92 / 138, 256
+// 154 / 141.
+bool tensor_cores(const mrl_ctx* ctx, const mrl_kv_cache& kv, const mrl_attn& a) {
+    const uint64_t group = a.q_heads / kv.kv_heads, rows = a.n_tokens * group, heads = kv.kv_heads, sms = (uint64_t)ctx->sms;
+    if (!a.cu || a.max_rows * group <= 16) return false;
+    const uint64_t per_page = kv.head_dim == 64 ? 630 : kv.head_dim == 128 ? 810 : 2600;  // of one SM, for two pages
+    const uint64_t per_step = kv.head_dim == 64 ? 1700 : kv.head_dim == 128 ? 2100 : 2700, widen = kv.head_dim * 118ull / 1000;
+    const uint64_t items = std::max<uint64_t>(a.n_seqs, rows / 16) * heads;
+    const uint64_t tiles = std::max<uint64_t>(a.n_seqs, rows / (kv.head_dim == 256 ? 128 : 256)) * heads;
+    return items * per_page / sms > (tiles + sms - 1) / sms * per_step + a.n_seqs * heads * widen;
+}
+
 // Windows and sinks beyond any sequence (2^28 rows) all mean the same; cut, sums with positions stay in an int.
 mrl_attn cut(const mrl_attn& a) {
     mrl_attn b = a;
@@ -238,7 +256,7 @@ int mrl_kv_attend(mrl_ctx* ctx, const mrl_kv_cache* kv, const mrl_attn* a) {
         if (a->layer >= kv->layers) return bad(ctx, "layer is not one of the cache's");
         if (int rc = check_attn(ctx, a, kv->kv_heads, kv->head_dim, true)) return rc;
         if (a->n_tokens == 0) return MRL_OK;
-        if (a->cu && (uint64_t)a->max_rows * (a->q_heads / kv->kv_heads) > 64) {
+        if (tensor_cores(ctx, *kv, *a)) {
             void* wide;
             if (int rc = kv_image(ctx, mrl::kv_wide_bytes(*kv), &wide)) return rc;
             return done(ctx, mrl::launch_attend_tc(kv, cut(*a), ctx->sms, wide, ctx->stream), "mrl_kv_attend");

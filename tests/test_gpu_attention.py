@@ -54,21 +54,21 @@ def plain_attention(q, k, v, first, causal, window, sinks, scale, present=None):
     t, hq, d = q.shape
     n, h, _ = k.shape
     out, lse, big = np.zeros((t, hq, d)), np.full((t, hq), -np.inf), 0.0
-    for i in range(t):
-        ok = visible(first + i, n, causal, window, sinks)
-        if present is not None:
-            ok &= present
-        idx = np.nonzero(ok)[0]
-        if idx.size == 0:
-            continue
-        for a in range(hq):
-            kk, vv = k[idx, a // (hq // h)], v[idx, a // (hq // h)]
-            s = kk @ q[i, a] * scale
-            big = max(big, float((np.abs(kk) @ np.abs(q[i, a])).max() * scale))
-            m = s.max()
-            w = np.exp(s - m)
-            out[i, a] = w @ vv / w.sum()
-            lse[i, a] = m + math.log(w.sum())
+    if t == 0 or n == 0:
+        return out, lse, big
+    ok = np.stack([visible(first + i, n, causal, window, sinks) for i in range(t)])
+    if present is not None:
+        ok &= present
+    some = ok.any(1)
+    for a in range(hq):
+        kk, vv = k[:, a // (hq // h)], v[:, a // (hq // h)]
+        s = np.where(ok, q[:, a] @ kk.T * scale, -np.inf)
+        big = max(big, float(np.where(ok, np.abs(q[:, a]) @ np.abs(kk).T, 0).max() * scale))
+        m = np.where(some, s.max(1), 0.0)
+        w = np.exp(s - m[:, None])
+        total = w.sum(1)
+        out[:, a] = w @ vv / np.where(some, total, 1.0)[:, None]
+        lse[some, a] = m[some] + np.log(total[some])
     return out, lse, big
 
 
@@ -842,3 +842,84 @@ def test_refusals(M, dev):
     assert cache.read(0, none)[0].shape == (0, 2, 64)
     assert M.window_attention(half(0, 2, 64), half(0, 2, 64), half(0, 2, 64), i32([0]), 0, dev=dev).shape == (0, 2, 64)
     assert int(cache.status) == 0
+
+
+# ---- attention of many rows over the cache (the pages widened first, 128-row tiles) ------------------------------
+
+MANY_LENS = [0, 1, 5, 64, 66, 131, 300, 520, 900, 1300]
+MANY_ROWS = [0, 1, 5, 64, 2, 0, 300, 400, 900, 1000]
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("h,g,window,sinks", [(2, 4, 0, 0), (4, 3, 0, 0), (2, 4, 100, 70), (1, 17, 33, 0), (3, 4, 400, 4), (8, 1, 1, 1)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_attend_many_rows(M, dev, d, h, g, window, sinks, dtype):
+    rng = np.random.default_rng(d + h + g + window)
+    run_attend(M, dev, rng, MANY_LENS, MANY_ROWS, h, g, d, dtype, window, sinks)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attend_many_rows_missing_pages(M, dev, d):
+    """Pages that are gone in the middle, out-of-range entries, a sequence without any, sequences out of range."""
+    rng = np.random.default_rng(d)
+    cache, codes, scales, tables = filled_cache(M, rng, dev, MANY_LENS, 2, d)
+    tables[9, 1], tables[9, 4], tables[8, 2], tables[8, 3] = -1, 1 << 28, -7, -1
+    tables[6, :] = -1
+    cache.tables.copy_(torch.from_numpy(tables))
+    q = torch.from_numpy(rng.normal(0, 1, (sum(MANY_ROWS), 8, d))).half().cuda()
+    out, lse = cache.attend(0, q, i32(range(10)), cu_of(MANY_ROWS), max_q=1000, return_lse=True)
+    verify(cache, codes[0], scales[0], tables, MANY_LENS, range(10), MANY_ROWS, q, out, lse, 0, 0)
+    seqs = list(range(10))
+    seqs[9], seqs[7] = -1, 1 << 30
+    out2, lse2 = cache.attend(0, q, i32(seqs), cu_of(MANY_ROWS), max_q=1000, return_lse=True)
+    cu = np.concatenate([[0], np.cumsum(MANY_ROWS)])
+    for i in (7, 9):
+        assert bool((out2[cu[i]:cu[i + 1]] == 0).all()) and bool((lse2[cu[i]:cu[i + 1]] == -math.inf).all())
+    assert torch.equal(out2[cu[8]:cu[9]], out[cu[8]:cu[9]])
+
+
+def test_attend_many_rows_shared_pages(M, dev):
+    """Forks: a prefix that many sequences share is widened once, their own tails each."""
+    rng = np.random.default_rng(21)
+    n, h, g, d = 40, 2, 4, 64
+    cache = M.KvCache.create(2, 120, h, d, n + 1, 8, dev=dev)
+
+    def extend(seqs, counts):
+        cache.reserve(i32(seqs), i32(counts))
+        for layer in range(2):
+            kv = torch.from_numpy(rng.normal(0, 1, (sum(counts), 2, h, d))).half().cuda()
+            cache.append(layer, kv[:, 0], kv[:, 1], i32(seqs), cu_of(counts))
+
+    extend([0], [150])
+    kids = list(range(1, n + 1))
+    cache.fork(i32([0] * n), i32(kids))
+    counts = [int(x) for x in rng.integers(20, 100, n)]
+    extend(kids, counts)
+    assert int(cache.refs.max()) == n + 1
+    q = torch.from_numpy(rng.normal(0, 1, (sum(counts), h * g, d))).half().cuda()
+    for layer in range(2):
+        out, lse = cache.attend(layer, q, i32(kids), cu_of(counts), max_q=100, return_lse=True)
+        verify(cache, cache.codes[layer].cpu().numpy(), cache.scales[layer].cpu().numpy(), cache.tables.cpu().numpy(),
+               [int(x) for x in cache.lens], kids, counts, q, out, lse, 0, 0)
+
+
+def test_attend_many_rows_again_and_strided(M, dev):
+    rng = np.random.default_rng(22)
+    cache, codes, scales, tables = filled_cache(M, rng, dev, MANY_LENS, 2, 128)
+    wide = torch.from_numpy(rng.normal(0, 1, (sum(MANY_ROWS), 17, 128))).bfloat16().cuda()[:, 1::2]
+    dst = torch.full((sum(MANY_ROWS), 9, 136), 7.0, dtype=torch.bfloat16, device="cuda")
+    out, lse = cache.attend(0, wide, i32(range(10)), cu_of(MANY_ROWS), max_q=1000, out=dst[:, 1:, :128], return_lse=True)
+    verify(cache, codes[0], scales[0], tables, MANY_LENS, range(10), MANY_ROWS, wide, out, lse, 0, 0)
+    assert bool((dst[:, 0] == 7.0).all()) and bool((dst[:, :, 128:] == 7.0).all())
+    first = out.clone()
+    for _ in range(4):
+        assert torch.equal(first, cache.attend(0, wide, i32(range(10)), cu_of(MANY_ROWS), max_q=1000))
+
+
+def test_attend_more_sequences_than_a_launch_holds(M, dev):
+    """1,300 sequences of one row and of several: more than one launch's table of sequences."""
+    rng = np.random.default_rng(23)
+    lens = [int(x) for x in rng.integers(1, 90, 1300)]
+    run_attend(M, dev, rng, lens, [1] * 1300, 1, 2, 64, torch.float16)
+    run_attend(M, dev, rng, lens, [min(x, 40) for x in lens], 1, 8, 64, torch.float16)
+    run_window(M, dev, rng, lens, 1, 2, 64, torch.float16, True, 0, 0)
