@@ -17,8 +17,15 @@
 // a first launch has widened to f16 (exact) in the operand layout, once for all the tiles that read them, and
 // warps 10 and 11 bring in Q as f16; the blocks' scales go to S and P, which are f32 there. Every wait is bounded; when one runs out the kernel records it and ends.
 //
-// Bound by the tensor core and the exponentials together: per 128 x 128 x D tile pair 2 x 2 x 128 x 128 x D
-// products against 2 x 16384 exponentials at 16 per clock and SM.
+// Bounds: per 128 keys a tile pair needs 2 x 2 x 128 x 128 x D products (2,048 clocks at head_dim 128) and 2 x 16,384
+// exponentials and as many conversions (about 2,560). What a pair takes is the chain of one tile's step, about 3,500
+// clocks, the other tile in the gaps: S into registers 200, maximum 250, P 1,270, hand-over 100, P V and the next S
+// 1,100, waits. Measured on one B200, full attention over 2 x 8,192 tokens: 16 heads of 128 in bf16 928 us, 1,184
+// TFLOP/s (tensor pipe 54% active); 16 heads of 64 in f16 819 us, 671; 8 heads of 256 in bf16 1,199 us, 917; causal
+// with a window of 1,024 and 4 sinks, 16 query heads on 4, 209 us. The rows of two tiles rather than one per CTA halve
+// the traffic of K and V from L2 (64 KB per step); 128 keys a step is what tensor memory holds beside two O.
+// The instructions' operands have to be in uniform registers: issued from one divergent lane, each product cost
+// 75 clocks and the same kernel ran at 972 instead of 1,097 TFLOP/s.
 #include <cuda.h>
 
 #include <algorithm>
@@ -943,33 +950,39 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
 // The pages that the call's sequences see, codes to f16 in the operands' layout: every 64 codes of K (a
 // token's dims 64 i ..) or V (a dim's tokens) become a swizzled row of 128 bytes. A page that several
 // sequences share lies at the same index of their tables after a fork: the first of them widens it.
-// Bound by HBM: 1 byte read, 2 written per code.
-constexpr int kWidenThreads = 256, kWidenSeqs = 1024;
+// 1 byte read, 2 written per code; a CTA takes several blocks of a page at a time, all their loads at once, since
+// the way to a page (sequence, table, refs) is a chain of dependent loads. Measured, 324 pages of 8 kv heads of
+// 128 (42 MB of codes, 127 MB in all): 20.5 us, 6.2 TB/s; 31 us with 16-byte stores.
+constexpr int kWidenThreads = 256, kWidenSeqs = 512;
 template <int D> __global__ void __launch_bounds__(kWidenThreads) widen_kernel(mrl_kv_cache c, mrl_attn a, unsigned char* wide) {
+    constexpr int kBlocks = D == 256 ? 2 : 4;                             // blocks of 64 x D codes per turn
+    constexpr int kPieces = kPage * D / 16 / kWidenThreads;               // of a thread, per block
+    struct Seen {
+        int seq, head, lo, n;  // visible pages [0, head) and [lo, lo + n - head)
+    };
+    __shared__ Seen seen[kWidenSeqs];
     __shared__ unsigned start[kWidenSeqs];
     __shared__ unsigned scan_s[kWidenThreads / 32];
     __shared__ int skip_s;
     const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5, n = (int)a.n_seqs, window = (int)a.window, sinks = (int)a.sinks;
     const Rows rows{a.seqs, a.cu, n, (int)a.n_tokens};
-    struct Seen {
-        int seq, head, lo, n;  // visible pages [0, head) and [lo, lo + n - head)
-    };
-    auto seen = [&](int b) {
-        const int seq = a.seqs[b], m = rows.end(b) - rows.begin(b);
-        Seen s{seq, 0, 0, 0};
-        if (seq < 0 || seq >= (int)c.max_seqs || m <= 0) return s;
-        const int len = min(max(c.lens[seq], 0), (int)c.max_pages * kPage);
-        const Span v = visible(max(len - m, 0), len, 1, window, sinks);  // the first row sees the earliest
-        s.lo = min(v.lo, len) / kPage;
-        s.head = min(pages_of(min(sinks, v.lo)), s.lo);
-        s.n = s.head + pages_of(len) - s.lo;
-        return s;
-    };
     unsigned carry = 0;
     for (int at = 0; at < n; at += kWidenThreads) {
         const int b = at + tid;
-        const unsigned v = b < n ? (unsigned)seen(b).n : 0;
-        unsigned x = v;
+        Seen s{0, 0, 0, 0};
+        if (b < n) {
+            const int seq = a.seqs[b], m = rows.end(b) - rows.begin(b);
+            if (seq >= 0 && seq < (int)c.max_seqs && m > 0) {
+                const int len = min(max(c.lens[seq], 0), (int)c.max_pages * kPage);
+                const Span v = visible(max(len - m, 0), len, 1, window, sinks);  // the first row sees the earliest
+                s.seq = seq;
+                s.lo = min(v.lo, len) / kPage;
+                s.head = min(pages_of(min(sinks, v.lo)), s.lo);
+                s.n = s.head + pages_of(len) - s.lo;
+            }
+            seen[b] = s;
+        }
+        unsigned x = (unsigned)s.n;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const unsigned y = __shfl_up_sync(~0u, x, d);
@@ -982,47 +995,61 @@ template <int D> __global__ void __launch_bounds__(kWidenThreads) widen_kernel(m
             if (w < warp) before += scan_s[w];
             carry += scan_s[w];
         }
-        if (b < n) start[b] = before + x - v;
+        if (b < n) start[b] = before + x - (unsigned)s.n;
         __syncthreads();
     }
-    const unsigned heads = 2 * c.kv_heads, units = carry * heads;  // one block of 64 x D codes each
+    const unsigned heads = 2 * c.kv_heads, turns = (heads + kBlocks - 1) / kBlocks, units = carry * turns;
     for (unsigned u = blockIdx.x; u < units; u += gridDim.x) {
-        const unsigned p = u / heads, block = u % heads;
+        const unsigned p = u / turns, block0 = u % turns * kBlocks;
         int lo = 0, hi = n;
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
             if (start[mid] <= p) lo = mid;
             else hi = mid;
         }
-        const Seen s = seen(lo);
+        const Seen s = seen[lo];
         const int i = (int)(p - start[lo]), index = i < s.head ? i : s.lo + i - s.head;
         const int page = c.tables[(size_t)s.seq * c.max_pages + index];
         if (page < 0 || page >= (int)c.pages) continue;
+        const uint4* src = reinterpret_cast<const uint4*>(c.codes + (block_index(c, a.layer, page, 0, 0) + block0) * (size_t)(kPage * D));
+        uint4 w[kBlocks][kPieces];
+#pragma unroll
+        for (int k = 0; k < kBlocks; ++k)
+#pragma unroll
+            for (int x = 0; x < kPieces; ++x)
+                if (block0 + k < heads) w[k][x] = src[k * (kPage * D / 16) + x * kWidenThreads + tid];
         if (c.refs[page] > 1) {
             __syncthreads();
             if (tid == 0) skip_s = 0;
             __syncthreads();
             for (int b = tid; b < lo; b += kWidenThreads) {
-                const Seen o = seen(b);
+                const Seen o = seen[b];
                 const bool has = index < o.head || (index >= o.lo && index < o.lo + o.n - o.head);
                 if (has && c.tables[(size_t)o.seq * c.max_pages + index] == page) skip_s = 1;
             }
             __syncthreads();
             if (skip_s) continue;
         }
-        const uint4* src = reinterpret_cast<const uint4*>(c.codes + (block_index(c, a.layer, page, 0, 0) + block) * (size_t)(kPage * D));
-        unsigned char* dst = wide + ((size_t)page * heads + block) * (kPage * D * 2);
+        unsigned char* dst = wide + ((size_t)page * heads + block0) * kWide<D>;
 #pragma unroll
-        for (int x = 0; x < kPage * D / 16 / kWidenThreads; ++x) {
-            const int k = x * kWidenThreads + tid, line = k >> 2, quarter = k & 3, sw = line & 7;
-            const uint4 w = src[k];
-            uint4 e0, e1;
-            widen4(w.x, e0.x, e0.y);
-            widen4(w.y, e0.z, e0.w);
-            widen4(w.z, e1.x, e1.y);
-            widen4(w.w, e1.z, e1.w);
-            *reinterpret_cast<uint4*>(dst + line * 128 + (((2 * quarter) ^ sw) << 4)) = e0;
-            *reinterpret_cast<uint4*>(dst + line * 128 + (((2 * quarter + 1) ^ sw) << 4)) = e1;
+        for (int k = 0; k < kBlocks; ++k) {
+#pragma unroll
+            for (int x = 0; x < kPieces; ++x) {
+                if (block0 + k >= heads) continue;
+                const int at = x * kWidenThreads + tid, line = at >> 2, quarter = at & 3, sw = line & 7;
+                uint4 e0, e1;
+                widen4(w[k][x].x, e0.x, e0.y);
+                widen4(w[k][x].y, e0.z, e0.w);
+                widen4(w[k][x].z, e1.x, e1.y);
+                widen4(w[k][x].w, e1.z, e1.w);
+                // the two chunks are one 32-byte sector, written as one: halves apart would be merged in L2
+                unsigned char* to = dst + k * kWide<D> + line * 128 + ((((2 * quarter) ^ sw) >> 1) << 5);
+                const bool odd = sw & 1;
+                const uint4 f0 = odd ? e1 : e0, f1 = odd ? e0 : e1;
+                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(f0.x), "r"(f0.y), "r"(f0.z), "r"(f0.w), "r"(f1.x),
+                             "r"(f1.y), "r"(f1.z), "r"(f1.w)
+                             : "memory");
+            }
         }
     }
 }

@@ -4,7 +4,9 @@
 // moved by a second launch over the whole device.
 //
 // A fork or a compact has to read and write each copied page once (2 x layers x 2 x kv_heads x 64 x
-// head_dim bytes a page): bound by HBM for large ones, by the two launches for small ones.
+// head_dim bytes a page): bound by HBM for large ones, by the two launches for small ones. Measured, 8 kv heads of 128: 48
+// forks over 8 layers 5.3 us for the plan and 11.8 us for the tails (50 MB written, their 8 sources in L2); a compact that moves
+// 116 MB 5.3 and 35 us (6.6 TB/s read and written); a reserve of 24 sequences 6.5 us; a release 2.7 us.
 #include "kv.cuh"
 
 namespace mrl {
