@@ -19,6 +19,8 @@
 // of 2,304 59 us (3.84), 8 of 1,000 13.2 us, one of 37 9.8 us; 64 of 2,000, 4 kv heads of 256, 88 us (2.99); 128 of 8,000
 // through a window of 1,024, 8 kv heads of 64, 40 us (3.35). About 25 us of the long ones are not the stream: 4 until the
 // work is dealt out, 3.5 until the first page is there, 7 for joining the pieces of split items, the rest uneven ends.
+#include <algorithm>
+
 #include "kv.cuh"
 
 namespace mrl {
@@ -130,10 +132,10 @@ __device__ __forceinline__ float quad_sum(float x) {
     return x + __shfl_xor_sync(~0u, x, 2);
 }
 
-// How the launch's pages are dealt out to its teams.
+// How the launch's pages are dealt out to its teams: runs of consecutive warps of a CTA.
 struct Plan {
     unsigned units;  // pages of all items
-    int teams, width;  // teams of the launch, warps per team
+    int teams;       // of the launch
     bool few;        // short launch: jobs instead of equal shares of the units
 };
 
@@ -144,8 +146,9 @@ struct Segment {
     int parts, part, first;  // pieces the item is in, this one's number, and the first one's team (or job)
 };
 
-template <class T, int D> __global__ void __launch_bounds__(kWarps<D> * 32, 1) decode_kernel(Params pr) {
-    constexpr int NW = kWarps<D>, kThreads = NW * 32, kBlock = kPage * D;
+// WIDE: teams of kWidest warps, for few items; else every warp is a team.
+template <class T, int D, bool WIDE> __global__ void __launch_bounds__(kWarps<D> * 32, 1) decode_kernel(Params pr) {
+    constexpr int W = WIDE ? kWidest<D> : 1, NW = kWarps<D>, kThreads = NW * 32, kBlock = kPage * D;
     extern __shared__ __align__(1024) unsigned char smem[];
     unsigned char* ring = smem;                                              // per warp: K block, V block
     float* acc_s = reinterpret_cast<float*>(ring + (size_t)NW * 2 * kBlock);  // per warp 16 rows of kAccStride
@@ -153,7 +156,7 @@ template <class T, int D> __global__ void __launch_bounds__(kWarps<D> * 32, 1) d
     uint64_t* bars = reinterpret_cast<uint64_t*>(ml_s + NW * 32);            // per warp {K, V}
     SeqInfo* info = reinterpret_cast<SeqInfo*>(bars + NW * 2);               // [n]
     int* seq_s = reinterpret_cast<int*>(info + pr.a.n_seqs);                 // [n] table row, or -1
-    __shared__ unsigned scan_s[NW][2];
+    __shared__ unsigned scan_s[NW];
     __shared__ unsigned arrived_s[NW];
 
     const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -170,7 +173,7 @@ template <class T, int D> __global__ void __launch_bounds__(kWarps<D> * 32, 1) d
 
     // ---- the call's sequences: their items and pages, summed up
     const Rows rows{a.seqs, a.cu, n, (int)a.n_tokens};
-    unsigned my_items = 0, my_units = 0;
+    unsigned my_units = 0;
     for (int b = tid; b < n; b += kThreads) {
         SeqInfo s;
         s.row = a.cu ? rows.begin(b) : pr.row0 + b;
@@ -181,44 +184,28 @@ template <class T, int D> __global__ void __launch_bounds__(kWarps<D> * 32, 1) d
         seq_s[b] = known ? seq : -1;
         s.start = 0;
         info[b] = s;
-        if (s.m > 0) {
-            const unsigned items = (unsigned)((s.m * group + 15) / 16) * c.kv_heads;
-            my_items += items;
-            my_units += items * (unsigned)max(1, page_span(s.len, s.m, window, sinks).n);
-        }
+        if (WIDE && s.m > 0)
+            my_units += (unsigned)((s.m * group + 15) / 16) * c.kv_heads * (unsigned)max(1, page_span(s.len, s.m, window, sinks).n);
     }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) {
-        my_items += __shfl_xor_sync(~0u, my_items, d);
-        my_units += __shfl_xor_sync(~0u, my_units, d);
-    }
-    if (lane == 0) {
-        scan_s[warp][0] = my_items;
-        scan_s[warp][1] = my_units;
-    }
-    __syncthreads();
-    unsigned items = 0;
     Plan pl;
     pl.units = 0;
+    if constexpr (WIDE) {
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-        items += scan_s[w][0];
-        pl.units += scan_s[w][1];
+        for (int d = 16; d; d >>= 1) my_units += __shfl_xor_sync(~0u, my_units, d);
+        if (lane == 0) scan_s[warp] = my_units;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < NW; ++w) pl.units += scan_s[w];
     }
-    if (pl.units == 0) return;
-    // Warps per team: an item's share of the launch's warps, so that an item is in few pieces, none of
-    // them joined by fewer threads than it has to (few items: whole CTAs; many: each warp on its own).
-    pl.width = kWidest<D>;
-    while (pl.width > 1 && items * pl.width > gridDim.x * (unsigned)NW) pl.width >>= 1;
-    const int per_cta = NW / pl.width;
-    pl.teams = (int)gridDim.x * per_cta;
-    // With no more than a page per warp an item's pieces are whole jobs, so that short items are not split
-    // at a team's border; beyond that every team takes an equal run of pages.
-    pl.few = pl.units <= (unsigned)(pl.teams * pl.width);
+    pl.teams = (int)gridDim.x * (NW / W);
+    // Few items with no more than a page per warp are dealt out in whole jobs, so that short ones are not split at a
+    // team's border; beyond that every team takes an equal share. Measured, 8 sequences of 1,000 tokens and 8 kv heads
+    // of 128: 12.0 us with jobs, 15.1 us with shares.
+    pl.few = WIDE && pl.units <= (unsigned)(pl.teams * W);
     __syncthreads();  // scan_s is read
     // An item costs its pages and a fixed part (Q, joining, writing: about 1.5 pages' time of a warp), so equal
     // shares are of pages + `fixed` per item. A share that would begin in an item's fixed part begins with the item.
-    const unsigned fixed = pl.few ? 0 : (unsigned)(3 * pl.width + 1) / 2;
+    const unsigned fixed = pl.few ? 0 : (unsigned)(3 * W + 1) / 2;
     // Exclusive sums over the sequences of their items' cost, or of their jobs.
     unsigned carry = 0;
     for (int at = 0; at < n; at += kThreads) {
@@ -226,7 +213,7 @@ template <class T, int D> __global__ void __launch_bounds__(kWarps<D> * 32, 1) d
         unsigned v = 0;
         if (b < n && info[b].m > 0) {
             const int np = max(1, page_span(info[b].len, info[b].m, window, sinks).n);
-            v = (unsigned)((info[b].m * group + 15) / 16) * c.kv_heads * (pl.few ? (unsigned)((np + pl.width - 1) / pl.width) : np + fixed);
+            v = (unsigned)((info[b].m * group + 15) / 16) * c.kv_heads * (pl.few ? (unsigned)((np + W - 1) / W) : np + fixed);
         }
         unsigned x = v;
 #pragma unroll
@@ -234,21 +221,25 @@ template <class T, int D> __global__ void __launch_bounds__(kWarps<D> * 32, 1) d
             const unsigned y = __shfl_up_sync(~0u, x, d);
             if (lane >= d) x += y;
         }
-        if (lane == 31) scan_s[warp][0] = x;
+        if (lane == 31) scan_s[warp] = x;
         __syncthreads();
         unsigned before = carry;
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
-            if (w < warp) before += scan_s[w][0];
-            carry += scan_s[w][0];
+            if (w < warp) before += scan_s[w];
+            carry += scan_s[w];
         }
         if (b < n) info[b].start = before + x - v;
         __syncthreads();
     }
     const unsigned total = carry;  // cost of the launch, or its jobs
+    if (total == 0) return;
+    if (!pl.few) pl.teams = (int)min((unsigned)pl.teams, total);  // no share is empty: an item's pieces are those of consecutive teams
 
     // ---- this team's share
-    const int team = warp / pl.width, w_in = warp % pl.width, threads = pl.width * 32, t_in = w_in * 32 + lane;
+    const int team = warp / W, w_in = warp % W;
+    constexpr int threads = W * 32;
+    const int t_in = w_in * 32 + lane;
     const unsigned t_all = blockIdx.x + (unsigned)team * gridDim.x;  // neighbours in work on different SMs
     // Sequence of position x: the last one that starts at or before it, which passes over those without work.
     auto seq_at = [&](unsigned x) {
@@ -305,7 +296,7 @@ template <class T, int D> __global__ void __launch_bounds__(kWarps<D> * 32, 1) d
             if (w.job >= total) return false;
             w.at.b = seq_at(w.job);
             enter(w);
-            const int k = (w.np + pl.width - 1) / pl.width;
+            const int k = (w.np + W - 1) / W;
             const unsigned local = w.job - info[w.at.b].start;
             const int item = (int)(local / (unsigned)k), piece = (int)(local % (unsigned)k);
             s.b = w.at.b;
@@ -361,7 +352,7 @@ template <class T, int D> __global__ void __launch_bounds__(kWarps<D> * 32, 1) d
     auto look_up = [&]() {
         raw_page = -1;
         if (!more) return;
-        if (!fresh) ai += pl.width;
+        if (!fresh) ai += W;
         while (fresh || ai >= as.p1) {
             fresh = false;
             if (!next_segment(awalk, as)) {
@@ -459,7 +450,7 @@ template <class T, int D> __global__ void __launch_bounds__(kWarps<D> * 32, 1) d
         for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
         float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f, vref = 0.0f;
 
-        for (int i = s.p0 + w_in; i < s.p1; i += pl.width) {
+        for (int i = s.p0 + w_in; i < s.p1; i += W) {
             const int page = npage, index = nindex;
             const float ks = nks, vs = nvs;
             advance();
@@ -606,7 +597,7 @@ template <class T, int D> __global__ void __launch_bounds__(kWarps<D> * 32, 1) d
         }
         team_sync(team, threads);
         const int tile_rows = min(16, rows_all - s.tile * 16);
-        const int w0 = team * pl.width;
+        const int w0 = team * W;
         auto emit = [&](int r, int d, float4 x, float m, float l) {
             const int row = s.tile * 16 + r;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -620,11 +611,11 @@ template <class T, int D> __global__ void __launch_bounds__(kWarps<D> * 32, 1) d
         for (int i = t_in; i < tile_rows * (D / 4); i += threads) {
             const int r = i / (D / 4), d = i % (D / 4) * 4;
             float m = -INFINITY;
-            for (int w = 0; w < pl.width; ++w) m = fmaxf(m, ml_s[((w0 + w) * 16 + r) * 2]);
+            for (int w = 0; w < W; ++w) m = fmaxf(m, ml_s[((w0 + w) * 16 + r) * 2]);
             const float z = m == -INFINITY ? 0.0f : m;
             float l = 0.0f;
             float4 x = make_float4(0, 0, 0, 0);
-            for (int w = 0; w < pl.width; ++w) {
+            for (int w = 0; w < W; ++w) {
                 const float k = ex2(ml_s[((w0 + w) * 16 + r) * 2] - z);
                 const float4 y = *reinterpret_cast<const float4*>(acc_s + ((w0 + w) * 16 + r) * kAccStride<D> + d);
                 l = fmaf(k, ml_s[((w0 + w) * 16 + r) * 2 + 1], l);
@@ -697,8 +688,19 @@ template <class T, int D> cudaError_t launch(const Params& p, int sms, cudaStrea
     constexpr int NW = kWarps<D>;
     const size_t smem = (size_t)NW * 2 * kPage * D + sizeof(float) * NW * 16 * kAccStride<D> + sizeof(float) * NW * 32 + 16 * NW +
                         (sizeof(SeqInfo) + sizeof(int)) * p.a.n_seqs;
-    if (const cudaError_t e = allow_smem<decode_kernel<T, D>>(232448 - 2048)) return e;
-    decode_kernel<T, D><<<sms, NW * 32, smem, s>>>(p);
+    // Teams of a whole CTA (4 warps, head_dim 64) where there is no more than an item per SM: an item is then in few
+    // pieces, joined in shared memory; single warps beyond, which need no joining. Measured us, teams / warps: 8 kv heads
+    // of 128, 8 sequences of 1,000 12.0 / 19.7, one of 130,000 55 / 124, 4 of 130,000 174 / 192, 48 of 2,300 59 / 52.5, 256 of
+    // 512 90 / 63; 64 of 2,000 with 4 kv heads of 256 86 / 81.
+    const uint64_t group = p.a.q_heads / p.c.kv_heads;
+    const uint64_t tiles = p.a.cu ? std::max<uint64_t>(p.a.n_seqs, p.a.n_tokens * group / 16) : p.a.n_seqs * ((group + 15) / 16);
+    if (tiles * p.c.kv_heads <= (uint64_t)sms) {
+        if (const cudaError_t e = allow_smem<decode_kernel<T, D, true>>(232448 - 2048)) return e;
+        decode_kernel<T, D, true><<<sms, NW * 32, smem, s>>>(p);
+    } else {
+        if (const cudaError_t e = allow_smem<decode_kernel<T, D, false>>(232448 - 2048)) return e;
+        decode_kernel<T, D, false><<<sms, NW * 32, smem, s>>>(p);
+    }
     return cudaGetLastError();
 }
 
