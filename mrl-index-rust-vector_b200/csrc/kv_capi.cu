@@ -106,10 +106,10 @@ int kv_image(mrl_ctx* ctx, size_t bytes, void** out) {
 // (kv_decode.cu). A sequence whose rows are one item reads its pages once either way: always the latter. Else
 // the smaller estimate, in ns per 128 keys of every sequence: an item pays for each of its pages, all SMs
 // together; a tile pair (a tile, head_dim 256) for each step on its SM, and widening each page once. Measured us,
-// items / tiles, 8 kv heads of 128, group 4: 8 sequences of 8,000 with 64 rows 116 / 220, with 128 204 / 224, with
-// 256 372 / 246, with 512 706 / 249; one of 30,000 with 512 rows 332 / 549. 64 sequences of 1,000, 8 heads of 64,
-// group 2: 64 rows 75 / 135, 128 135 / 137, 256 260 / 164. 8 of 4,000, 2 heads of 256, group 4: 128 rows 92 / 138, 256
-// 154 / 141.
+// items / tiles, 8 kv heads of 128, group 4: 8 sequences of 8,000 with 64 rows 116 / 220, with 128 188 / 224, with
+// 256 372 / 228, with 512 706 / 232; one of 30,000 with 512 rows 327 / 549. 64 sequences of 1,000, 8 heads of 64,
+// group 2: 64 rows 71 / 135, 128 119 / 137, 256 260 / 148. 8 of 4,000, 2 heads of 256, group 4: 128 rows 88 / 138, 256
+// 154 / 134.
 bool tensor_cores(const mrl_ctx* ctx, const mrl_kv_cache& kv, const mrl_attn& a) {
     const uint64_t group = a.q_heads / kv.kv_heads, rows = a.n_tokens * group, heads = kv.kv_heads, sms = (uint64_t)ctx->sms;
     if (!a.cu || a.max_rows * group <= 16) return false;
