@@ -72,6 +72,7 @@ struct TcParams {
     mrl_attn a;
     int heads, group, tokens;  // kv heads, query heads per kv head, tokens per tile
     int causal;
+    int sectors;  // out and its strides are multiples of 32 bytes
     int inner_q, inner_k, inner_v;  // the map's second dimension is the row, not the head
     // over the cache: f16 image of the layer's pool, [pages][2][kv heads][wide], and a block of zeros. The image only
     // ever holds codes, so pages of it that a step touches but no row sees are finite.
@@ -208,6 +209,18 @@ __device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
     __half2 a = __hsub2(*reinterpret_cast<__half2*>(&x), off), b = __hsub2(*reinterpret_cast<__half2*>(&y), off);
     lo = *reinterpret_cast<uint32_t*>(&a);
     hi = *reinterpret_cast<uint32_t*>(&b);
+}
+
+// 32 bytes, as one sector where the output's rows are aligned to sectors.
+__device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8], int sectors) {
+    if (sectors) {
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+                     "r"(w[5]), "r"(w[6]), "r"(w[7])
+                     : "memory");
+    } else {
+        reinterpret_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        reinterpret_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
 }
 
 // Key steps of a tile: [0, head) and [lo, hi), of 128 keys each. Empty: hi == 0.
@@ -595,16 +608,15 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                         if (lane == 0) arrive(&o_free[tile]);
                     }
 #pragma unroll
-                    for (int k = 0; k < 32; k += 8) {
-                        uint4 y;
-                        uint32_t* w = &y.x;
+                    for (int k = 0; k < 32; k += 16) {
+                        uint32_t w[8];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
+                        for (int e = 0; e < 8; ++e) {
                             const float u = __uint_as_float(x[k + 2 * e]), v = __uint_as_float(x[k + 2 * e + 1]);
                             if (!PAGED) bad = fmaf(u, 0.0f, fmaf(v, 0.0f, bad));
                             w[e] = pack16<!__is_same(T, __half)>(l == 0.0f ? 0.0f : u * inv, l == 0.0f ? 0.0f : v * inv);
                         }
-                        if (in) *reinterpret_cast<uint4*>(dst + j * 32 + k) = y;
+                        if (in) store32(dst + j * 32 + k, w, pr.sectors);
                     }
                 }
             } else if (in) {
@@ -1132,6 +1144,7 @@ int launch_attend_tc(const mrl_kv_cache* c, const mrl_attn& a, int sms, void* wi
     p.heads = (int)(c ? c->kv_heads : a.kv_heads);
     p.group = (int)a.q_heads / p.heads;
     p.causal = c ? 1 : (int)(a.causal != 0);
+    p.sectors = reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.o_row % 16 == 0 && a.o_head % 16 == 0;
     p.inner_q = p.inner_k = p.inner_v = 0;
     return c ? kv::dispatch<true>(p, c->head_dim, sms, s) : kv::dispatch<false>(p, a.head_dim, sms, s);
 }
