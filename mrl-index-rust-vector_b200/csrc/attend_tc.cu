@@ -56,8 +56,8 @@ template <int D, bool PAGED> struct Shape {
     static constexpr int seqs = 512;  // sequences per launch (their table is in shared memory)
     static constexpr int threads = 12 * 32;
     // Registers: launched with 168 a thread, of which the two softmax warpgroups take more and the other gives up
-    // as many: 8 x 216 + 4 x 72 = 12 x 168.
-    static constexpr int regs_softmax = 216, regs_other = 72;
+    // as many: 8 x 208 + 4 x 88 = 12 x 168.
+    static constexpr int regs_softmax = 208, regs_other = 88;
     static constexpr int tmem_s = 0;                           // S (and P) columns of tile or buffer i at 128 i
     static constexpr int tmem_o = 256;                         // O columns of tile i at 256 + D i
     static constexpr size_t smem = 1024 + (size_t)tiles * q_bytes + 2 * stages * kv_bytes;
@@ -903,7 +903,7 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                 }
             };
             auto finish_q = [&](int t) {
-                constexpr int kTurn = 8;  // rows of a thread in flight
+                constexpr int kTurn = 4;  // rows of a thread in flight
                 for (int r0 = q_row; r0 < 128 && !__is_same(T, __half); r0 += kTurn * kRows) {
                     uint4 x[kTurn];
                     float top[kTurn];
