@@ -20,9 +20,9 @@
 // Bounds: per 128 keys a tile pair needs 2 x 2 x 128 x 128 x D products (2,048 clocks at head_dim 128) and 2 x 16,384
 // exponentials and as many conversions (about 2,560). What a pair takes is the chain of one tile's step, about 3,500
 // clocks, the other tile in the gaps: S into registers 200, maximum 250, P 1,270, hand-over 100, P V and the next S
-// 1,100, waits. Measured on one B200, full attention over 2 x 8,192 tokens: 16 heads of 128 in bf16 928 us, 1,184
-// TFLOP/s (tensor pipe 54% active); 16 heads of 64 in f16 819 us, 671; 8 heads of 256 in bf16 1,199 us, 917; causal
-// with a window of 1,024 and 4 sinks, 16 query heads on 4, 209 us. The rows of two tiles rather than one per CTA halve
+// 1,100, waits. Measured on two B200s, full attention over 2 x 8,192 tokens: 16 heads of 128 in bf16 900 and 925 us, 1,222
+// and 1,189 TFLOP/s (tensor pipe 54% active); 16 heads of 64 in f16 771 and 821 us; 8 heads of 256 in bf16 1,174 and 1,182 us;
+// causal with a window of 1,024 and 4 sinks, 16 query heads on 4, 203 us. The rows of two tiles rather than one per CTA halve
 // the traffic of K and V from L2 (64 KB per step); 128 keys a step is what tensor memory holds beside two O.
 // The instructions' operands have to be in uniform registers: issued from one divergent lane, each product cost
 // 75 clocks and the same kernel ran at 972 instead of 1,097 TFLOP/s.
@@ -56,7 +56,8 @@ template <int D, bool PAGED> struct Shape {
     static constexpr int seqs = 512;  // sequences per launch (their table is in shared memory)
     static constexpr int threads = 12 * 32;
     // Registers: launched with 168 a thread, of which the two softmax warpgroups take more and the other gives up
-    // as many: 8 x 208 + 4 x 88 = 12 x 168.
+    // as many: 8 x 208 + 4 x 88 = 12 x 168. At 216 and 72 the warps that convert Q spill: 229 instead of 217 us for 4 x 500
+    // rows on 5,000 tokens, 32 heads of 128 on 8.
     static constexpr int regs_softmax = 208, regs_other = 88;
     static constexpr int tmem_s = 0;                           // S (and P) columns of tile or buffer i at 128 i
     static constexpr int tmem_o = 256;                         // O columns of tile i at 256 + D i
