@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
     __shared__ volatile int failed;
     __shared__ float4 scales_s[kInfo];  // over the cache: K scales of a step's two pages, V scales
     __shared__ int present_s[kInfo];    // bit i: page i of the step exists
-    __shared__ uint8_t q_up_s[PAGED ? 2 * TILES * 128 : 1];  // over the cache: log2 + 127 of what each row of Q was divided by, of two items
+    __shared__ uint8_t q_up_s[PAGED ? 2 * TILES * 128 : 1];  // over the cache: log2 + 127 of what each row of Q was divided by, of a tile's last two items with steps
 
     const mrl_attn& a = pr.a;
     const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -449,8 +449,9 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
         const uint32_t lane_off = (uint32_t)(warp & 3) << 21;  // lane 32 (warp % 4) of tensor memory
         const int tok = pr.inner_q ? r % tokens : r / group, qh = pr.inner_q ? r / tokens : r % group;
         const bool row_used = r < tokens * group;
-        uint32_t s_par = 0, o_par = 0;  // bit i: buffer i
-        int step_no = 0, used = 0, items_done = 0;
+        uint32_t s_par = 0;  // bit i: buffer i
+        uint32_t o_par = 0;  // the tile's items with steps so far, mod 2
+        int step_no = 0, used = 0;
         for (unsigned r_no = 0; r_no * grid < items && !failed; ++r_no) {
             const unsigned i = item_no(r_no);
             if (i >= items) break;
@@ -472,7 +473,7 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                 tc::fence_after();
                 const uint32_t s_col = tmem + lane_off + S::tmem_s + buf * 128;
                 const int key0 = s * kKeys;
-                if (PAGED && !__is_same(T, __half) && !any) cur *= __uint_as_float((uint32_t)q_up_s[((items_done & 1) * TILES + tile) * 128 + r] << 23);
+                if (PAGED && !__is_same(T, __half) && !any) cur *= __uint_as_float((uint32_t)q_up_s[(o_par * TILES + tile) * 128 + r] << 23);
                 float ka = cur, kb = cur, va = 1.0f, vb = 1.0f;
                 bool full = key0 + kKeys <= it.len && (!causal || key0 + kKeys - 1 <= p_lo) &&
                             (window == 0 || key0 + kKeys <= sinks || (key0 > p_hi - window && (causal || key0 + kKeys - 1 < p_lo + window)));
@@ -587,7 +588,6 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                 if (lane == 0) arrive(&p_full[buf]);
                 ++used;
             }
-            ++items_done;
             const bool in = row_used && f + tok < it.m;
             const int t_row = it.row + f + tok, h = it.head * group + qh;
             T* dst = static_cast<T*>(a.out) + (int64_t)t_row * a.o_row + (int64_t)h * a.o_head;
@@ -880,10 +880,9 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
         // ---- Q of the cache's attention, as f16
         constexpr int kConv = 64;
         const int ct = tid - 10 * 32;
-        int items_done = 0;
-        uint32_t q_par = 0;
+        uint32_t q_par = 0;  // bit t: items with steps of tile t so far, mod 2
         bool ok = true;
-        for (unsigned r_no = 0; r_no * grid < items && ok && !failed; ++r_no, ++items_done) {
+        for (unsigned r_no = 0; r_no * grid < items && ok && !failed; ++r_no) {
             const unsigned i = item_no(r_no);
             if (i >= items) break;
             const Item<TILES> it = item_at(i);
@@ -905,6 +904,9 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
             };
             auto finish_q = [&](int t) {
                 constexpr int kTurn = 4;  // rows of a thread in flight
+                // Of the tile's items with steps, the one two before has used its slot up: the tile's last S of the one
+                // before was issued after that one's P, and q_empty waited for it.
+                uint8_t* const up_s = q_up_s + ((((q_par >> t) & 1) ^ 1) * TILES + t) * 128;
                 for (int r0 = q_row; r0 < 128 && !__is_same(T, __half); r0 += kTurn * kRows) {
                     uint4 x[kTurn];
                     float top[kTurn];
@@ -936,7 +938,7 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
 #pragma unroll
                         for (int j = 0; j < 4; ++j) y[j] = pack16<false>(to_f32<T>(e[2 * j]) * down, to_f32<T>(e[2 * j + 1]) * down);
                         *reinterpret_cast<uint4*>(q_at(t, r)) = make_uint4(y[0], y[1], y[2], y[3]);
-                        if (q_col == 0) q_up_s[((items_done & 1) * TILES + t) * 128 + r] = (uint8_t)up;
+                        if (q_col == 0) up_s[r] = (uint8_t)up;
                     }
                 }
                 tc::fence_proxy_async_smem();

@@ -1,0 +1,58 @@
+"""The attention operators where they went wrong or could: unknown sequences among known ones, pages that a row does
+not see, values that are not finite, scratch and captured graphs, refused calls. Plain forms and the derivation of the
+tolerances are those of test_gpu_attention.py."""
+import math
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from test_gpu_attention import (M, PAGE, U, check_rows, cu_of, filled_cache, held_rows, i32,  # noqa: E402,F401
+                                plain_attention)
+
+pytestmark = pytest.mark.gpu
+
+
+def check_known(codes, scales, tables, lens, seqs, rows, q, out, lse, window=0, sinks=0, vmax_of=None):
+    """attend's rows of every listed sequence against the plain form; unknown sequences, and rows beyond a
+    sequence's length, are empty."""
+    d = q.shape[2]
+    qn, on, ln = q.double().cpu().numpy(), out.double().cpu().numpy(), lse.double().cpu().numpy()
+    at = 0
+    for s, m in zip(seqs, rows):
+        known = 0 <= s < len(lens)
+        n = lens[s] if known else 0
+        none = max(0, m - n)
+        assert np.all(on[at:at + none] == 0) and np.all(ln[at:at + none] == -np.inf)
+        if known and m > none:
+            k, present = held_rows(codes, scales, tables[s], n, 0)
+            v, _ = held_rows(codes, scales, tables[s], n, 1)
+            lo, hi = at + none, at + m
+            want, wl, big = plain_attention(qn[lo:hi], k, v, n - (m - none), True, window, sinks, d ** -0.5, present)
+            check_rows(on[lo:hi], ln[lo:hi], want, wl, big, d, n, np.abs(v).max(), U[q.dtype], 2.0 ** -11)
+        at += m
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_unknown_sequences_between_known_ones(M, dev, d, dtype):
+    """More sequences than the kernel sorts by length, half of them unknown or with more rows than tokens, rows whose
+    magnitudes lie powers of two apart: every row has its own scale."""
+    rng = np.random.default_rng(d)
+    n, h, g = 240, 2, 4
+    lens = [int(x) for x in rng.integers(1, 129, n)]
+    cache, codes, scales, tables = filled_cache(M, rng, dev, lens, h, d)
+    seqs = [int(x) for x in rng.permutation(n)]
+    rows = [min(lens[s], int(rng.integers(1, 90))) for s in seqs]
+    for i in range(n):
+        if i % 3 == 1:
+            seqs[i], rows[i] = (-1 - i if i % 2 else n + i), int(rng.integers(1, 90))
+        elif i % 3 == 2 and i % 4 < 2:
+            rows[i] = lens[seqs[i]] + int(rng.integers(1, 150))
+    t = sum(rows)
+    q = rng.normal(0, 1.5, (t, h * g, d)) * np.exp2(rng.integers(-9, 1, (t, h * g, 1)))
+    q = torch.from_numpy(q).to(dtype).cuda()
+    for _ in range(3):
+        out, lse = cache.attend(0, q, i32(seqs), cu_of(rows), max_q=max(rows), return_lse=True)
+        check_known(codes[0], scales[0], tables, lens, seqs, rows, q, out, lse)
