@@ -81,6 +81,8 @@ struct mrl_ctx {
 
 inline int fail(mrl_ctx* ctx, int code, const std::string& msg) {
     if (ctx) ctx->err = msg;
+    // the runtime keeps a failed call's error for the next cudaGetLastError, which a later launch would report as its own
+    if (code == MRL_ERR_CUDA || code == MRL_ERR_NOMEM) (void)cudaGetLastError();
     return code;
 }
 

@@ -56,3 +56,24 @@ def test_unknown_sequences_between_known_ones(M, dev, d, dtype):
     for _ in range(3):
         out, lse = cache.attend(0, q, i32(seqs), cu_of(rows), max_q=max(rows), return_lse=True)
         check_known(codes[0], scales[0], tables, lens, seqs, rows, q, out, lse)
+
+
+def huge_pool(cache):
+    """The cache said to have 2^24 pages: its tables hold small ones alone, so nothing past its tensors is touched, and
+    an image of such a pool (2^24 x 4 kv heads x 64 x 64 x 2 bytes = 550 GB) fits no device."""
+    cache._c.pages = 1 << 24
+    return cache
+
+
+def test_failed_scratch_is_no_error_of_the_next_call(M, dev):
+    rng = np.random.default_rng(1)
+    cache, codes, scales, tables = filled_cache(M, rng, dev, [500] * 4, 2, 64)
+    q = torch.from_numpy(rng.normal(0, 1, (2000, 8, 64))).half().cuda()
+    small = cache._c.pages
+    try:
+        huge_pool(cache).attend(0, q, i32(range(4)), cu_of([500] * 4), max_q=500)
+    except M.MrlError:
+        pass
+    cache._c.pages = small
+    cache.reserve(i32([1]), i32([3]))
+    assert cache.lens.tolist() == [500, 503, 500, 500]
