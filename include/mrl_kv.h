@@ -6,12 +6,20 @@
  * src/gemma_embed.rs), and for a reader of the passages that the scan finds.
  *
  * Conventions of mrl_cuda.h hold: int status, never an abort or an exception across the boundary,
- * mrl_last_error for the message, every call asynchronous on the context's stream, no host
- * synchronisation. All buffers are device memory owned by the caller. Index arrays (sequences,
- * offsets, tables) live on the device, so what only their contents can show is checked there: an
- * index out of range is never followed, and the page operations set a bit of *status and change
- * nothing. A context keeps one scratch buffer per stream for these calls (grown on demand; grow it
- * with a first call before a stream capture begins).
+ * mrl_last_error for the message, every call asynchronous on the context's stream. All buffers are
+ * device memory owned by the caller. Index arrays (sequences, offsets, tables) live on the device, so
+ * what only their contents can show is checked there: an index out of range is never followed, and the
+ * page operations set a bit of *status and change nothing.
+ *
+ * Scratch. A context keeps scratch for every stream that these calls were made on, until it is
+ * destroyed: about 20 MiB, more for pools of millions of pages, and for mrl_kv_attend of many rows
+ * twice the size of one layer's codes. It grows on demand, and a call that makes it grow allocates
+ * device memory and may wait for the device; the others do not synchronise. During a stream capture
+ * nothing can grow: such a call is refused, so make a call of the same size on the stream before the
+ * capture. A captured graph goes on using the scratch of the stream it was captured on, which stays
+ * where it is whatever is called later: replay it on that stream, or where nothing else runs on that
+ * stream's scratch (its calls and the other graphs captured on it) at the same time. Destroy the
+ * context after the graphs, and a stream only when its work is done.
  */
 #ifndef MRL_KV_H
 #define MRL_KV_H

@@ -355,9 +355,10 @@ void mrl_ctx_destroy(mrl_ctx* ctx) {
     cudaFree(ctx->ebuf);
     cudaFree(ctx->bbuf);
     for (mrl_kv_scratch& k : ctx->kv) {
-        cudaFree(k.buf);
-        cudaFree(k.image);
+        cudaFree(k.work.p);
+        cudaFree(k.image.p);
     }
+    for (void* p : ctx->kv_kept) cudaFree(p);
     if (ctx->join_event) cudaEventDestroy(ctx->join_event);
     if (ctx->h_io) cudaFreeHost(ctx->h_io);
     if (ctx->h_slots) cudaFreeHost(ctx->h_slots);

@@ -3,19 +3,23 @@
 #pragma once
 
 #include <cstdint>
+#include <deque>
 #include <string>
+#include <vector>
 
 #include "mrl_internal.cuh"
 
 // Scratch of the paged-cache and attention entry points on one stream (include/mrl_kv.h): calls on
 // different streams never share a buffer.
+struct mrl_kv_block {
+    void* p = nullptr;
+    size_t bytes = 0;
+    bool captured = false;  // a graph holds the address
+};
 struct mrl_kv_scratch {
     cudaStream_t stream = nullptr;
-    void* buf = nullptr;    // working memory
-    size_t bytes = 0;
-    void* image = nullptr;  // 16-bit image of a layer's pool
-    size_t image_bytes = 0;
-    bool used = false;
+    mrl_kv_block work;   // counters and working memory
+    mrl_kv_block image;  // 16-bit image of a layer's pool
 };
 
 struct mrl_ctx {
@@ -71,11 +75,10 @@ struct mrl_ctx {
     uint32_t slot_k = 0;
     uint32_t slot_seq[MRL_MAX_INFLIGHT] = {};
     bool slot_busy[MRL_MAX_INFLIGHT] = {};
-    // paged cache and attention (kv_capi.cu): scratch per stream, and the event that orders a torch
-    // stream with the context's
-    static constexpr int kKvStreams = 8;
-    mrl_kv_scratch kv[kKvStreams];
-    int kv_next = 0;
+    // paged cache and attention (kv_capi.cu): scratch per stream, blocks that were outgrown but are held by captured
+    // graphs, and the event that orders a torch stream with the context's
+    std::deque<mrl_kv_scratch> kv;
+    std::vector<void*> kv_kept;
     cudaEvent_t join_event = nullptr;
 };
 

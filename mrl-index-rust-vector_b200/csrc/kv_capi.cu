@@ -58,47 +58,52 @@ int check_rows16(mrl_ctx* ctx, const char* name, const void* p, int64_t row, int
     return MRL_OK;
 }
 
-// The scratch of the context's current stream.
-int kv_scratch_slot(mrl_ctx* ctx, mrl_kv_scratch** out) {
-    mrl_kv_scratch* k = nullptr;
+// The scratch of the context's current stream, made by the first call on it. It is never handed to another stream: a graph
+// captured on this one keeps using it.
+mrl_kv_scratch& kv_stream(mrl_ctx* ctx) {
     for (mrl_kv_scratch& x : ctx->kv)
-        if (x.used && x.stream == ctx->stream) k = &x;
-    if (!k) {
-        k = &ctx->kv[ctx->kv_next];
-        if (k->used) MRL_CUDA_TRY(ctx, cudaDeviceSynchronize());  // its old stream may still use the buffers
-        ctx->kv_next = (ctx->kv_next + 1) % mrl_ctx::kKvStreams;
-        k->stream = ctx->stream;
-        k->used = true;
+        if (x.stream == ctx->stream) return x;
+    ctx->kv.emplace_back();
+    ctx->kv.back().stream = ctx->stream;
+    return ctx->kv.back();
+}
+
+// At least `bytes` in a block of the scratch, zero when they are made. A block whose address a captured graph may hold
+// is kept beside its successor; another one is freed, which waits for the device.
+int kv_grow(mrl_ctx* ctx, mrl_kv_block* b, size_t bytes) {
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(ctx->stream, &capture) != cudaSuccess) (void)cudaGetLastError();  // the launch will say so
+    const bool capturing = capture != cudaStreamCaptureStatusNone;
+    if (b->bytes < bytes) {
+        if (capturing) return bad(ctx, "scratch cannot grow during a stream capture: make a call of this size on the stream before it");
+        if (b->captured) {
+            ctx->kv_kept.push_back(b->p);
+            *b = mrl_kv_block{};
+        }
+        if (int rc = ensure_buf(ctx, &b->p, &b->bytes, (bytes + (size_t)0xfffff) & ~(size_t)0xfffff)) return rc;
+        MRL_CUDA_TRY(ctx, cudaMemsetAsync(b->p, 0, b->bytes, ctx->stream));
     }
-    *out = k;
+    b->captured = b->captured || capturing;
     return MRL_OK;
 }
 
-// A buffer of the scratch, at least `bytes` long and zero when it is made.
-int kv_grow(mrl_ctx* ctx, void** buf, size_t* have, size_t bytes) {
-    if (*have >= bytes) return MRL_OK;
-    if (int rc = ensure_buf(ctx, buf, have, (bytes + (size_t)0xfffff) & ~(size_t)0xfffff)) return rc;
-    MRL_CUDA_TRY(ctx, cudaMemsetAsync(*buf, 0, *have, ctx->stream));
-    return MRL_OK;
-}
-
-// `bytes` of working memory, and counters before it (zero; the kernels that use them leave them zero).
+// `bytes` of working memory, and counters before it (zero; the kernels that use them leave them zero). From the first
+// call there is room for every mrl_kv_attend of few rows.
 constexpr size_t kCounterBytes = 65536;
 int kv_scratch(mrl_ctx* ctx, size_t bytes, void** out, unsigned** counters = nullptr) {
-    mrl_kv_scratch* k;
-    if (int rc = kv_scratch_slot(ctx, &k)) return rc;
-    if (int rc = kv_grow(ctx, &k->buf, &k->bytes, bytes + kCounterBytes)) return rc;
-    *out = static_cast<char*>(k->buf) + kCounterBytes;
-    if (counters) *counters = static_cast<unsigned*>(k->buf);
+    mrl_kv_scratch& k = kv_stream(ctx);
+    for (const uint32_t d : {64u, 128u, 256u}) bytes = std::max(bytes, mrl::kv_decode_bytes(d, ctx->sms));
+    if (int rc = kv_grow(ctx, &k.work, bytes + kCounterBytes)) return rc;
+    *out = static_cast<char*>(k.work.p) + kCounterBytes;
+    if (counters) *counters = static_cast<unsigned*>(k.work.p);
     return MRL_OK;
 }
 
 // Room for a layer's pool as f16 (launch_attend_tc).
 int kv_image(mrl_ctx* ctx, size_t bytes, void** out) {
-    mrl_kv_scratch* k;
-    if (int rc = kv_scratch_slot(ctx, &k)) return rc;
-    if (int rc = kv_grow(ctx, &k->image, &k->image_bytes, bytes)) return rc;
-    *out = k->image;
+    mrl_kv_scratch& k = kv_stream(ctx);
+    if (int rc = kv_grow(ctx, &k.image, bytes)) return rc;
+    *out = k.image.p;
     return MRL_OK;
 }
 

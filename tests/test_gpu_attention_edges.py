@@ -77,3 +77,110 @@ def test_failed_scratch_is_no_error_of_the_next_call(M, dev):
     cache._c.pages = small
     cache.reserve(i32([1]), i32([3]))
     assert cache.lens.tolist() == [500, 503, 500, 500]
+
+
+# ---- scratch and captured graphs ------------------------------------------------------------------------------
+
+
+def reader(M, dev, rng, n, length, h, d, rows, spare=3):
+    """A filled cache of n sequences, queries of `rows` rows each, and the call that attends with them."""
+    lens = [length] * n
+    cache, codes, scales, tables = filled_cache(M, rng, dev, lens, h, d, spare=spare)
+    q = torch.from_numpy(rng.normal(0, 1, (n * rows, 4 * h, d))).bfloat16().cuda()
+    seqs, cu = i32(range(n)), cu_of([rows] * n)
+    return cache, lambda out=None: cache.attend(0, q, seqs, cu, max_q=rows, out=out)
+
+
+def test_graphs_outlive_growth_and_other_streams(M):
+    """Graphs of single rows, of many rows and of a fork, replayed after calls that need more scratch than was there, and
+    after calls on more streams than any fixed number of slots."""
+    own = M.Device(0)
+    rng = np.random.default_rng(2)
+    cache1, one = reader(M, own, rng, 8, 3000, 2, 128, 1)
+    cache2, many = reader(M, own, rng, 4, 700, 2, 128, 300)
+    forks = M.KvCache.create(1, 40, 1, 64, 12, 4, dev=own)
+    forks.reserve(i32([0]), i32([150]))
+    parents, kids = i32([0] * 8), i32(range(1, 9))
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        own.use_torch_stream()
+        want1, want2 = one(), many()
+        forks.fork(parents, kids)
+        forks.release(kids)
+    torch.cuda.synchronize()
+    out1, out2 = torch.zeros_like(want1), torch.zeros_like(want2)
+    g1, g2, g3 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g1, stream=s):
+        one(out1)
+    with torch.cuda.graph(g2, stream=s):
+        many(out2)
+    with torch.cuda.graph(g3, stream=s):
+        forks.release(kids)
+        forks.fork(parents, kids)
+
+    def replayed():
+        out1.zero_()
+        out2.zero_()
+        forks.status.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            for g in (g1, g2, g3):
+                g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out1, want1) and torch.equal(out2, want2)
+        assert forks.lens.tolist() == [150] * 9 + [0] * 3 and forks.refs.tolist() == [9] * 2 + [1] * 9 + [0] * 29
+        assert int(forks.status) == 0
+
+    replayed()
+    with torch.cuda.stream(s):
+        _, other = reader(M, own, rng, 70, 500, 2, 64, 1)        # another head_dim
+        other()
+        _, bigger = reader(M, own, rng, 4, 700, 2, 256, 300, spare=400)  # a larger image
+        bigger()
+        pool = M.KvCache.create(1, 4, 1, 64, 2, 2, dev=own)      # longer lists: a reserve reads refs, tables and lens alone
+        refs = torch.zeros(4 << 20, dtype=torch.int32, device="cuda")
+        pool._c.refs, pool._c.pages = refs.data_ptr(), refs.shape[0]
+        pool.reserve(i32([0]), i32([100]))
+        junk = [torch.randn(8 << 20, device="cuda") for _ in range(4)]   # what was freed, if anything was, is used
+    torch.cuda.synchronize()
+    replayed()
+    torch.cuda.synchronize()
+    for t in [torch.cuda.Stream() for _ in range(12)]:
+        with torch.cuda.stream(t):
+            own.use_torch_stream()
+            assert torch.equal(one(), want1) and torch.equal(many(), want2)
+    torch.cuda.synchronize()
+    replayed()
+    del g1, g2, g3, junk
+    own.close()
+
+
+def test_growth_during_a_capture_is_refused(M):
+    """A capture whose call needs more scratch than there is stays valid: the call is refused before anything is queued."""
+    own = M.Device(0)
+    rng = np.random.default_rng(3)
+    cache, one = reader(M, own, rng, 3, 200, 1, 64, 1)
+    s = torch.cuda.Stream()
+    x = torch.zeros(4, device="cuda")
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        own.use_torch_stream()
+        x.add_(1)
+        with pytest.raises(M.MrlError, match="capture"):
+            one()
+    g.replay()
+    torch.cuda.synchronize()
+    assert x.tolist() == [1.0] * 4
+    with torch.cuda.stream(s):
+        want = one()
+    torch.cuda.synchronize()
+    out = torch.zeros_like(want)
+    with torch.cuda.graph(g2 := torch.cuda.CUDAGraph(), stream=s):
+        one(out)
+    g2.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    del g, g2
+    own.close()
