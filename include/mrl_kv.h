@@ -133,7 +133,7 @@ typedef struct mrl_attn {
 /* Attention of the last rows of sequences over the cache (always causal; k, v, kv_heads, head_dim
  * and causal of `a` are not read). Softmax statistics and sums in f32. Any max_rows is right; it
  * helps to choose the kernel: calls of few rows read the pages as codes; calls of many widen them first, into
- * scratch of twice the size of a layer's codes. Work of the former is counted in 32 bits: (n_tokens x group
+ * scratch of twice the size of a layer's codes, or read the codes too where the device has no room for it. Work of the former is counted in 32 bits: (n_tokens x group
  * / 16 + n_seqs) x kv_heads x (max_pages + 16), per 1024 sequences where cu is NULL, must stay below 2^32. */
 int mrl_kv_attend(mrl_ctx* ctx, const mrl_kv_cache* kv, const mrl_attn* a);
 /* Self-attention over ragged packed rows: sequence b's q, k and v rows are cu[b] .. cu[b+1] - 1 and

@@ -261,15 +261,19 @@ int mrl_kv_attend(mrl_ctx* ctx, const mrl_kv_cache* kv, const mrl_attn* a) {
         if (a->layer >= kv->layers) return bad(ctx, "layer is not one of the cache's");
         if (int rc = check_attn(ctx, a, kv->kv_heads, kv->head_dim, true)) return rc;
         if (a->n_tokens == 0) return MRL_OK;
+        int no_image = MRL_OK;
         if (tensor_cores(ctx, *kv, *a)) {
             void* wide;
-            if (int rc = kv_image(ctx, mrl::kv_wide_bytes(*kv), &wide)) return rc;
-            return done(ctx, mrl::launch_attend_tc(kv, cut(*a), ctx->sms, wide, ctx->stream), "mrl_kv_attend");
+            no_image = kv_image(ctx, mrl::kv_wide_bytes(*kv), &wide);
+            if (no_image == MRL_OK) return done(ctx, mrl::launch_attend_tc(kv, cut(*a), ctx->sms, wide, ctx->stream), "mrl_kv_attend");
+            if (no_image != MRL_ERR_NOMEM) return no_image;
+            // no room for it: the kernel on the codes takes any number of rows
         }
         // the cost of a launch's items (pages and a fixed part of at most 16 each) is summed in 32 bits
         const uint64_t group = a->q_heads / kv->kv_heads, per_launch = std::min(a->n_seqs, mrl::kKvDecodeSeqs);
         const uint64_t tiles = a->cu ? a->n_tokens * group / 16 + per_launch : per_launch * ((group + 15) / 16);
-        if (tiles * kv->kv_heads * (kv->max_pages + 16ull) >= (1ull << 32)) return bad(ctx, "rows x kv_heads x max_pages is too large for one call");
+        if (tiles * kv->kv_heads * (kv->max_pages + 16ull) >= (1ull << 32))
+            return no_image ? no_image : bad(ctx, "rows x kv_heads x max_pages is too large for one call");
         void* scratch;
         unsigned* counters;
         if (int rc = kv_scratch(ctx, mrl::kv_decode_bytes(kv->head_dim, ctx->sms), &scratch, &counters)) return rc;

@@ -184,3 +184,14 @@ def test_growth_during_a_capture_is_refused(M):
     assert torch.equal(out, want)
     del g, g2
     own.close()
+
+
+@pytest.mark.parametrize("d", [64, 256])
+def test_many_rows_without_room_for_the_image(M, dev, d):
+    """An image that no device has room for: the kernel on the codes gives the same rows."""
+    rng = np.random.default_rng(4)
+    lens, rows = [700, 64, 300], [500, 64, 300]
+    cache, codes, scales, tables = filled_cache(M, rng, dev, lens, 2, d)
+    q = torch.from_numpy(rng.normal(0, 1, (sum(rows), 8, d))).bfloat16().cuda()
+    out, lse = huge_pool(cache).attend(0, q, i32(range(3)), cu_of(rows), max_q=500, return_lse=True)
+    check_known(codes[0], scales[0], tables, lens, range(3), rows, q, out, lse)
