@@ -28,6 +28,8 @@ namespace kv {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLeastScale = 1e-37f;       // V scales are taken relative to this at least
+constexpr float kNoGrowth = 1.000001f;      // a scale times the rounded reciprocal of itself
 constexpr long long kWaitClocks = 4000000000ll;  // a wait for a page gives up after about two seconds
 
 // Warps per CTA: each holds one page's K and V block, 96 to 128 KiB in all, enough in flight per SM to cover
@@ -448,7 +450,11 @@ template <class T, int D, bool WIDE> __global__ void __launch_bounds__(kWarps<D>
         float o[D / 8][4];
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f, vref = 0.0f;
+        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+        // P carries V's scale relative to the largest one of the pages that the row has seen so far, and O is in units of
+        // that; its reciprocal is kept. Pages that a row sees nothing of do not count: their scale may be any number of
+        // times larger, and would push the P of the others out of f16.
+        float per0 = 1.0f / kLeastScale, per1 = per0;
 
         for (int i = s.p0 + w_in; i < s.p1; i += W) {
             const int page = npage, index = nindex;
@@ -495,7 +501,7 @@ template <class T, int D, bool WIDE> __global__ void __launch_bounds__(kWarps<D>
             fetch(0);
             const float f0 = c0 * ks, f1 = c1 * ks;
             const int key0 = index * kPage;
-            float n0 = m0, n1 = m1;
+            float n0 = -INFINITY, n1 = -INFINITY;
             // Token 16 t + 2 j + e of the page is column e of score tile j here.
             if (key0 + kPage - 1 <= low_pos && (window == 0 || key0 > high_pos - window || key0 + kPage <= sinks)) {
 #pragma unroll
@@ -523,14 +529,25 @@ template <class T, int D, bool WIDE> __global__ void __launch_bounds__(kWarps<D>
             }
             n0 = quad_max(n0);
             n1 = quad_max(n1);
-            // P carries V's scale relative to the largest one so far, and O is in units of that.
-            const float up = fmaxf(vref, vs), vf = up > 0.0f ? vs / up : 0.0f;
-            if (__any_sync(~0u, n0 != m0 || n1 != m1) || up != vref) {
-                const float unit = up > 0.0f ? vref / up : 0.0f;
+            const float s0 = n0 > -INFINITY ? vs : 0.0f, s1 = n1 > -INFINITY ? vs : 0.0f;
+            const bool grow0 = s0 * per0 > kNoGrowth, grow1 = s1 * per1 > kNoGrowth;
+            n0 = fmaxf(n0, m0);
+            n1 = fmaxf(n1, m1);
+            if (__any_sync(~0u, n0 != m0 || n1 != m1 || grow0 || grow1)) {
                 const float k0 = m0 == -INFINITY ? 0.0f : ex2(m0 - n0), k1 = m1 == -INFINITY ? 0.0f : ex2(m1 - n1);
                 l0 *= k0;
                 l1 *= k1;
-                const float a0 = k0 * unit, a1 = k1 * unit;
+                float a0 = k0, a1 = k1;
+                if (grow0) {
+                    const float to = __fdividef(1.0f, s0);
+                    a0 *= __fdividef(to, per0);
+                    per0 = to;
+                }
+                if (grow1) {
+                    const float to = __fdividef(1.0f, s1);
+                    a1 *= __fdividef(to, per1);
+                    per1 = to;
+                }
 #pragma unroll
                 for (int x = 0; x < D / 8; ++x) {
                     o[x][0] *= a0;
@@ -540,9 +557,9 @@ template <class T, int D, bool WIDE> __global__ void __launch_bounds__(kWarps<D>
                 }
                 m0 = n0;
                 m1 = n1;
-                vref = up;
             }
             const float z0 = m0 == -INFINITY ? 0.0f : m0, z1 = m1 == -INFINITY ? 0.0f : m1;
+            const float vf0 = s0 * per0, vf1 = s1 * per1;
             uint32_t pf[4][4];
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
@@ -555,8 +572,8 @@ template <class T, int D, bool WIDE> __global__ void __launch_bounds__(kWarps<D>
                     w[3] = ex2(w[3] - z1);
                     l0 += w[0] + w[1];
                     l1 += w[2] + w[3];
-                    pf[x][2 * y] = pack_half(w[0] * vf, w[1] * vf);
-                    pf[x][2 * y + 1] = pack_half(w[2] * vf, w[3] * vf);
+                    pf[x][2 * y] = pack_half(w[0] * vf0, w[1] * vf0);
+                    pf[x][2 * y + 1] = pack_half(w[2] * vf1, w[3] * vf1);
                 }
             }
             fine = fine && bar_wait(bar_v, parity);
@@ -583,13 +600,14 @@ template <class T, int D, bool WIDE> __global__ void __launch_bounds__(kWarps<D>
         l1 = quad_sum(l1);
 
         // ---- the team's warps joined: O in real units, then rescaled to the rows' common maximum
+        const float vref0 = 1.0f / per0, vref1 = 1.0f / per1;
         float* mine = acc_s + warp * 16 * kAccStride<D>;
 #pragma unroll
         for (int x = 0; x < D / 8; ++x) {
             if (r0 < rows_all)
-                *reinterpret_cast<float2*>(mine + g * kAccStride<D> + 8 * x + 2 * t) = make_float2(o[x][0] * vref, o[x][1] * vref);
+                *reinterpret_cast<float2*>(mine + g * kAccStride<D> + 8 * x + 2 * t) = make_float2(o[x][0] * vref0, o[x][1] * vref0);
             if (r1 < rows_all)
-                *reinterpret_cast<float2*>(mine + (g + 8) * kAccStride<D> + 8 * x + 2 * t) = make_float2(o[x][2] * vref, o[x][3] * vref);
+                *reinterpret_cast<float2*>(mine + (g + 8) * kAccStride<D> + 8 * x + 2 * t) = make_float2(o[x][2] * vref1, o[x][3] * vref1);
         }
         if (t == 0) {
             *reinterpret_cast<float2*>(ml_s + (warp * 16 + g) * 2) = make_float2(m0, l0);

@@ -195,3 +195,78 @@ def test_many_rows_without_room_for_the_image(M, dev, d):
     q = torch.from_numpy(rng.normal(0, 1, (sum(rows), 8, d))).bfloat16().cuda()
     out, lse = huge_pool(cache).attend(0, q, i32(range(3)), cu_of(rows), max_q=500, return_lse=True)
     check_known(codes[0], scales[0], tables, lens, range(3), rows, q, out, lse)
+
+
+# ---- pages that a row does not see ------------------------------------------------------------------------------
+
+
+def check_by_row(codes, scales, table, n, q, out, lse, window, sinks):
+    """One sequence's last rows against the plain form, each row within what the pages that it sees allow: vmax is
+    127 times the largest V scale of a page in which the row sees a key."""
+    t, hq, d = q.shape
+    qn, on, ln = q.double().cpu().numpy(), out.double().cpu().numpy(), lse.double().cpu().numpy()
+    k, present = held_rows(codes, scales, table, n, 0)
+    v, _ = held_rows(codes, scales, table, n, 1)
+    want, wl, big = plain_attention(qn, k, v, n - t, True, window, sinks, d ** -0.5, present)
+    h = k.shape[1]
+    key = np.arange(n)
+    for i in range(t):
+        p = n - t + i
+        ok = present & (key <= p) & ((p - key < window) | (key < sinks) if window else True)
+        pages = sorted({int(table[j]) for j in np.nonzero(ok)[0] // PAGE})
+        for a in range(h):
+            rows = slice(a * hq // h, (a + 1) * hq // h)
+            vmax = 127 * float(scales[pages, 1, a].max()) if pages else 0.0
+            got, w = on[i, rows], want[i, rows]
+            # beyond the output's type the result is its infinity; within a tolerance's width of its end, either
+            end, near = float(torch.finfo(q.dtype).max), 0.01 * vmax
+            over = np.abs(w) > end - near
+            assert np.all((got[over] == np.sign(w[over]) * np.inf) | (np.abs(w[over]) < end + near))
+            check_rows(np.where(over, w, got), ln[i, rows], w, wl[i, rows], big, d, n, vmax, U[q.dtype], 2.0 ** -11)
+
+
+def unseen_scale_case(M, dev, rng, n, t, h, g, d, dtype, window, sinks, pages, ratio):
+    cache, codes, scales, tables = filled_cache(M, rng, dev, [n], h, d)
+    for p in pages:
+        scales[0, tables[0, p], 1] *= ratio
+    cache.scales.copy_(torch.from_numpy(scales))
+    q = torch.from_numpy(rng.normal(0, 1, (t, h * g, d))).to(dtype).cuda()
+    out, lse = cache.attend(0, q, i32([0]), cu_of([t]), max_q=t, window=window, sinks=sinks, return_lse=True)
+    check_by_row(codes[0], scales[0], tables[0], n, q, out, lse, window, sinks)
+
+
+RATIOS = [1e6, 1e10]
+
+
+@pytest.mark.parametrize("ratio", RATIOS)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_unseen_value_scales_few_rows(M, dev, d, dtype, ratio):
+    """A page with far larger values that some rows of a 16-row item see and others do not: a later page (causal), an
+    earlier one (window), and one between the sinks and the window."""
+    rng = np.random.default_rng(d)
+    unseen_scale_case(M, dev, rng, 64 * 3 + 8, 16, 2, 1, d, dtype, 0, 0, [3], ratio)
+    unseen_scale_case(M, dev, rng, 64 * 4 + 15, 16, 1, 1, d, dtype, 10, 0, [3], ratio)
+    unseen_scale_case(M, dev, rng, 64 * 9 + 20, 12, 2, 2, d, dtype, 6, 4, [1, 8], ratio)
+    unseen_scale_case(M, dev, rng, 64 * 40 + 5, 8, 2, 2, d, dtype, 0, 0, [40], ratio)
+
+
+@pytest.mark.parametrize("ratio", RATIOS)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("n_seqs", [1, 160])
+def test_unseen_value_scales_of_one_warp(M, dev, d, ratio, n_seqs):
+    """The first page of a long window, seen by the first four of 16 rows alone and followed by pages of the same warp;
+    scores so peaked that a row's result is a few values of a few pages."""
+    rng = np.random.default_rng(d + n_seqs)
+    n, window, t = 64 * 24 + 11 + 16, 64 * 22 + 16, 16
+    assert (n - t - window + 1) % 64 == 60
+    lens = [n] * n_seqs
+    cache, codes, scales, tables = filled_cache(M, rng, dev, lens, 1, d)
+    for i in range(n_seqs):
+        scales[0, tables[i, (n - t - window + 1) // 64], 1] *= ratio
+    cache.scales.copy_(torch.from_numpy(scales))
+    q = torch.from_numpy(rng.normal(0, 8, (n_seqs * t, 1, d))).bfloat16().cuda()
+    out, lse = cache.attend(0, q, i32(range(n_seqs)), cu_of([t] * n_seqs), max_q=t, window=window, return_lse=True)
+    for i in range(min(n_seqs, 6)):
+        rows = slice(i * t, (i + 1) * t)
+        check_by_row(codes[0], scales[0], tables[i], n, q[rows], out[rows], lse[rows], window, 0)
