@@ -10,7 +10,8 @@
 //
 // The running maximum a row subtracts moves only when a new one exceeds it by 2^8 (base-2 logits): O and
 // the sum l are kept relative to the stale one, which cancels in o = O / l, and O is rescaled rarely. P is
-// at most 2^8, well inside f16, and its rounding is relative either way.
+// at most 2^8, over the cache, where it carries V's scale in a unit that lags by up to 2^6, at most 2^14: inside f16,
+// and its rounding is relative either way.
 //
 // Roles: warps 0-3 and 4-7 softmax and epilogue of the tiles, warp 8 issues the products, warp 9 loads Q, K
 // and V by TMA (16-bit rows); over the cache warp 9 copies blocks of codes that
@@ -518,8 +519,13 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                 for (int j = 0; j < 8; ++j) mx[j] = fmaxf(mx[j], __uint_as_float(x[16 * j + 15]));
                 const float top_a = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), top_b = fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7]));
                 const float top = fmaxf(top_a * ka, top_b * kb);
-                // the maximum that is subtracted, and V's scale unit, move rarely
+                // the maximum that is subtracted, and V's scale unit, move rarely; a page that the row sees nothing of has no
+                // part in the unit, however large its scale
                 float keep = 1.0f;
+                if (PAGED) {
+                    if (!(top_a > -INFINITY)) va = 0.0f;
+                    if (!(top_b > -INFINITY)) vb = 0.0f;
+                }
                 const float vmax = fmaxf(va, vb);
                 const bool grow = top > m + kSlack;
                 if (PAGED && vmax > kScaleSlack * vref) {

@@ -225,12 +225,12 @@ def check_by_row(codes, scales, table, n, q, out, lse, window, sinks):
             check_rows(np.where(over, w, got), ln[i, rows], w, wl[i, rows], big, d, n, vmax, U[q.dtype], 2.0 ** -11)
 
 
-def unseen_scale_case(M, dev, rng, n, t, h, g, d, dtype, window, sinks, pages, ratio):
+def unseen_scale_case(M, dev, rng, n, t, h, g, d, dtype, window, sinks, pages, ratio, spread=1.0):
     cache, codes, scales, tables = filled_cache(M, rng, dev, [n], h, d)
     for p in pages:
         scales[0, tables[0, p], 1] *= ratio
     cache.scales.copy_(torch.from_numpy(scales))
-    q = torch.from_numpy(rng.normal(0, 1, (t, h * g, d))).to(dtype).cuda()
+    q = torch.from_numpy(rng.normal(0, spread, (t, h * g, d))).to(dtype).cuda()
     out, lse = cache.attend(0, q, i32([0]), cu_of([t]), max_q=t, window=window, sinks=sinks, return_lse=True)
     check_by_row(codes[0], scales[0], tables[0], n, q, out, lse, window, sinks)
 
@@ -270,3 +270,16 @@ def test_unseen_value_scales_of_one_warp(M, dev, d, ratio, n_seqs):
     for i in range(min(n_seqs, 6)):
         rows = slice(i * t, (i + 1) * t)
         check_by_row(codes[0], scales[0], tables[i], n, q[rows], out[rows], lse[rows], window, 0)
+
+
+@pytest.mark.parametrize("ratio", RATIOS)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_unseen_value_scales_many_rows(M, dev, d, dtype, ratio):
+    """The same with 128-row tiles: a page that later rows alone see, in either half of a step of 128 keys, pages that
+    have left the window, and one between the sinks and the window."""
+    rng = np.random.default_rng(d)
+    for page in (4, 5):
+        unseen_scale_case(M, dev, rng, 700, 660, 2, 4, d, dtype, 0, 0, [page], ratio, spread=5.0)
+        unseen_scale_case(M, dev, rng, 700, 700, 1, 8, d, dtype, 40, 0, [page], ratio, spread=5.0)
+        unseen_scale_case(M, dev, rng, 900, 600, 2, 4, d, dtype, 70, 4, [1, page], ratio, spread=5.0)
