@@ -44,6 +44,7 @@ constexpr int kKeys = 128;        // keys per step
 constexpr float kSlack = 8.0f;    // log2 by which a row's maximum may lead the one it subtracts
 constexpr float kScaleSlack = 64.0f;  // the same for V's scales over the cache (a factor)
 constexpr int kInfo = 8;          // steps of scales kept
+constexpr uint32_t kOwnNaN = 0xffffffffu;  // two NaNs that mark a row whose scores are not finite; conversions give 0x7fff
 
 template <int D> constexpr int kWide = kPage * D * 2;  // bytes of a page and head's K or V as f16
 // What a template instance is: D, two tiles or one, stages of K and V, and its threads.
@@ -251,10 +252,81 @@ template <int TILES> struct Item {
     __device__ __forceinline__ int begin() const { return all.head > 0 ? 0 : all.lo; }
 };
 
-// The exact result of one row whose fast one is not finite: Inf or NaN in a value that the row does not see
-// reaches a product as 0 x Inf; here only the visible keys are read. Lane e holds dims e D/32 .. .
+// The call's items, dealt out to the CTAs; the tables are in shared memory.
+template <int TILES> struct Items {
+    const SeqItem* info;
+    const unsigned* start;   // first item of the i-th sequence in order
+    const uint16_t* order;   // that sequence
+    int n, tokens;
+    unsigned heads, items;
+    int causal, window, sinks;
+
+    // Item i; the tiles with the latest tokens come first, they have the most keys where the mask is causal.
+    __device__ __forceinline__ Item<TILES> at(unsigned i) const {
+        Item<TILES> it;
+        int lo = 0, hi = n;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (start[mid] <= i) lo = mid;
+            else hi = mid;
+        }
+        const unsigned local = i - start[lo];
+        lo = order[lo];
+        const SeqItem q = info[lo];
+        const int count = (q.m + TILES * tokens - 1) / (TILES * tokens);
+        it.b = lo;
+        it.head = (int)(local % heads);
+        it.first = (count - 1 - (int)(local / heads)) * TILES * tokens;
+        it.len = q.len;
+        it.row = q.row;
+        it.m = q.m;
+        it.all = Steps{0, 0, 0};
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+            const int f = it.first + t * tokens, base = q.len - q.m;
+            it.st[t] = f < q.m ? steps_of(base + f, base + imin(f + tokens, q.m) - 1, q.len, causal, window, sinks) : Steps{0, 0, 0};
+            if (it.st[t].hi > 0) {
+                const bool none = it.all.hi == 0;
+                it.all.hi = imax(it.all.hi, it.st[t].hi);
+                it.all.lo = none ? it.st[t].lo : imin(it.all.lo, it.st[t].lo);
+                it.all.head = imax(it.all.head, it.st[t].head);
+            }
+        }
+        it.all.head = imin(it.all.head, it.all.lo);
+        return it;
+    }
+    // The CTA's item in round r: there and back over the CTAs, so that a long one is followed by a short one.
+    __device__ __forceinline__ unsigned number(unsigned r) const {
+        const unsigned grid = gridDim.x;
+        return r & 1 ? (r + 1) * grid - 1 - blockIdx.x : r * grid + blockIdx.x;
+    }
+};
+
+// The softmax warps of a CTA, without the others.
+template <int TILES> __device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, %0;" ::"n"(128 * TILES) : "memory"); }
+
+// E 16-bit values at p, 4 to 16 bytes aligned to themselves.
+template <int E> __device__ __forceinline__ void load16(const void* p, uint32_t (&w)[E / 2]) {
+    if (E == 2) w[0] = *static_cast<const uint32_t*>(p);
+    else if (E == 4) *reinterpret_cast<uint2*>(w) = *static_cast<const uint2*>(p);
+    else *reinterpret_cast<uint4*>(w) = *static_cast<const uint4*>(p);
+}
+// Of 16-bit values: bit 0, one is a NaN; bit 1, one is an Inf; bit 2, one has every bit set (kOwnNaN).
+template <class T, int E> __device__ __forceinline__ int odd_values(const uint32_t (&w)[E / 2]) {
+    constexpr uint32_t kExp = __is_same(T, __half) ? 0x7c00u : 0x7f80u;
+    int kind = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const uint32_t x = w[i / 2] >> (16 * (i & 1)) & 0xffffu, mag = x & 0x7fffu;
+        kind |= mag > kExp ? 1 : mag == kExp ? 2 : 0;
+        if (x == 0xffffu) kind |= 4;
+    }
+    return kind;
+}
+
+// The exact result of one row, from its visible keys alone. A warp, lane e holds dims e D/32 ..; four keys at a time.
 template <class T, int D> __device__ __noinline__ void slow_row(const mrl_attn& a, int row0, int n, int p, int t_row, int h, int kvh, int causal) {
-    constexpr int E = D / 32;
+    constexpr int E = D / 32, kTurn = 4;
     const int lane = (int)threadIdx.x & 31;
     const Span span = visible(p, n, causal, (int)a.window, (int)a.sinks);
     float q[E], o[E];
@@ -267,27 +339,119 @@ template <class T, int D> __device__ __noinline__ void slow_row(const mrl_attn& 
     float m = -INFINITY, l = 0.0f;
     for (int part = 0; part < 2; ++part) {
         const int from = part ? span.lo : 0, to = part ? span.hi : span.head;
-        for (int j = from; j < to; ++j) {
-            const T* kp = static_cast<const T*>(a.k) + (int64_t)(row0 + j) * a.k_row + (int64_t)kvh * a.k_head + lane * E;
-            const T* vp = static_cast<const T*>(a.v) + (int64_t)(row0 + j) * a.v_row + (int64_t)kvh * a.v_head + lane * E;
-            float s = 0.0f;
+        for (int j = from; j < to; j += kTurn) {
+            uint32_t kw[kTurn][E / 2], vw[kTurn][E / 2];
+            float s[kTurn];
 #pragma unroll
-            for (int e = 0; e < E; ++e) s = fmaf(q[e], to_f32<T>(kp[e]), s);
+            for (int u = 0; u < kTurn; ++u) {
+                const int key = imin(j + u, to - 1);
+                load16<E>(static_cast<const T*>(a.k) + (int64_t)(row0 + key) * a.k_row + (int64_t)kvh * a.k_head + lane * E, kw[u]);
+                load16<E>(static_cast<const T*>(a.v) + (int64_t)(row0 + key) * a.v_row + (int64_t)kvh * a.v_head + lane * E, vw[u]);
+            }
 #pragma unroll
-            for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
-            s *= a.scale;
-            const float top = s > m || s != s ? s : m;  // a NaN stays
-            const float keep = m == -INFINITY ? 0.0f : expf(m - top), add = s == -INFINITY && top == -INFINITY ? 0.0f : expf(s - top);
+            for (int u = 0; u < kTurn; ++u) {
+                const T* k = reinterpret_cast<const T*>(kw[u]);
+                s[u] = 0.0f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) s[u] = fmaf(q[e], to_f32<T>(k[e]), s[u]);
+            }
+#pragma unroll
+            for (int d = 16; d; d >>= 1)
+#pragma unroll
+                for (int u = 0; u < kTurn; ++u) s[u] += __shfl_xor_sync(~0u, s[u], d);
+            float top = m;
+#pragma unroll
+            for (int u = 0; u < kTurn; ++u) {
+                s[u] *= a.scale;
+                if (j + u < to) top = s[u] > top || s[u] != s[u] ? s[u] : top;  // a NaN stays
+            }
+            const float keep = m == -INFINITY ? 0.0f : expf(m - top);
             m = top;
-            l = fmaf(l, keep, add);
+            l *= keep;
 #pragma unroll
-            for (int e = 0; e < E; ++e) o[e] = (keep == 0.0f ? 0.0f : o[e] * keep) + add * to_f32<T>(vp[e]);
+            for (int e = 0; e < E; ++e) o[e] = keep == 0.0f ? 0.0f : o[e] * keep;
+#pragma unroll
+            for (int u = 0; u < kTurn; ++u) {
+                if (j + u >= to) break;
+                const float add = s[u] == -INFINITY && top == -INFINITY ? 0.0f : expf(s[u] - top);
+                const T* v = reinterpret_cast<const T*>(vw[u]);
+                l += add;
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[e] = fmaf(add, to_f32<T>(v[e]), o[e]);
+            }
         }
     }
     T* op = static_cast<T*>(a.out) + (int64_t)t_row * a.o_row + (int64_t)h * a.o_head + lane * E;
 #pragma unroll
     for (int e = 0; e < E; ++e) op[e] = from_f32<T>(l == 0.0f ? 0.0f : o[e] / l);
     if (a.lse && lane == 0) a.lse[(size_t)t_row * a.q_heads + h] = l == 0.0f ? -INFINITY : m + logf(l);
+}
+
+// A tile's rows whose fast result is not finite, all its softmax warps. A value of V that a row does not see (a later
+// key, another sequence's row) reaches its products as 0 x Inf: such a row is computed again from its visible keys. Where every
+// odd value of V that the tile met is seen by the row, the fast result is the right one, except that an Inf under a weight that
+// rounds to 0 is a NaN there. Written by the same CTA before a barrier; rows marked kOwnNaN are right as they are.
+struct OddKeys {
+    int lo, hi, inf, rows;  // first and last key with an odd value of V, whether one is an Inf, whether any row is to be looked at
+};
+template <class T, int D, int TILES> __device__ __forceinline__ void redo_tile(const mrl_attn& a, int row0, int n, int m, int first, int tokens, int group, int kvh, Steps st, int causal, OddKeys* odd) {
+    constexpr int E = D / 32, kWarps = 4 * TILES;
+    const int lane = (int)threadIdx.x & 31, warp = (int)threadIdx.x >> 5;
+    const int rows = imin(tokens, m - first) * group;
+    auto kind_of = [&](int r) {  // of the result in row r of the tile
+        uint32_t w[E / 2];
+        load16<E>(static_cast<const T*>(a.out) + (int64_t)(row0 + first + r / group) * a.o_row + (int64_t)(kvh * group + r % group) * a.o_head + lane * E, w);
+        const int kind = odd_values<T, E>(w);
+        return __any_sync(~0u, kind & 4) ? 0 : (__any_sync(~0u, kind & 1) ? 1 : 0) | (__any_sync(~0u, kind & 2) ? 2 : 0);
+    };
+    if (threadIdx.x == 0) *odd = OddKeys{0x7fffffff, -1, 0, 0};
+    softmax_sync<TILES>();
+    bool any = false;
+    for (int r = warp; r < rows; r += kWarps) any = any || kind_of(r) != 0;
+    if (any && lane == 0) odd->rows = 1;
+    softmax_sync<TILES>();
+    const bool look = odd->rows != 0;
+    if (look) {
+        for (int s = 0; s < st.hi; ++s) {
+            if (!st.has(s)) continue;
+            for (int j = s * kKeys + warp; j < (s + 1) * kKeys && row0 + j < (int)a.n_tokens; j += kWarps) {
+                uint32_t w[E / 2];
+                load16<E>(static_cast<const T*>(a.v) + (int64_t)(row0 + j) * a.v_row + (int64_t)kvh * a.v_head + lane * E, w);
+                const int kind = odd_values<T, E>(w);
+                const bool some = __any_sync(~0u, kind & 3), inf = __any_sync(~0u, kind & 2);
+                if (some && lane == 0) {
+                    atomicMin(&odd->lo, j);
+                    atomicMax(&odd->hi, j);
+                    if (inf) odd->inf = 1;
+                }
+            }
+        }
+        softmax_sync<TILES>();
+        const OddKeys o = *odd;
+        for (int r = warp; r < rows; r += kWarps) {
+            const int kind = kind_of(r);
+            if (kind == 0) continue;
+            const int f = first + r / group, p = n - m + f;
+            const Span v = visible(p, n, causal, (int)a.window, (int)a.sinks);
+            const bool seen = o.hi >= 0 && (o.hi < v.head || (o.hi < v.hi && (o.lo >= v.lo || v.head >= v.lo)));
+            if (seen && !(o.inf && (kind & 1))) continue;
+            slow_row<T, D>(a, row0, n, p, row0 + f, kvh * group + r % group, kvh, causal);
+        }
+    }
+    softmax_sync<TILES>();  // `odd` is free again
+}
+
+template <class T, int D, int TILES> __device__ __noinline__ void redo_items(const mrl_attn& a, const Items<TILES> work, int group, OddKeys* odd) {
+    for (unsigned r_no = 0; r_no * gridDim.x < work.items; ++r_no) {
+        const unsigned i = work.number(r_no);
+        if (i >= work.items) break;
+        const Item<TILES> it = work.at(i);
+#pragma unroll 1
+        for (int t = 0; t < TILES; ++t) {
+            const Steps st = TILES == 2 && t == 1 ? it.st[TILES - 1] : it.st[0];
+            if (st.hi > 0) redo_tile<T, D, TILES>(a, it.row, it.len, it.m, it.first + t * work.tokens, work.tokens, group, it.head, st, work.causal, odd);
+        }
+    }
 }
 
 template <class T, int D, bool PAGED>
@@ -311,7 +475,8 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
     __shared__ uint64_t q_full[TILES], q_empty[TILES], k_full[ST * KP], k_empty[ST * KP], v_full[ST * VP], v_empty[ST * VP], s_full[2], p_full[2], o_full[TILES], o_free[TILES],
         pv_done[2];
     __shared__ uint32_t tmem_s;
-    __shared__ volatile int failed;
+    __shared__ volatile int failed, redo_s;  // redo_s: some row's result is not finite
+    __shared__ OddKeys odd_s;
     __shared__ float4 scales_s[kInfo];  // over the cache: K scales of a step's two pages, V scales
     __shared__ int present_s[kInfo];    // bit i: page i of the step exists
     __shared__ uint8_t q_up_s[PAGED ? 2 * TILES * 128 : 1];  // over the cache: log2 + 127 of what each row of Q was divided by, of a tile's last two items with steps
@@ -323,6 +488,7 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
 
     if (tid == 0) {
         failed = 0;
+        redo_s = 0;
         for (int i = 0; i < TILES; ++i) {
             tc::mbar_init(&q_full[i], PAGED ? 2 : 1);
             tc::mbar_init(&q_empty[i], 1);
@@ -403,44 +569,10 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
     tc::fence_after();
     const uint32_t tmem = tmem_s;
 
-    // Item i; the tiles with the latest tokens come first, they have the most keys where the mask is causal.
-    auto item_at = [&](unsigned i) {
-        Item<TILES> it;
-        int lo = 0, hi = n;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (start_s[mid] <= i) lo = mid;
-            else hi = mid;
-        }
-        const unsigned local = i - start_s[lo];
-        lo = order_s[lo];
-        const SeqItem q = info[lo];
-        const int count = (q.m + TILES * tokens - 1) / (TILES * tokens);
-        it.b = lo;
-        it.head = (int)(local % (unsigned)pr.heads);
-        it.first = (count - 1 - (int)(local / (unsigned)pr.heads)) * TILES * tokens;
-        it.len = q.len;
-        it.row = q.row;
-        it.m = q.m;
-        it.all = Steps{0, 0, 0};
-#pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-            const int f = it.first + t * tokens, base = q.len - q.m;
-            it.st[t] = f < q.m ? steps_of(base + f, base + imin(f + tokens, q.m) - 1, q.len, causal, window, sinks) : Steps{0, 0, 0};
-            if (it.st[t].hi > 0) {
-                const bool none = it.all.hi == 0;
-                it.all.hi = imax(it.all.hi, it.st[t].hi);
-                it.all.lo = none ? it.st[t].lo : imin(it.all.lo, it.st[t].lo);
-                it.all.head = imax(it.all.head, it.st[t].head);
-            }
-        }
-        it.all.head = imin(it.all.head, it.all.lo);
-        return it;
-    };
-
-    // The CTA's item in round r: there and back over the CTAs, so that a long one is followed by a short one.
+    const Items<TILES> work{info, start_s, order_s, n, tokens, (unsigned)pr.heads, items, causal, window, sinks};
+    auto item_at = [&](unsigned i) { return work.at(i); };
     const unsigned grid = gridDim.x;
-    auto item_no = [&](unsigned r) { return r & 1 ? (r + 1) * grid - 1 - blockIdx.x : r * grid + blockIdx.x; };
+    auto item_no = [&](unsigned r) { return work.number(r); };
 
     if (warp >= 8) fewer_registers<S::regs_other>();
     else if (warp < 4 * TILES) more_registers<S::regs_softmax>();
@@ -630,15 +762,19 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                 for (int j = 0; j < D / 8; ++j) *reinterpret_cast<uint4*>(dst + j * 8) = make_uint4(0, 0, 0, 0);
             }
             if (in && a.lse) a.lse[(size_t)t_row * a.q_heads + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
-            if (!PAGED) {
-                // not finite: a value the row sees, or one it does not (a later key, another sequence's row)
-                unsigned again = __ballot_sync(~0u, in && !(bad == 0.0f && l < INFINITY && m < INFINITY));
-                while (again) {
-                    const int who = __ffs((int)again) - 1;
-                    again &= again - 1;
-                    slow_row<T, D>(a, it.row, it.len, __shfl_sync(~0u, p, who), __shfl_sync(~0u, t_row, who), __shfl_sync(~0u, h, who), it.head, causal);
-                }
+            if (!PAGED && in && !(bad == 0.0f && l < INFINITY && m < INFINITY)) {
+                // not finite: by the row's own scores, which makes it NaN throughout, or by a value of V that it sees or not
+                if (!(l < INFINITY && m < INFINITY)) *reinterpret_cast<uint4*>(dst) = make_uint4(kOwnNaN, kOwnNaN, kOwnNaN, kOwnNaN);
+                else redo_s = 1;
             }
+        }
+        if constexpr (!PAGED) {
+            // Rows to be looked at again, when the CTA's pipeline has nothing to wait for any more: a row from its visible keys
+            // alone takes long.
+            softmax_sync<TILES>();
+            if (tid == 0) redo_s = redo_s && !failed;
+            softmax_sync<TILES>();
+            if (redo_s) redo_items<T, D, TILES>(a, Items<TILES>{info, start_s, order_s, n, tokens, (unsigned)pr.heads, items, causal, window, sinks}, group, &odd_s);
         }
     } else if (warp == 8) {
         // ---- the products: the warp runs converged, so that what the instructions take sits in uniform registers,

@@ -268,7 +268,8 @@ def window_attention(q, k, v, cu, max_len: int, causal: bool = True, window: int
     """Self-attention over ragged packed sequences (mrl_window_attention): q [tokens, q_heads, head_dim],
     k and v [tokens, kv_heads, head_dim], float16 or bfloat16; sequence b is rows cu[b] .. cu[b+1] - 1 (cu
     int32), at most max_len of them. A query at position p sees key j where j <= p (causal) and, with
-    window > 0, |p - j| < window or j < sinks. Returns out, or (out, lse [tokens, q_heads] float32)."""
+    window > 0, |p - j| < window or j < sinks. Returns out, or (out, lse [tokens, q_heads] float32).
+    dev.attention_status, an int32 CUDA tensor from the first call on, gets KV_TIMEOUT if a kernel gave up."""
     torch = _torch()
     dev = dev or default_device()
     q_row, q_head = _rows(q, "q", dev)

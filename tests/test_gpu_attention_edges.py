@@ -283,3 +283,86 @@ def test_unseen_value_scales_many_rows(M, dev, d, dtype, ratio):
         unseen_scale_case(M, dev, rng, 700, 660, 2, 4, d, dtype, 0, 0, [page], ratio, spread=5.0)
         unseen_scale_case(M, dev, rng, 700, 700, 1, 8, d, dtype, 40, 0, [page], ratio, spread=5.0)
         unseen_scale_case(M, dev, rng, 900, 600, 2, 4, d, dtype, 70, 4, [1, page], ratio, spread=5.0)
+
+
+# ---- values that are not finite, windowed attention ---------------------------------------------------------------
+
+
+def test_redone_rows_do_not_stop_the_call(M, dev):
+    """A very long sequence whose last value is not finite: the rows of its last tile that do not see it are computed from
+    400,000 keys each, and neither they nor the sequence behind them are given up."""
+    rng = np.random.default_rng(6)
+    n, m, d = 400000, 300, 64
+    q, k, v = (torch.from_numpy(rng.normal(0, 1, (n + m, 1, d)).astype(np.float32)).half().cuda() for _ in range(3))
+    v[n - 1, 0, 7] = float("inf")
+    out, lse = M.window_attention(q, k, v, i32([0, n, n + m]), max_len=n, causal=True, return_lse=True, dev=dev)
+    assert int(dev.attention_status) == 0
+    kn, vn = (x[:n - 1, 0].double() for x in (k, v))
+    first = n - 400
+    s = q[first:n - 1, 0].double() @ kn.T * d ** -0.5
+    s.masked_fill_(torch.arange(n - 1, device="cuda") > torch.arange(first, n - 1, device="cuda")[:, None], -math.inf)
+    want, wl = torch.softmax(s, 1) @ vn, torch.logsumexp(s, 1)
+    big = float((q[first:n - 1, 0].double().abs().max(0).values @ kn.abs().max(0).values) * d ** -0.5)
+    check_rows(out[first:n - 1, 0].double().cpu().numpy(), lse[first:n - 1, 0].double().cpu().numpy(), want.cpu().numpy(), wl.cpu().numpy(),
+               big, d, n, float(vn.abs().max()), U[q.dtype], U[q.dtype])
+    assert float(out[n - 1, 0, 7]) == math.inf and bool(torch.isfinite(out[n - 1, 0, :7]).all())
+    qn, kn, vn = (x[n:].double().cpu().numpy() for x in (q, k, v))
+    want, wl, big = plain_attention(qn, kn, vn, 0, True, 0, 0, d ** -0.5)
+    check_rows(out[n:].double().cpu().numpy(), lse[n:].double().cpu().numpy(), want, wl, big, d, m, np.abs(vn).max(), U[q.dtype], U[q.dtype])
+
+
+def plain_with_odd_values(q, k, v, causal, window, sinks, scale):
+    """plain_attention that keeps what is not visible out of the products: v may hold what is not finite."""
+    t, hq, d = q.shape
+    h = k.shape[1]
+    out = np.zeros((t, hq, d))
+    j = np.arange(t)
+    for i in range(t):
+        ok = np.ones(t, bool)
+        if causal:
+            ok &= j <= i
+        if window:
+            ok &= (np.abs(i - j) < window) | (j < sinks)
+        for a in range(hq):
+            with np.errstate(invalid="ignore"):
+                s = k[ok, a // (hq // h)] @ q[i, a] * scale
+                w = np.exp(s - s.max())
+                out[i, a] = (w / w.sum()) @ v[ok, a // (hq // h)]
+    return out
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("causal,window,sinks", [(True, 0, 0), (True, 60, 4), (False, 0, 0), (False, 90, 2)])
+def test_odd_values_seen_and_unseen(M, dev, d, dtype, causal, window, sinks):
+    """NaN and both infinities in values at several places, one of them a sink: every column of every row is what its
+    visible keys give, NaN and infinity included (weights of these scores are far from 0)."""
+    rng = np.random.default_rng(d + window)
+    t, h, g = 330, 2, 2
+    q, k, v = (torch.from_numpy(rng.normal(0, 0.7, (t, n, d))).to(dtype).cuda() for n in (h * g, h, h))
+    nan, inf = float("nan"), float("inf")
+    for key, head, dim, x in ((1, 0, 3, inf), (50, 0, 9, nan), (140, 1, 0, -inf), (141, 1, 0, inf), (200, 1, 5, inf), (300, 0, 60, nan)):
+        v[key, head, dim] = x
+    out = M.window_attention(q, k, v, i32([0, t]), max_len=t, causal=causal, window=window, sinks=sinks, dev=dev).double().cpu().numpy()
+    vn = v.double().cpu().numpy()
+    want = plain_with_odd_values(q.double().cpu().numpy(), k.double().cpu().numpy(), vn, causal, window, sinks, d ** -0.5)
+    assert np.array_equal(np.isnan(want), np.isnan(out))
+    odd = ~np.isfinite(want)
+    assert np.array_equal(want[odd & ~np.isnan(want)], out[odd & ~np.isnan(want)])
+    vmax = np.abs(vn[np.isfinite(vn)]).max()
+    check_rows(np.where(odd, 0, out), np.zeros(0), np.where(odd, 0, want), np.zeros(0), 0.0, d, t, vmax, U[dtype], U[dtype])
+
+
+@pytest.mark.parametrize("where", ["k", "q"])
+def test_odd_scores(M, dev, where):
+    """A NaN in a key makes every row that sees it NaN, in a query its own row; no other row changes."""
+    rng = np.random.default_rng(8)
+    t, d = 400, 128
+    q, k, v = (torch.from_numpy(rng.normal(0, 1, (t, n, d))).bfloat16().cuda() for n in (4, 2, 2))
+    clean, clean_lse = M.window_attention(q, k, v, i32([0, t]), max_len=t, window=100, return_lse=True, dev=dev)
+    (k if where == "k" else q)[170, 1] = float("nan")
+    out, lse = M.window_attention(q, k, v, i32([0, t]), max_len=t, window=100, return_lse=True, dev=dev)
+    rows, heads = (slice(170, 270), slice(2, 4)) if where == "k" else (slice(170, 171), slice(1, 2))
+    assert bool(torch.isnan(out[rows, heads]).all()) and bool(torch.isnan(lse[rows, heads]).all())
+    out[rows, heads], lse[rows, heads] = clean[rows, heads], clean_lse[rows, heads]
+    assert torch.equal(out, clean) and torch.equal(lse, clean_lse)
