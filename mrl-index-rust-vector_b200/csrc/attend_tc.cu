@@ -14,7 +14,7 @@
 // and its rounding is relative either way.
 //
 // Roles: warps 0-3 and 4-7 softmax and epilogue of the tiles, warp 8 issues the products, warp 9 loads Q, K
-// and V by TMA (16-bit rows); over the cache warp 9 copies blocks of codes that
+// and V by TMA (16-bit rows), where warp 10 clears V past a sequence's end; over the cache warp 9 copies blocks of codes that
 // a first launch has widened to f16 (exact) in the operand layout, once for all the tiles that read them, and
 // warps 10 and 11 bring in Q as f16; the blocks' scales go to S and P, which are f32 there. Every wait is bounded; when one runs out the kernel records it and ends.
 //
@@ -388,7 +388,7 @@ template <class T, int D> __device__ __noinline__ void slow_row(const mrl_attn& 
 }
 
 // A tile's rows whose fast result is not finite, all its softmax warps. A value of V that a row does not see (a later
-// key, another sequence's row) reaches its products as 0 x Inf: such a row is computed again from its visible keys. Where every
+// key, one before its window) reaches its products as 0 x Inf: such a row is computed again from its visible keys. Where every
 // odd value of V that the tile met is seen by the row, the fast result is the right one, except that an Inf under a weight that
 // rounds to 0 is a NaN there. Written by the same CTA before a barrier; rows marked kOwnNaN are right as they are.
 struct OddKeys {
@@ -414,7 +414,7 @@ template <class T, int D, int TILES> __device__ __forceinline__ void redo_tile(c
     if (look) {
         for (int s = 0; s < st.hi; ++s) {
             if (!st.has(s)) continue;
-            for (int j = s * kKeys + warp; j < (s + 1) * kKeys && row0 + j < (int)a.n_tokens; j += kWarps) {
+            for (int j = s * kKeys + warp; j < imin((s + 1) * kKeys, n); j += kWarps) {
                 uint32_t w[E / 2];
                 load16<E>(static_cast<const T*>(a.v) + (int64_t)(row0 + j) * a.v_row + (int64_t)kvh * a.v_head + lane * E, w);
                 const int kind = odd_values<T, E>(w);
@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
     __shared__ int seq_s[PAGED ? S::seqs : 1];
     __shared__ unsigned scan_s[32];
     constexpr int KP = S::k_parts, VP = S::v_parts;
-    __shared__ uint64_t q_full[TILES], q_empty[TILES], k_full[ST * KP], k_empty[ST * KP], v_full[ST * VP], v_empty[ST * VP], s_full[2], p_full[2], o_full[TILES], o_free[TILES],
+    __shared__ uint64_t q_full[TILES], q_empty[TILES], k_full[ST * KP], k_empty[ST * KP], v_full[ST * VP], v_empty[ST * VP], v_raw[ST * VP], s_full[2], p_full[2], o_full[TILES], o_free[TILES],
         pv_done[2];
     __shared__ uint32_t tmem_s;
     __shared__ volatile int failed, redo_s;  // redo_s: some row's result is not finite
@@ -502,6 +502,7 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
         for (int i = 0; i < ST * VP; ++i) {
             tc::mbar_init(&v_full[i], 1);
             tc::mbar_init(&v_empty[i], 1);
+            tc::mbar_init(&v_raw[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
             tc::mbar_init(&s_full[i], 1);
@@ -944,7 +945,8 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                                  pr.inner_k ? it.head : row, bar);
                     }
                     for (int part = 0; part < VP && ok; ++part) {
-                        uint64_t* bar = &v_full[stage * VP + part];
+                        // keys past the sequence's end: warp 10 has the stage first
+                        uint64_t* bar = s * kKeys + (part + 1) * (kKeys / VP) > it.len ? &v_raw[stage * VP + part] : &v_full[stage * VP + part];
                         ok = wait(&v_empty[stage * VP + part], par ^ 1, &failed);
                         if (!ok) break;
                         expect(bar, S::kv_bytes / VP);
@@ -953,6 +955,37 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                             tma3(tc::smem_u32(v_s + (size_t)stage * S::kv_bytes + part * (S::kv_bytes / VP) + d * (kKeys / VP * 128)), &map_v, d * 64,
                                  pr.inner_v ? v_row : it.head, pr.inner_v ? it.head : v_row, bar);
                     }
+                }
+            }
+        }
+        if (warp == 10) {
+            // ---- V of keys past the sequence's end set to zero: rows of another sequence, or of none, may hold anything, and
+            // 0 x NaN would reach every row of the item. Only an item's last step has such keys.
+            int step_no = 0;
+            uint32_t raw_par = 0;
+            bool ok = true;
+            for (unsigned r_no = 0; r_no * grid < items && ok && !failed; ++r_no) {
+                const unsigned i = item_no(r_no);
+                if (i >= items) break;
+                const Item<TILES> it = item_at(i);
+                if (it.all.hi == 0) continue;
+                step_no += it.all.head + it.all.hi - it.all.lo;
+                const int stage = (step_no - 1) % ST;
+                for (int part = 0; part < VP && ok; ++part) {
+                    constexpr int kRows = kKeys / VP;
+                    const int have = it.len - (it.all.hi - 1) * kKeys - part * kRows;
+                    if (have >= kRows) continue;
+                    const int x = stage * VP + part;
+                    ok = wait(&v_raw[x], (raw_par >> x) & 1, &failed);
+                    if (!ok) break;
+                    raw_par ^= 1u << x;
+                    unsigned char* v = v_s + (size_t)stage * S::kv_bytes + part * (S::kv_bytes / VP);
+                    const int from = imax(have, 0);
+                    for (int d = 0; d < D / 64; ++d)
+                        for (int y = from * 8 + lane; y < kRows * 8; y += 32) *reinterpret_cast<uint4*>(v + d * (kRows * 128) + y * 16) = make_uint4(0, 0, 0, 0);
+                    tc::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) arrive(&v_full[x]);
                 }
             }
         }

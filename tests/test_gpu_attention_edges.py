@@ -366,3 +366,22 @@ def test_odd_scores(M, dev, where):
     assert bool(torch.isnan(out[rows, heads]).all()) and bool(torch.isnan(lse[rows, heads]).all())
     out[rows, heads], lse[rows, heads] = clean[rows, heads], clean_lse[rows, heads]
     assert torch.equal(out, clean) and torch.equal(lse, clean_lse)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("causal,window", [(True, 0), (False, 0), (False, 100)])
+def test_rows_behind_a_sequence_do_not_matter(M, dev, d, dtype, causal, window):
+    """The rows behind a sequence, those of the next one or none's, hold NaN or Inf: its results keep every bit, as no
+    product of theirs meets them (sequences that end at, before and after a step of 128 keys and half of one)."""
+    rng = np.random.default_rng(d)
+    for n in (1, 60, 64, 65, 127, 128, 129, 190, 193, 400):
+        cu = i32([0, n, n + 140])
+        q, k, v = (torch.from_numpy(rng.normal(0, 1, (n + 300, x, d))).to(dtype).cuda() for x in (4, 2, 2))
+        f = lambda: M.window_attention(q, k, v, cu, max_len=max(n, 140), causal=causal, window=window, return_lse=True, dev=dev)  # noqa: E731
+        clean, clean_lse = f()
+        for x in (float("nan"), float("inf")):
+            for y in (q, k, v):
+                y[n:] = x
+            out, lse = f()
+            assert torch.equal(out[:n], clean[:n]) and torch.equal(lse[:n], clean_lse[:n])
