@@ -16,7 +16,8 @@
 // Roles: warps 0-3 and 4-7 softmax and epilogue of the tiles, warp 8 issues the products, warp 9 loads Q, K
 // and V by TMA (16-bit rows), where warp 10 clears V past a sequence's end; over the cache warp 9 copies blocks of codes that
 // a first launch has widened to f16 (exact) in the operand layout, once for all the tiles that read them, and
-// warps 10 and 11 bring in Q as f16; the blocks' scales go to S and P, which are f32 there. Every wait is bounded; when one runs out the kernel records it and ends.
+// warps 10 and 11 bring in Q as f16; the blocks' scales go to S and P, which are f32 there. Every wait is bounded; when one runs out
+// the kernel records it, waits for what it has in flight and ends.
 //
 // Bounds: per 128 keys a tile pair needs 2 x 2 x 128 x 128 x D products (2,048 clocks at head_dim 128) and 2 x 16,384
 // exponentials and as many conversions (about 2,560). What a pair takes is the chain of one tile's step, about 3,500
@@ -94,6 +95,26 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
     }
     return true;
 }
+// For a copy or product that may be in flight when its CTA has no more to do, as after a wait that ran out: the CTA does not
+// end before it, or before this limit.
+__device__ __noinline__ void settle(uint64_t* bar, uint32_t parity) {
+    const long long start = clock64();
+    while (!tc::mbar_wait(bar, parity, 16) && clock64() - start <= kWaitClocks) {}
+}
+// The fills of up to 8 barriers that a loading thread has issued: which, and the parity of the last one's phase.
+struct Fills {
+    uint32_t any = 0, parity = 0;
+    __device__ __forceinline__ void note(int i, uint32_t par) {
+        any |= 1u << i;
+        parity = (parity & ~(1u << i)) | par << i;
+    }
+    // barrier i's last fill is known to have landed, and its phases go on
+    __device__ __forceinline__ void drop(int i) { any &= ~(1u << i); }
+    __device__ __forceinline__ void settle_all(uint64_t* bars, int n) const {
+        for (int i = 0; i < n; ++i)
+            if (any >> i & 1) settle(&bars[i], parity >> i & 1);
+    }
+};
 __device__ __forceinline__ void arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc::smem_u32(bar)) : "memory");
 }
@@ -473,7 +494,7 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
     __shared__ unsigned scan_s[32];
     constexpr int KP = S::k_parts, VP = S::v_parts;
     __shared__ uint64_t q_full[TILES], q_empty[TILES], k_full[ST * KP], k_empty[ST * KP], v_full[ST * VP], v_empty[ST * VP], v_raw[ST * VP], s_full[2], p_full[2], o_full[TILES], o_free[TILES],
-        pv_done[2];
+        pv_done[2], drained;
     __shared__ uint32_t tmem_s;
     __shared__ volatile int failed, redo_s;  // redo_s: some row's result is not finite
     __shared__ OddKeys odd_s;
@@ -509,6 +530,7 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
             tc::mbar_init(&p_full[i], 4);
             tc::mbar_init(&pv_done[i], 1);
         }
+        tc::mbar_init(&drained, 1);
         tc::fence_mbar_init();
     }
     if (warp == 8) {
@@ -910,12 +932,17 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                 }
                 if (VP == 1 && prev >= 0 && ok) commit(&v_empty[prev % ST]);
             }
+            // no product, and no arrival of one on a barrier, outlasts the CTA
+            commit(&drained);
+            settle(&drained, 0);
         }
     } else if constexpr (!PAGED) {
         // ---- Q, K and V by TMA: boxes of 64 dims x 128 rows (Q: a tile's tokens x heads, V: a part's keys)
         if (warp == 9 && lane == 0) {
             int step_no = 0;
             uint32_t q_par = 0;
+            Fills q_fills, k_fills, v_fills, raw_fills;
+            uint32_t raw_par = 0;
             bool ok = true;
             for (unsigned r_no = 0; r_no * grid < items && ok && !failed; ++r_no) {
                 const unsigned i = item_no(r_no);
@@ -925,6 +952,7 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                     if (it.st[t].hi == 0) continue;
                     ok = wait(&q_empty[t], ((q_par >> t) & 1) ^ 1, &failed);
                     if (!ok) break;
+                    q_fills.note(t, (q_par >> t) & 1);
                     q_par ^= 1u << t;
                     expect(&q_full[t], (uint32_t)(tokens * group) * D * 2);
                     const int row = it.row + it.first + t * tokens, h = it.head * group;
@@ -940,16 +968,26 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                         ok = wait(&k_empty[stage * KP + part], par ^ 1, &failed);
                         if (!ok) break;
                         expect(bar, S::kv_bytes / KP);
+                        k_fills.note(stage * KP + part, par);
                         for (int d = part * (D / 64 / KP); d < (part + 1) * (D / 64 / KP); ++d)
                             tma3(tc::smem_u32(k_s + (size_t)stage * S::kv_bytes + d * 16384), &map_k, d * 64, pr.inner_k ? row : it.head,
                                  pr.inner_k ? it.head : row, bar);
                     }
                     for (int part = 0; part < VP && ok; ++part) {
                         // keys past the sequence's end: warp 10 has the stage first
-                        uint64_t* bar = s * kKeys + (part + 1) * (kKeys / VP) > it.len ? &v_raw[stage * VP + part] : &v_full[stage * VP + part];
-                        ok = wait(&v_empty[stage * VP + part], par ^ 1, &failed);
+                        const int x = stage * VP + part;
+                        const bool cut = s * kKeys + (part + 1) * (kKeys / VP) > it.len;
+                        uint64_t* bar = cut ? &v_raw[x] : &v_full[x];
+                        ok = wait(&v_empty[x], par ^ 1, &failed);
                         if (!ok) break;
                         expect(bar, S::kv_bytes / VP);
+                        if (cut) {
+                            raw_fills.note(x, (raw_par >> x) & 1);
+                            raw_par ^= 1u << x;
+                            v_fills.drop(x);  // warp 10 ends that barrier's phase
+                        } else {
+                            v_fills.note(x, par);
+                        }
                         const int v_row = row + part * (kKeys / VP);
                         for (int d = 0; d < D / 64; ++d)
                             tma3(tc::smem_u32(v_s + (size_t)stage * S::kv_bytes + part * (S::kv_bytes / VP) + d * (kKeys / VP * 128)), &map_v, d * 64,
@@ -957,6 +995,10 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                     }
                 }
             }
+            q_fills.settle_all(q_full, TILES);
+            k_fills.settle_all(k_full, ST * KP);
+            v_fills.settle_all(v_full, ST * VP);
+            raw_fills.settle_all(v_raw, ST * VP);
         }
         if (warp == 10) {
             // ---- V of keys past the sequence's end set to zero: rows of another sequence, or of none, may hold anything, and
@@ -994,6 +1036,7 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
         if (lane == 0) {
             const mrl_kv_cache& c = pr.c;
             int step_no = 0;
+            Fills k_fills, v_fills;
             bool ok = true;
             for (unsigned r_no = 0; r_no * grid < items && ok && !failed; ++r_no) {
                 const unsigned i = item_no(r_no);
@@ -1026,6 +1069,7 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                         ok = wait(&k_empty[stage * KP + part], par ^ 1, &failed);
                         if (!ok) break;
                         expect(bar, S::kv_bytes / KP);
+                        k_fills.note(stage * KP + part, par);
                         for (int d = part * (D / 64 / KP); d < (part + 1) * (D / 64 / KP); ++d) {
                             const uint32_t to = tc::smem_u32(k_s + (size_t)stage * S::kv_bytes + d * 16384);
                             bulk(to, w0 + d * 8192, 8192, bar);
@@ -1037,6 +1081,7 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                         ok = wait(&v_empty[stage * VP + part], par ^ 1, &failed);
                         if (!ok) break;
                         expect(bar, S::kv_bytes / VP);
+                        v_fills.note(stage * VP + part, par);
                         const uint32_t to = tc::smem_u32(v_s + (size_t)stage * S::kv_bytes);
                         if (part == 0) bulk(to, image(p0, 1), kWide<D>, bar);
                         if (part == VP - 1) bulk(to + kWide<D>, image(p1, 1), kWide<D>, bar);
@@ -1050,6 +1095,8 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
                     if (s1 < it.all.hi) n0 = page_of(2 * s1), n1 = page_of(2 * s1 + 1);
                 }
             }
+            k_fills.settle_all(k_full, ST * KP);
+            v_fills.settle_all(v_full, ST * VP);
         }
     } else if (warp >= 10) {
         // ---- Q of the cache's attention, as f16

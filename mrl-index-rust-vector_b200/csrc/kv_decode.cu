@@ -95,6 +95,8 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
         }
     }
 }
+// After a wait has run out: the warp does not end while its load is in flight, or before this limit.
+__device__ __noinline__ void settle(uint32_t bar, uint32_t parity) { bar_wait(bar, parity); }
 // A team is `threads` threads of consecutive warps; one warp needs no barrier resource.
 __device__ __forceinline__ void team_sync(int team, int threads) {
     if (threads == 32) __syncwarp();
@@ -465,7 +467,11 @@ template <class T, int D, bool WIDE> __global__ void __launch_bounds__(kWarps<D>
                 fetch(1);
                 continue;
             }
-            fine = fine && bar_wait(bar_k, parity);
+            if (fine && !bar_wait(bar_k, parity)) {
+                fine = false;
+                settle(bar_k, parity);
+                settle(bar_v, parity);
+            }
             float sc[8][4];
 #pragma unroll
             for (int j = 0; j < 8; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.0f;
@@ -576,7 +582,11 @@ template <class T, int D, bool WIDE> __global__ void __launch_bounds__(kWarps<D>
                     pf[x][2 * y + 1] = pack_half(w[2] * vf1, w[3] * vf1);
                 }
             }
-            fine = fine && bar_wait(bar_v, parity);
+            if (fine && !bar_wait(bar_v, parity)) {
+                fine = false;
+                settle(bar_v, parity);
+                if (npage >= 0) settle(bar_k, parity ^ 1);
+            }
             parity ^= 1;
             if (fine) {
 #pragma unroll
