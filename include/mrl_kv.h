@@ -39,8 +39,9 @@ extern "C" {
 /* Bits of mrl_kv_cache.status, set by the device and cleared by the caller. */
 #define MRL_KV_NO_PAGES 1u   /* a reserve or fork needed more free pages than there are; it did nothing */
 #define MRL_KV_ROW_FULL 2u   /* a reserve needed more than max_pages pages for a sequence; it did nothing */
-#define MRL_KV_BAD_INDEX 4u  /* a sequence, page or count out of range, or a fork onto a sequence that
-                                is not empty or onto its own parent; the operation did nothing */
+#define MRL_KV_BAD_INDEX 4u  /* a sequence, page or count out of range, a fork of an empty sequence, onto one that is
+                                not empty or onto its own parent, or attention with row offsets that decrease; the
+                                operation did nothing (attention: for the 512 or 1,024 sequences around them) */
 #define MRL_KV_NONFINITE 8u  /* an append met an Inf (stored as the largest code) or a NaN (stored as 0) */
 #define MRL_KV_TIMEOUT 16u   /* a kernel gave up waiting for its own loads; the call's outputs mean nothing */
 
@@ -122,7 +123,8 @@ typedef struct mrl_attn {
     float* lse; /* [n_tokens][q_heads], or NULL */
     const int32_t* seqs; /* mrl_kv_attend only */
     const int32_t* cu;
-    uint32_t* status; /* mrl_window_attention: receives MRL_KV_TIMEOUT, or NULL (mrl_kv_attend reports to the cache's) */
+    uint32_t* status; /* mrl_window_attention: receives MRL_KV_TIMEOUT and MRL_KV_BAD_INDEX, or NULL (mrl_kv_attend
+                         reports to the cache's) */
     int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head;
     uint32_t n_seqs, n_tokens, max_rows; /* max_rows: at least the rows of every sequence */
     uint32_t q_heads, kv_heads, head_dim, dtype;

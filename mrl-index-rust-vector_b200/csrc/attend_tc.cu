@@ -538,8 +538,10 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
         tc::tmem_relinquish();
     }
     // ---- the call's sequences, longest first where there are few, so that the last items are short ones
+    bool falls = false;
     for (int b = tid; b < n; b += S::threads) {
         const Rows r{a.seqs, a.cu, n, (int)a.n_tokens};
+        falls = falls || r.falls(b);
         SeqItem q{0, r.begin(b), 0};
         q.m = r.end(b) - q.row;
         q.len = q.m;
@@ -551,7 +553,8 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
         }
         info[b] = q;
     }
-    __syncthreads();
+    const bool none = __syncthreads_or(falls);  // the items
+    if (none && blockIdx.x == 0 && tid == 0 && (PAGED || a.status)) atomicOr(PAGED ? pr.c.status : a.status, MRL_KV_BAD_INDEX);
     for (int b = tid; b < n; b += S::threads) {
         int rank = b;
         if (n <= 128) {
@@ -568,7 +571,7 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
         unsigned v = 0;
         if (b < n) {
             const int m = info[order_s[b]].m;
-            v = m > 0 ? (unsigned)((m + TILES * tokens - 1) / (TILES * tokens)) * (unsigned)pr.heads : 0;
+            v = m > 0 && !none ? (unsigned)((m + TILES * tokens - 1) / (TILES * tokens)) * (unsigned)pr.heads : 0;
         }
         unsigned x = v;
 #pragma unroll

@@ -37,6 +37,9 @@ struct Rows {
     int n, tokens;
     __device__ __forceinline__ int begin(int b) const { return cu ? min(max(cu[b], 0), tokens) : b; }
     __device__ __forceinline__ int end(int b) const { return cu ? min(max(cu[b + 1], 0), tokens) : b + 1; }
+    // Offsets that decrease at b. Where none do, the sequences' rows are at most `tokens` together, and sums over them
+    // stay in range; else a call does nothing.
+    __device__ __forceinline__ bool falls(int b) const { return cu && cu[b + 1] < cu[b]; }
 };
 
 // Largest b in [0, n) with f(b) <= x, f not decreasing, f(0) <= x: 32 probes a step by one warp.

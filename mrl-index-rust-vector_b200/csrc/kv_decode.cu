@@ -178,7 +178,9 @@ template <class T, int D, bool WIDE> __global__ void __launch_bounds__(kWarps<D>
     // ---- the call's sequences: their items and pages, summed up
     const Rows rows{a.seqs, a.cu, n, (int)a.n_tokens};
     unsigned my_units = 0;
+    bool falls = false;
     for (int b = tid; b < n; b += kThreads) {
+        falls = falls || rows.falls(b);
         SeqInfo s;
         s.row = a.cu ? rows.begin(b) : pr.row0 + b;
         s.m = a.cu ? rows.end(b) - s.row : 1;
@@ -206,7 +208,8 @@ template <class T, int D, bool WIDE> __global__ void __launch_bounds__(kWarps<D>
     // team's border; beyond that every team takes an equal share. Measured, 8 sequences of 1,000 tokens and 8 kv heads
     // of 128: 12.0 us with jobs, 15.1 us with shares.
     pl.few = WIDE && pl.units <= (unsigned)(pl.teams * W);
-    __syncthreads();  // scan_s is read
+    const bool none = __syncthreads_or(falls);  // and scan_s is read
+    if (none && blockIdx.x == 0 && tid == 0) atomicOr(c.status, MRL_KV_BAD_INDEX);
     // An item costs its pages and a fixed part (Q, joining, writing: about 1.5 pages' time of a warp), so equal
     // shares are of pages + `fixed` per item. A share that would begin in an item's fixed part begins with the item.
     const unsigned fixed = pl.few ? 0 : (unsigned)(3 * W + 1) / 2;
@@ -215,7 +218,7 @@ template <class T, int D, bool WIDE> __global__ void __launch_bounds__(kWarps<D>
     for (int at = 0; at < n; at += kThreads) {
         const int b = at + tid;
         unsigned v = 0;
-        if (b < n && info[b].m > 0) {
+        if (b < n && info[b].m > 0 && !none) {
             const int np = max(1, page_span(info[b].len, info[b].m, window, sinks).n);
             v = (unsigned)((info[b].m * group + 15) / 16) * c.kv_heads * (pl.few ? (unsigned)((np + W - 1) / W) : np + fixed);
         }

@@ -241,7 +241,7 @@ class KvCache:
 
 def _call_buffer(dev: Device, like):
     """What a device's calls without a cache keep: the argument struct, its address, and the status
-    word (Device.attention_status: KV_TIMEOUT or 0)."""
+    word (Device.attention_status: KV_TIMEOUT and KV_BAD_INDEX bits)."""
     dev.attention_status = _torch_module.zeros(1, dtype=_torch_module.int32, device=like.device)
     buf = bytearray(_ATTN.size)
     dev.attention_call = (buf, C.addressof((C.c_char * _ATTN.size).from_buffer(buf)), dev.attention_status)
@@ -269,7 +269,8 @@ def window_attention(q, k, v, cu, max_len: int, causal: bool = True, window: int
     k and v [tokens, kv_heads, head_dim], float16 or bfloat16; sequence b is rows cu[b] .. cu[b+1] - 1 (cu
     int32), at most max_len of them. A query at position p sees key j where j <= p (causal) and, with
     window > 0, |p - j| < window or j < sinks. Returns out, or (out, lse [tokens, q_heads] float32).
-    dev.attention_status, an int32 CUDA tensor from the first call on, gets KV_TIMEOUT if a kernel gave up."""
+    dev.attention_status, an int32 CUDA tensor from the first call on, gets
+    KV_BAD_INDEX if cu decreases (nothing is computed then) and KV_TIMEOUT if a kernel gave up."""
     torch = _torch()
     dev = dev or default_device()
     q_row, q_head = _rows(q, "q", dev)

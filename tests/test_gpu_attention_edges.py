@@ -385,3 +385,27 @@ def test_rows_behind_a_sequence_do_not_matter(M, dev, d, dtype, causal, window):
                 y[n:] = x
             out, lse = f()
             assert torch.equal(out[:n], clean[:n]) and torch.equal(lse[:n], clean_lse[:n])
+
+
+# ---- index tensors whose contents are wrong -----------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("n_seqs,rows", [(4, 8), (200, 8), (4, 300), (200, 300)])
+def test_decreasing_offsets_do_nothing(M, dev, n_seqs, rows):
+    """Offsets that decrease give no rows at all, and the status bit: sums over them could leave every range."""
+    rng = np.random.default_rng(n_seqs)
+    t = n_seqs * rows
+    cache, *_ = filled_cache(M, rng, dev, [rows] * n_seqs, 2, 64)
+    q, k, v = (torch.from_numpy(rng.normal(0, 1, (t, h, 64)).astype(np.float32)).half().cuda() for h in (4, 2, 2))
+    good = cu_of([rows] * n_seqs)
+    bad = good.clone()
+    bad[2] = 1
+    for cu, bits in ((bad, 4), (good, 0)):
+        out = torch.full_like(q, 7.0)
+        cache.attend(0, q, i32(range(n_seqs)), cu, max_q=rows, out=out)
+        assert int(cache.status) == bits and bool((out == 7.0).all()) == (cu is bad)
+        out = torch.full_like(q, 7.0)
+        M.window_attention(q, k, v, cu, max_len=rows, out=out, dev=dev)
+        assert int(dev.attention_status) == bits and bool((out == 7.0).all()) == (cu is bad)
+        cache.status.zero_()
+        dev.attention_status.zero_()
