@@ -103,17 +103,19 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_kernel(mrl_kv_cache c, c
     if (tid == 0) bad = 0;
     __syncthreads();
     // Each listed sequence's length carries a mark while its need is counted: a sequence listed twice,
-    // or one whose length is not a length, shows.
+    // or one whose length is not a length, shows. Entries that set no mark have offset -1.
     long long need_all = 0;
     for (int at = 0; at < n; at += kPlanThreads) {
         const int i = at + tid;
         int need = 0;
+        bool marked = false;
         if (i < n) {
             const int s = seqs[i], a = add[i];
             if (!in_range(s, c.max_seqs) || a < 0) {
                 atomicOr(&bad, MRL_KV_BAD_INDEX);
             } else {
                 const int len = atomicOr(&c.lens[s], kMark);
+                marked = len >= 0;
                 if (len < 0) {
                     atomicOr(&bad, MRL_KV_BAD_INDEX);
                 } else if ((long long)len + a > (long long)c.max_pages * kPage) {
@@ -125,7 +127,7 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_kernel(mrl_kv_cache c, c
         }
         int total;
         const int x = block_scan(need, &total, sh);
-        if (i < n) l.off[i] = (int)min(need_all + x, (long long)INT32_MAX);
+        if (i < n) l.off[i] = marked ? (int)min(need_all + x, (long long)INT32_MAX) : -1;
         need_all += total;
     }
     __syncthreads();
@@ -138,7 +140,7 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_kernel(mrl_kv_cache c, c
     __syncthreads();
     if (bad) {
         for (int i = tid; i < n; i += kPlanThreads)
-            if (in_range(seqs[i], c.max_seqs)) atomicAnd(&c.lens[seqs[i]], ~kMark);
+            if (l.off[i] >= 0) atomicAnd(&c.lens[seqs[i]], ~kMark);
         if (tid == 0) atomicOr(c.status, bad);
         return;
     }
@@ -170,13 +172,15 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(mrl_kv_cache c,
     for (int at = 0; at < n; at += kPlanThreads) {
         const int i = at + tid;
         int need = 0;
+        bool marked = false;
         if (i < n) {
             const int p = parents[i], ch = children[i];
             if (!in_range(p, c.max_seqs) || !in_range(ch, c.max_seqs)) {
                 atomicOr(&bad, MRL_KV_BAD_INDEX);
             } else {
-                const int len = c.lens[p];
-                if (p == ch || atomicOr(&c.lens[ch], kMark) != 0 || len <= 0 || len > (long long)c.max_pages * kPage) {
+                const int len = c.lens[p], was = p == ch ? -1 : atomicOr(&c.lens[ch], kMark);
+                marked = was >= 0;
+                if (was != 0 || len <= 0 || len > (long long)c.max_pages * kPage) {
                     atomicOr(&bad, MRL_KV_BAD_INDEX);
                 } else if (len % kPage) {
                     need = in_range(c.tables[(size_t)p * c.max_pages + len / kPage], c.pages);
@@ -185,7 +189,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(mrl_kv_cache c,
         }
         int total;
         const int x = block_scan(need, &total, sh);
-        if (i < n) l.off[i] = tails + x;
+        if (i < n) l.off[i] = marked ? tails + x : -1;
         tails += total;
     }
     __syncthreads();
@@ -196,7 +200,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(mrl_kv_cache c,
     __syncthreads();
     if (bad) {
         for (int i = tid; i < n; i += kPlanThreads)
-            if (in_range(children[i], c.max_seqs)) atomicAnd(&c.lens[children[i]], ~kMark);
+            if (l.off[i] >= 0) atomicAnd(&c.lens[children[i]], ~kMark);
         if (tid == 0) {
             atomicOr(c.status, bad);
             l.count[0] = -1;

@@ -409,3 +409,21 @@ def test_decreasing_offsets_do_nothing(M, dev, n_seqs, rows):
         assert int(dev.attention_status) == bits and bool((out == 7.0).all()) == (cu is bad)
         cache.status.zero_()
         dev.attention_status.zero_()
+
+
+def test_refused_page_operations_leave_every_length(M, dev):
+    """A refused reserve or fork changes nothing, lengths that are none (negative) included."""
+    cache = M.KvCache.create(1, 8, 1, 64, 6, 4, dev=dev)
+    cache.reserve(i32([0, 1]), i32([70, 10]))
+    cache.lens[2], cache.lens[3] = -5, -(1 << 31)
+    before = [x.clone() for x in (cache.tables, cache.lens, cache.refs)]
+    tried = [lambda: cache.reserve(i32([0, 2]), i32([1, 1])), lambda: cache.reserve(i32([3, 1, 3, 1]), i32([1] * 4)),
+             lambda: cache.reserve(i32([4, 4]), i32([1, 1])), lambda: cache.fork(i32([0]), i32([2])),
+             lambda: cache.fork(i32([0, 0, 1]), i32([3, 4, 1])), lambda: cache.fork(i32([2]), i32([4])),
+             lambda: cache.fork(i32([0, 0]), i32([5, 5]))]
+    for f in tried:
+        f()
+        assert int(cache.status) == 4
+        for x, y in zip(before, (cache.tables, cache.lens, cache.refs)):
+            assert torch.equal(x, y)
+        cache.status.zero_()
