@@ -229,9 +229,10 @@ class Device:
     def stream(self) -> int:
         return int(self.lib.mrl_ctx_stream(self.ptr) or 0)
 
-    def set_stream(self, stream: int) -> None:
+    def set_stream(self, stream: Optional[int]) -> None:
+        """Launch on this CUDA stream handle from now on; None or 0: the context's own stream."""
         check(self.ptr, self.lib.mrl_ctx_set_stream(self.ptr, C.c_void_p(stream)))
-        self.torch_stream = int(stream) or None
+        self.torch_stream = int(stream or 0) or None
 
     def use_torch_stream(self) -> None:
         """Launch on torch's current stream of this device from now on. The attention operators (KvCache,
