@@ -41,7 +41,10 @@ extern "C" {
 #define MRL_KV_ROW_FULL 2u   /* a reserve needed more than max_pages pages for a sequence; it did nothing */
 #define MRL_KV_BAD_INDEX 4u  /* a sequence, page or count out of range, a fork of an empty sequence, onto one that is
                                 not empty or onto its own parent, or attention with row offsets that decrease; the
-                                operation did nothing (attention: for the 512 or 1,024 sequences around them) */
+                                operation did nothing (attention: for the 512 or 1,024 sequences around them). Also
+                                rows of an unknown sequence, or more rows than it has tokens, in an append, a
+                                read or an attention over the cache, and appended rows whose page is missing: those
+                                are not stored, read as 0, or see no key, and the others are as they should be */
 #define MRL_KV_NONFINITE 8u  /* an append met an Inf (stored as the largest code) or a NaN (stored as 0) */
 #define MRL_KV_TIMEOUT 16u   /* a kernel gave up waiting for its own loads; the call's outputs mean nothing */
 
@@ -101,13 +104,13 @@ int mrl_kv_copy_pages(mrl_ctx* ctx, const mrl_kv_cache* kv, const int32_t* d_src
  * tokens gets scale a * (1/127); otherwise the old scale s stays where a <= 127 s, else it becomes
  * max(a * (1/127), 2 s) and the older codes are rounded to it (it at least doubles, so all such
  * roundings of a code together stay below one step). code = clamp(rint(x / scale), -127, 127), NaN
- * and scale 0 give 0. */
+ * and scale 0 give 0. Rows whose page or sequence is missing are not stored (MRL_KV_BAD_INDEX). */
 int mrl_kv_append(mrl_ctx* ctx, const mrl_kv_cache* kv, uint32_t layer, uint32_t dtype, const void* k, int64_t k_row,
                   int64_t k_head, const void* v, int64_t v_row, int64_t v_head, const int32_t* d_seqs,
                   const int32_t* d_cu, uint32_t n_seqs, uint32_t n_tokens);
 /* The values the cache holds for those rows, into contiguous [n_tokens][kv_heads][head_dim] outputs of
  * dtype MRL_F16, MRL_BF16 or MRL_F32 (code * scale in f32, rounded once). Rows whose page
- * or sequence is missing are 0. */
+ * or sequence is missing are 0; where it is the sequence, MRL_KV_BAD_INDEX is set. */
 int mrl_kv_read(mrl_ctx* ctx, const mrl_kv_cache* kv, uint32_t layer, uint32_t dtype, void* k, void* v,
                 const int32_t* d_seqs, const int32_t* d_cu, uint32_t n_seqs, uint32_t n_tokens);
 
@@ -133,7 +136,8 @@ typedef struct mrl_attn {
     uint32_t layer; /* mrl_kv_attend only */
 } mrl_attn;
 /* Attention of the last rows of sequences over the cache (always causal; k, v, kv_heads, head_dim
- * and causal of `a` are not read). Softmax statistics and sums in f32. Any max_rows is right; it
+ * and causal of `a` are not read). Rows of an unknown sequence, and rows beyond a sequence's tokens, see no
+ * key, and MRL_KV_BAD_INDEX is set. Softmax statistics and sums in f32. Any max_rows is right; it
  * helps to choose the kernel: calls of few rows read the pages as codes; calls of many widen them first, into
  * scratch of twice the size of a layer's codes, or read the codes too where the device has no room for it. Work of the former is counted in 32 bits: (n_tokens x group
  * / 16 + n_seqs) x kv_heads x (max_pages + 16), per 1024 sequences where cu is NULL, must stay below 2^32. */

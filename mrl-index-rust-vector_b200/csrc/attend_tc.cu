@@ -550,6 +550,7 @@ __global__ void __launch_bounds__(Shape<D, PAGED>::threads, 1)
             const bool known = seq >= 0 && seq < (int)pr.c.max_seqs;
             seq_s[b] = known ? seq : 0;
             q.len = known ? min(max(pr.c.lens[seq], 0), (int)pr.c.max_pages * kPage) : 0;
+            if (blockIdx.x == 0 && q.m > 0 && (!known || q.m > q.len)) atomicOr(pr.c.status, MRL_KV_BAD_INDEX);
         }
         info[b] = q;
     }

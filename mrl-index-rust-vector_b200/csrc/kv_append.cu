@@ -266,7 +266,11 @@ template <class T, int D, bool FEW> __global__ void __launch_bounds__(kThreads) 
     __shared__ float smax[kWarps];
     __shared__ uint32_t tile[D * (kPage / 4 + 1)];  // V's codes, a dim's 64 tokens and a padding word
     const PageUnit u = cta_page(c, r, &su);
-    if (u.page < 0 || u.count == 0) return;
+    if (u.count == 0) return;
+    if (u.page < 0) {  // these rows have nowhere to go
+        if (threadIdx.x == 0 && blockIdx.y == 0) atomicOr(c.status, MRL_KV_BAD_INDEX);
+        return;
+    }
     if constexpr (FEW) {
         const int first = (int)blockIdx.y * kWarps, blocks = min(kWarps, 2 * (int)c.kv_heads - first);
         if (u.count <= kFew) {
@@ -307,6 +311,7 @@ template <class O, int D> __global__ void __launch_bounds__(kThreads) read_kerne
     const int tid = (int)threadIdx.x;
     const PageUnit u = cta_page(c, r, &su);
     if (u.count == 0) return;
+    if (u.seq < 0 && tid == 0 && blockIdx.y == 0) atomicOr(c.status, MRL_KV_BAD_INDEX);
     const int first = (int)blockIdx.y * per, blocks = min(per, 2 * (int)c.kv_heads - first);
     const size_t stride = (size_t)c.kv_heads * D;
     if (u.count <= kFew) {  // a warp per block

@@ -188,6 +188,7 @@ template <class T, int D, bool WIDE> __global__ void __launch_bounds__(kWarps<D>
         const bool known = seq >= 0 && seq < (int)c.max_seqs;
         s.len = known ? min(max(c.lens[seq], 0), (int)c.max_pages * kPage) : 0;
         seq_s[b] = known ? seq : -1;
+        if (blockIdx.x == 0 && s.m > 0 && (!known || s.m > s.len)) atomicOr(c.status, MRL_KV_BAD_INDEX);
         s.start = 0;
         info[b] = s;
         if (WIDE && s.m > 0)

@@ -12,7 +12,8 @@ sliding-window attention over ragged 16-bit inputs. Tensors are torch CUDA tenso
 Every call is asynchronous and ordered after the work on torch's current stream, and later work on that
 stream after it: a Device whose launches are on that stream (Device.use_torch_stream) needs nothing for
 this, another one gets events. What only the contents of index tensors can show (a sequence out of
-range, a full pool) does not raise: it sets bits of `cache.status` and the operation does nothing.
+range, a full pool) does not raise: it sets bits of `cache.status`, and a page operation does nothing, while
+append, read and attend leave out the rows that are meant (not stored, 0, 0 with lse -inf).
 """
 from __future__ import annotations
 

@@ -427,3 +427,48 @@ def test_refused_page_operations_leave_every_length(M, dev):
         for x, y in zip(before, (cache.tables, cache.lens, cache.refs)):
             assert torch.equal(x, y)
         cache.status.zero_()
+
+
+def test_rows_that_are_left_out_set_the_status(M, dev):
+    """Unknown sequences, more rows than tokens and missing pages: an append, a read and both attention kernels say that
+    rows were left out, and the other rows are right."""
+    rng = np.random.default_rng(11)
+    cache = M.KvCache.create(1, 40, 2, 64, 4, 12, dev=dev)
+
+    def new(t, h=2):
+        return torch.from_numpy(rng.normal(0, 1, (t, h, 64)).astype(np.float32)).half().cuda()
+
+    def status():
+        s = int(cache.status)
+        cache.status.zero_()
+        return s
+
+    cache.reserve(i32([0, 1, 2]), i32([100, 300, 10]))
+    k = new(410)
+    cache.append(0, k, k, i32([0, 1, 2]), cu_of([100, 300, 10]))
+    assert status() == 0
+    codes, scales = cache.codes.clone(), cache.scales.clone()
+    for seqs, rows in (([4], [3]), ([-1], [70]), ([2], [11]), ([3], [1]), ([1 << 30, -5], [1, 1])):
+        x = new(sum(rows))
+        cache.append(0, x, x, i32(seqs), cu_of(rows))
+        assert status() == 4 and torch.equal(codes, cache.codes) and torch.equal(scales, cache.scales)
+        got, _ = cache.read(0, i32(seqs), cu_of(rows), tokens=sum(rows))
+        assert status() == 4 and not bool(got.any())
+    for rows in ([100, 40, 300], [1, 1, 1]):
+        q = new(sum(rows), 8)
+        out = cache.attend(0, q, i32([0, 1 << 30, 1]), cu_of(rows), max_q=max(rows))
+        assert status() == 4
+        keep = torch.cat([q[:rows[0]], q[-rows[2]:]])
+        assert torch.equal(torch.cat([out[:rows[0]], out[-rows[2]:]]),
+                           cache.attend(0, keep, i32([0, 1]), cu_of([rows[0], rows[2]]), max_q=max(rows)))
+        assert status() == 0
+    assert bool((cache.attend(0, new(3, 8), i32([0, -1, 1]))[1] == 0).all()) and status() == 4
+    cache.attend(0, new(12, 8), i32([2]), cu_of([12]), max_q=12)
+    assert status() == 4
+    # a page that was given back: appended rows that belong there are lost, reads of it are 0 by definition
+    cache.trim(i32([1]), 64)
+    x = new(300)
+    cache.append(0, x, x, i32([1]), cu_of([300]))
+    assert status() == 4
+    cache.read(0, i32([1]), cu_of([300]), tokens=300)
+    assert status() == 0
