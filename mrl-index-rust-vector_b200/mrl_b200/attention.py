@@ -14,6 +14,8 @@ stream after it: a Device whose launches are on that stream (Device.use_torch_st
 this, another one gets events. What only the contents of index tensors can show (a sequence out of
 range, a full pool) does not raise: it sets bits of `cache.status`, and a page operation does nothing, while
 append, read and attend leave out the rows that are meant (not stored, 0, 0 with lse -inf).
+
+Nothing here has a backward pass: a tensor that requires gradients is refused while gradients are recorded.
 """
 from __future__ import annotations
 
@@ -86,6 +88,8 @@ def _rows(x, name: str, dev: Device, heads=None, dims=None, dtype=None, tokens=N
                          f"{heads if heads is not None else 'heads'}, {dims if dims is not None else 'head_dim'}]")
     if dtype is not None and x.dtype is not dtype:
         raise ValueError(f"{name} is {x.dtype}, not {dtype}")
+    if x.requires_grad and _torch_module.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient, and there is none here: call under torch.no_grad() or detach it")
     row, head, one = x.stride()
     if one != 1:
         raise ValueError(f"{name}'s last dimension must be contiguous")

@@ -472,3 +472,26 @@ def test_rows_that_are_left_out_set_the_status(M, dev):
     assert status() == 4
     cache.read(0, i32([1]), cu_of([300]), tokens=300)
     assert status() == 0
+
+
+# ---- refusals ---------------------------------------------------------------------------------------------------------
+
+
+def test_gradients_are_refused_not_dropped(M, dev):
+    """A tensor that requires gradients is refused while they are recorded: the result would be detached without a word."""
+    half = lambda *s: torch.zeros(*s, dtype=torch.float16, device="cuda")  # noqa: E731
+    cache = M.KvCache.create(1, 4, 2, 64, 3, 2, dev=dev)
+    seqs, cu = i32([0, 1]), i32([0, 2])
+    cache.reserve(seqs, i32([1, 1]))
+    g = half(2, 2, 64).requires_grad_()
+    calls = [lambda: cache.append(0, g, half(2, 2, 64), seqs), lambda: cache.append(0, half(2, 2, 64), g, seqs),
+             lambda: cache.attend(0, g, seqs), lambda: cache.attend(0, half(2, 2, 64), seqs, out=g),
+             lambda: M.window_attention(g, half(2, 2, 64), half(2, 2, 64), cu, 2, dev=dev),
+             lambda: M.window_attention(half(2, 2, 64), g, half(2, 2, 64), cu, 2, dev=dev),
+             lambda: M.window_attention(half(2, 2, 64), half(2, 2, 64), g, cu, 2, dev=dev)]
+    for f in calls:
+        with pytest.raises(ValueError, match="gradient"):
+            f()
+        with torch.no_grad():
+            f()
+    assert int(cache.status) == 0
