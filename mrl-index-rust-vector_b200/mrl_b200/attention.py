@@ -209,11 +209,13 @@ class KvCache:
 
     def read(self, layer: int, seqs, cu=None, tokens: Optional[int] = None, dtype=None):
         """(k, v), [tokens, kv_heads, head_dim]: the values held for the same rows as append's
-        (mrl_kv_read). dtype float32 (default), float16 or bfloat16."""
+        (mrl_kv_read), tokens in all where cu is given. dtype float32 (default), float16 or bfloat16."""
         torch, dev = _torch_module, self.dev
         _index(seqs, "seqs", dev)
         n = seqs.shape[0]
-        t = n if tokens is None else int(tokens)
+        if cu is not None and tokens is None:
+            raise ValueError("with cu, tokens says how many rows there are: cu[-1], which is on the device")
+        t = n if tokens is None else _count(tokens, "tokens")
         cu_ptr = self._cu(cu, n, t)  # cu itself stays referenced: what is allocated below must not take its memory
         dtype = dtype or torch.float32
         if dtype not in _dtype_codes:

@@ -495,3 +495,19 @@ def test_gradients_are_refused_not_dropped(M, dev):
         with torch.no_grad():
             f()
     assert int(cache.status) == 0
+
+
+def test_read_with_offsets_needs_the_row_count(M, dev):
+    """Rows by offsets and no count: the count of sequences stood in for it, and cut the rows short at other positions."""
+    cache = M.KvCache.create(1, 8, 1, 64, 2, 4, dev=dev)
+    cache.reserve(i32([0, 1]), i32([5, 70]))
+    x = torch.randn(75, 1, 64, device="cuda").half()
+    cache.append(0, x, x, i32([0, 1]), cu_of([5, 70]))
+    with pytest.raises(ValueError, match="tokens"):
+        cache.read(0, i32([0, 1]), cu_of([5, 70]))
+    with pytest.raises(ValueError, match="tokens"):
+        cache.read(0, i32([0, 1]), cu_of([5, 70]), tokens=-1)
+    k, _ = cache.read(0, i32([0, 1]), cu_of([5, 70]), tokens=75)
+    # half a step of the page's scale, max|x| / 254
+    assert float((k - x.float()).abs().max()) <= float(x.float().abs().max()) / 254 * 1.0001
+    assert cache.read(0, i32([0, 1]))[0].shape == (2, 1, 64)
