@@ -1318,8 +1318,8 @@ bool make_map(CUtensorMap* map, const mrl_attn& a, const void* p, int64_t row, i
     const cuuint64_t strides[2] = {(cuuint64_t)(in ? row : head) * 2, (cuuint64_t)(in ? head : row) * 2};
     const cuuint32_t box[3] = {64, (cuuint32_t)(in ? box_rows : box_heads), (cuuint32_t)(in ? box_heads : box_rows)}, one[3] = {1, 1, 1};
     *inner = in;
-    const Encode f = encoder();
-    return f && f(map, a.dtype == MRL_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p), dims, strides, box,
+    if (strides[0] >= 1ull << 40 || strides[1] >= 1ull << 40) return false;  // a map's limit
+    return encoder()(map, a.dtype == MRL_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p), dims, strides, box,
                   one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -1327,10 +1327,12 @@ bool make_map(CUtensorMap* map, const mrl_attn& a, const void* p, int64_t row, i
 template <class T, int D, bool PAGED> int launch(TcParams p, int sms, cudaStream_t s) {
     using S = Shape<D, PAGED>;
     CUtensorMap mq = {}, mk = {}, mv = {};
-    if (!PAGED && (!make_map(&mq, p.a, p.a.q, p.a.q_row, p.a.q_head, p.a.q_heads, D, p.group, 128 / p.group, &p.inner_q) ||
-                   !make_map(&mk, p.a, p.a.k, p.a.k_row, p.a.k_head, p.a.kv_heads, D, 1, kKeys, &p.inner_k) ||
-                   !make_map(&mv, p.a, p.a.v, p.a.v_row, p.a.v_head, p.a.kv_heads, D, 1, kKeys / S::v_parts, &p.inner_v)))
-        return -1;
+    if (!PAGED) {
+        if (!encoder()) return kTcNoMaps;
+        if (!make_map(&mq, p.a, p.a.q, p.a.q_row, p.a.q_head, p.a.q_heads, D, p.group, 128 / p.group, &p.inner_q)) return kTcBadQ;
+        if (!make_map(&mk, p.a, p.a.k, p.a.k_row, p.a.k_head, p.a.kv_heads, D, 1, kKeys, &p.inner_k)) return kTcBadK;
+        if (!make_map(&mv, p.a, p.a.v, p.a.v_row, p.a.v_head, p.a.kv_heads, D, 1, kKeys / S::v_parts, &p.inner_v)) return kTcBadV;
+    }
     p.tokens = 128 / p.group;
     if (const cudaError_t e = allow_smem<tc_kernel<T, D, PAGED>>((int)S::smem)) return (int)e;
     const mrl_attn a = p.a;

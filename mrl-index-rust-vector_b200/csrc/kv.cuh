@@ -152,7 +152,9 @@ constexpr uint32_t kKvDecodeSeqs = 1024;
 size_t kv_decode_bytes(uint32_t head_dim, int sms);
 int launch_kv_decode(const mrl_kv_cache& c, const mrl_attn& a, int sms, void* scratch, unsigned* counters, cudaStream_t s);
 // Tensor-core attention: over the cache (c; `wide` is kKvZeroBytes of zeros and room for a 16-bit image of one
-// layer's pool) or over the call's own k and v. -1: strides that a TMA map cannot describe.
+// layer's pool) or over the call's own k and v. Below 0: no tensor maps in this driver, or an operand
+// with strides that a map cannot describe.
+enum : int { kTcNoMaps = -1, kTcBadQ = -2, kTcBadK = -3, kTcBadV = -4 };
 constexpr size_t kKvZeroBytes = 64 * 256 * 2;
 size_t kv_wide_bytes(const mrl_kv_cache& c);
 int launch_attend_tc(const mrl_kv_cache* c, const mrl_attn& a, int sms, void* wide, cudaStream_t s);

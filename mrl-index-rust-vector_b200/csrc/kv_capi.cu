@@ -287,7 +287,9 @@ int mrl_window_attention(mrl_ctx* ctx, const mrl_attn* a) {
         if (int rc = check_attn(ctx, a, a->kv_heads, a->head_dim, false)) return rc;
         if (a->n_tokens == 0) return MRL_OK;
         const int rc = mrl::launch_attend_tc(nullptr, cut(*a), ctx->sms, nullptr, ctx->stream);
-        if (rc < 0) return bad(ctx, "k or v has strides that a tensor map cannot describe");
+        if (rc == mrl::kTcNoMaps) return fail(ctx, MRL_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
+        if (rc < 0)
+            return fail(ctx, MRL_ERR_INVALID, std::string(rc == mrl::kTcBadQ ? "q" : rc == mrl::kTcBadK ? "k" : "v") + " has strides that a tensor map cannot describe");
         return done(ctx, rc, "mrl_window_attention");
     });
 }

@@ -511,3 +511,62 @@ def test_read_with_offsets_needs_the_row_count(M, dev):
     # half a step of the page's scale, max|x| / 254
     assert float((k - x.float()).abs().max()) <= float(x.float().abs().max()) / 254 * 1.0001
     assert cache.read(0, i32([0, 1]))[0].shape == (2, 1, 64)
+
+
+@pytest.mark.parametrize("name", ["q", "k", "v"])
+def test_strides_beyond_a_tensor_map_name_their_operand(M, dev, name):
+    """A row stride of 2^40 bytes, the first that a map cannot hold: refused on the host, by name."""
+    from mrl_b200 import attention as A
+
+    x = torch.zeros(2, 2, 64, dtype=torch.float16, device="cuda")
+    out, cu = torch.zeros_like(x), i32([0, 2])
+    strides = {n: (1 << 39 if n == name else 128, 64) for n in "qkv"}
+    M.window_attention(x, x, x, cu, 2, dev=dev)
+    args = bytearray(A._ATTN.pack(x.data_ptr(), x.data_ptr(), x.data_ptr(), out.data_ptr(), 0, 0, cu.data_ptr(), 0, *strides["q"], *strides["k"],
+                                  *strides["v"], 128, 64, 1, 2, 2, 2, 2, 64, 0, 1, 0, 0, 0.125, 0))
+    import ctypes as C
+
+    with pytest.raises(M.MrlError, match=f"^.*\\b{name} has strides"):
+        A.check(dev.ptr, dev.lib.mrl_window_attention(dev.ptr, C.addressof((C.c_char * len(args)).from_buffer(args))))
+    assert not bool(out.any())
+
+
+@pytest.mark.parametrize("d", [64, 256])
+def test_broadcast_heads_and_rows(M, dev, d):
+    """Keys and values of one head shown as several, and values of one row as all: strides of 0, as in an append."""
+    rng = np.random.default_rng(d)
+    t = 200
+    q = torch.from_numpy(rng.normal(0, 1, (t, 4, d)).astype(np.float32)).half().cuda()
+    k1, v1 = (torch.from_numpy(rng.normal(0, 1, (t, 1, d)).astype(np.float32)).half().cuda() for _ in range(2))
+    k, v, row = k1.expand(t, 2, d), v1.expand(t, 2, d), v1[:1].expand(t, 1, d)
+    cu = i32([0, 90, t])
+    f = lambda *x: M.window_attention(*x, cu, 110, dev=dev)  # noqa: E731
+    assert torch.equal(f(q, k, v), f(q, k.contiguous(), v.contiguous()))
+    assert torch.equal(f(q, k1, row), f(q, k1, row.contiguous()))
+    q1 = q[:, :1].expand(t, 4, d)
+    assert torch.equal(f(q1, k, v), f(q1.contiguous(), k.contiguous(), v.contiguous()))
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("h,g", [(1, 4), (2, 3), (3, 1)])
+@pytest.mark.parametrize("turned", ["q", "k", "v", "qkv"])
+def test_window_heads_outermost(M, dev, d, h, g, turned):
+    """Inputs laid out by heads, [heads][rows][dims], each alone and all three: the same bits as laid out by rows."""
+    rng = np.random.default_rng(d + h)
+    lens = [5, 130, 64, 257]
+    t = sum(lens)
+    x = {n: torch.from_numpy(rng.normal(0, 1, (t, heads, d)).astype(np.float32)).bfloat16().cuda() for n, heads in (("q", h * g), ("k", h), ("v", h))}
+    for causal, window, sinks in ((True, 0, 0), (False, 0, 0), (True, 70, 3), (False, 40, 0)):
+        f = lambda y: M.window_attention(y["q"], y["k"], y["v"], cu_of(lens), max_len=max(lens), causal=causal, window=window, sinks=sinks,  # noqa: E731,B023
+                                         return_lse=True, dev=dev)
+        want, want_lse = f(x)
+        y = {n: z.transpose(0, 1).contiguous().transpose(0, 1) if n in turned else z for n, z in x.items()}
+        out, lse = f(y)
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    qn, kn, vn = (x[n].double().cpu().numpy() for n in "qkv")
+    at = 0
+    for n in lens:
+        want, wl, big = plain_attention(qn[at:at + n], kn[at:at + n], vn[at:at + n], 0, False, 40, 0, d ** -0.5)
+        check_rows(out[at:at + n].double().cpu().numpy(), lse[at:at + n].double().cpu().numpy(), want, wl, big, d, n, np.abs(vn[at:at + n]).max(),
+                   U[torch.bfloat16], U[torch.bfloat16])
+        at += n
