@@ -345,7 +345,8 @@ template <class T, int E> __device__ __forceinline__ int odd_values(const uint32
     return kind;
 }
 
-// The exact result of one row, from its visible keys alone. A warp, lane e holds dims e D/32 ..; four keys at a time.
+// The exact result of one row, from its visible keys alone. A warp, lane e holds dims e D/32 ..; four keys at a time. O is kept
+// divided by l, so that it is never larger than the values: also where the products' sums are too large for f32.
 template <class T, int D> __device__ __noinline__ void slow_row(const mrl_attn& a, int row0, int n, int p, int t_row, int h, int kvh, int causal) {
     constexpr int E = D / 32, kTurn = 4;
     const int lane = (int)threadIdx.x & 31;
@@ -386,25 +387,29 @@ template <class T, int D> __device__ __noinline__ void slow_row(const mrl_attn& 
                 s[u] *= a.scale;
                 if (j + u < to) top = s[u] > top || s[u] != s[u] ? s[u] : top;  // a NaN stays
             }
-            const float keep = m == -INFINITY ? 0.0f : expf(m - top);
+            const float keep = m == -INFINITY ? 0.0f : l * expf(m - top);
             m = top;
-            l *= keep;
+            l = keep;
 #pragma unroll
-            for (int e = 0; e < E; ++e) o[e] = keep == 0.0f ? 0.0f : o[e] * keep;
+            for (int u = 0; u < kTurn; ++u) {
+                s[u] = j + u >= to || (s[u] == -INFINITY && top == -INFINITY) ? 0.0f : expf(s[u] - top);
+                l += s[u];
+            }
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = keep == 0.0f ? 0.0f : o[e] * (keep * inv);
 #pragma unroll
             for (int u = 0; u < kTurn; ++u) {
                 if (j + u >= to) break;
-                const float add = s[u] == -INFINITY && top == -INFINITY ? 0.0f : expf(s[u] - top);
                 const T* v = reinterpret_cast<const T*>(vw[u]);
-                l += add;
 #pragma unroll
-                for (int e = 0; e < E; ++e) o[e] = fmaf(add, to_f32<T>(v[e]), o[e]);
+                for (int e = 0; e < E; ++e) o[e] = fmaf(s[u] * inv, to_f32<T>(v[e]), o[e]);
             }
         }
     }
     T* op = static_cast<T*>(a.out) + (int64_t)t_row * a.o_row + (int64_t)h * a.o_head + lane * E;
 #pragma unroll
-    for (int e = 0; e < E; ++e) op[e] = from_f32<T>(l == 0.0f ? 0.0f : o[e] / l);
+    for (int e = 0; e < E; ++e) op[e] = from_f32<T>(l == 0.0f ? 0.0f : o[e]);
     if (a.lse && lane == 0) a.lse[(size_t)t_row * a.q_heads + h] = l == 0.0f ? -INFINITY : m + logf(l);
 }
 

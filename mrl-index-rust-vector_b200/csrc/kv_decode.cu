@@ -29,6 +29,9 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLeastScale = 1e-37f;       // V scales are taken relative to this at least
+// Pieces of O are summed up before they are divided by l, which may be as large as the number of keys: they are held 2^-20
+// times their size, so that sums of a million values of bf16's largest stay finite.
+constexpr float kDown = 1.0f / 1048576.0f, kUp = 1048576.0f;
 constexpr float kNoGrowth = 1.000001f;      // a scale times the rounded reciprocal of itself
 constexpr long long kWaitClocks = 4000000000ll;  // a wait for a page gives up after about two seconds
 
@@ -613,8 +616,8 @@ template <class T, int D, bool WIDE> __global__ void __launch_bounds__(kWarps<D>
         l0 = quad_sum(l0);
         l1 = quad_sum(l1);
 
-        // ---- the team's warps joined: O in real units, then rescaled to the rows' common maximum
-        const float vref0 = 1.0f / per0, vref1 = 1.0f / per1;
+        // ---- the team's warps joined: O in one unit, then rescaled to the rows' common maximum
+        const float vref0 = kDown / per0, vref1 = kDown / per1;
         float* mine = acc_s + warp * 16 * kAccStride<D>;
 #pragma unroll
         for (int x = 0; x < D / 8; ++x) {
@@ -632,7 +635,7 @@ template <class T, int D, bool WIDE> __global__ void __launch_bounds__(kWarps<D>
         const int w0 = team * W;
         auto emit = [&](int r, int d, float4 x, float m, float l) {
             const int row = s.tile * 16 + r;
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            const float inv = l == 0.0f ? 0.0f : kUp / l;
             T* dst = static_cast<T*>(a.out) + (int64_t)(q.row + row / group) * a.o_row + (int64_t)(s.head * group + row % group) * a.o_head + d;
             T y[4] = {from_f32<T>(x.x * inv), from_f32<T>(x.y * inv), from_f32<T>(x.z * inv), from_f32<T>(x.w * inv)};
             *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(y);

@@ -570,3 +570,44 @@ def test_window_heads_outermost(M, dev, d, h, g, turned):
         check_rows(out[at:at + n].double().cpu().numpy(), lse[at:at + n].double().cpu().numpy(), want, wl, big, d, n, np.abs(vn[at:at + n]).max(),
                    U[torch.bfloat16], U[torch.bfloat16])
         at += n
+
+
+# ---- very large values --------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 20, 700])
+@pytest.mark.parametrize("n_seqs", [1, 90])
+def test_values_near_the_end_of_bf16_over_the_cache(M, dev, d, rows, n_seqs):
+    """Values of 1e38, all of one sign in half of the dims: weighted sums of hundreds of them are beyond f32, their means are
+    not."""
+    if n_seqs * rows > 2000:
+        rows = 20
+    rng = np.random.default_rng(d)
+    n = 700
+    cache = M.KvCache.create(1, 11 * n_seqs, 2, d, n_seqs, 11, dev=dev)
+    seqs = list(range(n_seqs))
+    cache.reserve(i32(seqs), i32([n] * n_seqs))
+    k = torch.from_numpy(rng.normal(0, 0.3, (n * n_seqs, 2, d)).astype(np.float32)).bfloat16().cuda()
+    v = torch.from_numpy(rng.normal(0, 0.5, (n * n_seqs, 2, d)))
+    v[:, :, ::2] = 1 + v[:, :, ::2].abs().clamp(max=1)
+    v = (v.clamp(-2, 2) * 1e38).bfloat16().cuda()
+    cache.append(0, k, v, i32(seqs), cu_of([n] * n_seqs))
+    q = torch.from_numpy(rng.normal(0, 0.5, (rows * n_seqs, 4, d)).astype(np.float32)).bfloat16().cuda()
+    out, lse = cache.attend(0, q, i32(seqs), cu_of([rows] * n_seqs), max_q=rows, return_lse=True)
+    codes, scales, tables = (x.cpu().numpy() for x in (cache.codes, cache.scales, cache.tables))
+    picked = seqs[:3]
+    check_known(codes[0], scales[0], tables, [n] * n_seqs, picked, [rows] * len(picked), q, out, lse)
+    assert float(out[:, :, ::2].min()) > 0.9e38
+
+
+def test_values_near_the_end_of_bf16_in_rows(M, dev):
+    rng = np.random.default_rng(12)
+    n, d = 300, 128
+    q, k = (torch.from_numpy(rng.normal(0, 0.5, (n, h, d)).astype(np.float32)).bfloat16().cuda() for h in (4, 2))
+    v = (torch.from_numpy(rng.uniform(1, 3, (n, 2, d))) * 1e38).bfloat16().cuda()
+    for causal, window in ((True, 0), (False, 0), (True, 100)):
+        out, lse = M.window_attention(q, k, v, i32([0, n]), n, causal=causal, window=window, return_lse=True, dev=dev)
+        qn, kn, vn = (x.double().cpu().numpy() for x in (q, k, v))
+        want, wl, big = plain_attention(qn, kn, vn, 0, causal, window, 0, d ** -0.5)
+        check_rows(out.double().cpu().numpy(), lse.double().cpu().numpy(), want, wl, big, d, n, np.abs(vn).max(), U[q.dtype], U[q.dtype])
