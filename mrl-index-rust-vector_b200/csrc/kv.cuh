@@ -130,7 +130,6 @@ template <auto kernel> cudaError_t allow_smem(int bytes) {
 }
 
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void grid_go() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 }  // namespace kv
 

@@ -1,5 +1,5 @@
 // kv_decode.cu — attention of a few query rows per sequence over the paged 8-bit cache
-// (mrl_kv_attend, include/mrl_kv.h), one launch.
+// (mrl_kv_attend, include/mrl_kv.h), one launch for every 1,024 sequences.
 //
 // An item is 16 query rows (tokens x the query heads of one kv head) of one sequence: their K and V pages
 // are read once and serve all 16. The page is the unit of work: one warp takes a page of 64 tokens,

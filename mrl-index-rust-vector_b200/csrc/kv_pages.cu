@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(256) release_kernel(mrl_kv_cache c, const int3
     if (window == 0 && lane == 0) c.lens[s] = 0;
 }
 
-Lists lists_at(const mrl_kv_cache& c, uint32_t n, void* scratch) {
+Lists lists_at(const mrl_kv_cache& c, void* scratch) {
     int* p = static_cast<int*>(scratch);
     Lists l;
     l.count = p;
@@ -369,7 +369,6 @@ Lists lists_at(const mrl_kv_cache& c, uint32_t n, void* scratch) {
     l.b = l.a + c.pages;
     l.map = l.b + c.pages;
     l.off = l.map + c.pages;
-    (void)n;
     return l;
 }
 
@@ -393,13 +392,13 @@ cudaError_t launch_after(void (*kernel)(P...), int grid, int threads, cudaStream
 size_t kv_list_bytes(const mrl_kv_cache& c, uint32_t n) { return sizeof(int) * (4 + 3 * (size_t)c.pages + n); }
 
 int launch_kv_reserve(const mrl_kv_cache& c, const int32_t* seqs, const int32_t* add, uint32_t n, void* scratch, cudaStream_t s) {
-    kv::reserve_kernel<<<1, kv::kPlanThreads, 0, s>>>(c, seqs, add, (int)n, kv::lists_at(c, n, scratch));
+    kv::reserve_kernel<<<1, kv::kPlanThreads, 0, s>>>(c, seqs, add, (int)n, kv::lists_at(c, scratch));
     return (int)cudaGetLastError();
 }
 
 int launch_kv_fork(const mrl_kv_cache& c, const int32_t* parents, const int32_t* children, uint32_t n, int sms, void* scratch,
                    cudaStream_t s) {
-    const kv::Lists l = kv::lists_at(c, n, scratch);
+    const kv::Lists l = kv::lists_at(c, scratch);
     kv::fork_plan_kernel<<<1, kv::kPlanThreads, 0, s>>>(c, parents, children, (int)n, l);
     if (const cudaError_t e = cudaGetLastError()) return (int)e;
     return (int)kv::launch_after(kv::fork_apply_kernel, sms * 4, kv::kCopyThreads, s, c, parents, children, (int)n, l);
@@ -412,7 +411,7 @@ int launch_kv_release(const mrl_kv_cache& c, const int32_t* seqs, uint32_t n, ui
 }
 
 int launch_kv_compact(const mrl_kv_cache& c, int sms, void* scratch, cudaStream_t s) {
-    const kv::Lists l = kv::lists_at(c, 0, scratch);
+    const kv::Lists l = kv::lists_at(c, scratch);
     kv::compact_plan_kernel<<<1, kv::kPlanThreads, 0, s>>>(c, l);
     if (const cudaError_t e = cudaGetLastError()) return (int)e;
     return (int)kv::launch_after(kv::compact_apply_kernel, sms * 4, kv::kCopyThreads, s, c, l);
