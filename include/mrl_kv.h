@@ -11,15 +11,18 @@
  * what only their contents can show is checked there: an index out of range is never followed, and the
  * page operations set a bit of *status and change nothing.
  *
- * Scratch. A context keeps scratch for every stream that these calls were made on, until it is
+ * Scratch. A context keeps scratch for each stream that these calls were made on, until it is
  * destroyed: about 20 MiB, more for pools of millions of pages, and for mrl_kv_attend of many rows
  * twice the size of one layer's codes. It grows on demand, and a call that makes it grow allocates
- * device memory and may wait for the device; the others do not synchronise. During a stream capture
+ * device memory and may wait for the device; so does the first call on a stream past 32, which takes
+ * over what another stream has not used for longest. The others do not synchronise. During a stream capture
  * nothing can grow: such a call is refused, so make a call of the same size on the stream before the
  * capture. A captured graph goes on using the scratch of the stream it was captured on, which stays
  * where it is whatever is called later: replay it on that stream, or where nothing else runs on that
  * stream's scratch (its calls and the other graphs captured on it) at the same time. Destroy the
  * context after the graphs, and a stream only when its work is done.
+ *
+ * Outputs may not overlap inputs.
  */
 #ifndef MRL_KV_H
 #define MRL_KV_H

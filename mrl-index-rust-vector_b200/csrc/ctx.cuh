@@ -18,6 +18,7 @@ struct mrl_kv_block {
 };
 struct mrl_kv_scratch {
     cudaStream_t stream = nullptr;
+    uint64_t last = 0;   // the context's call that used it last
     mrl_kv_block work;   // counters and working memory
     mrl_kv_block image;  // 16-bit image of a layer's pool
 };
@@ -77,7 +78,9 @@ struct mrl_ctx {
     bool slot_busy[MRL_MAX_INFLIGHT] = {};
     // paged cache and attention (kv_capi.cu): scratch per stream, blocks that were outgrown but are held by captured
     // graphs, and the event that orders a torch stream with the context's
+    static constexpr size_t kKvStreams = 32;  // that scratch is kept for beside those of captured graphs
     std::deque<mrl_kv_scratch> kv;
+    uint64_t kv_calls = 0;
     std::vector<void*> kv_kept;
     cudaEvent_t join_event = nullptr;
 };

@@ -58,24 +58,47 @@ int check_rows16(mrl_ctx* ctx, const char* name, const void* p, int64_t row, int
     return MRL_OK;
 }
 
-// The scratch of the context's current stream, made by the first call on it. It is never handed to another stream: a graph
-// captured on this one keeps using it.
-mrl_kv_scratch& kv_stream(mrl_ctx* ctx) {
-    for (mrl_kv_scratch& x : ctx->kv)
-        if (x.stream == ctx->stream) return x;
-    ctx->kv.emplace_back();
-    ctx->kv.back().stream = ctx->stream;
-    return ctx->kv.back();
+bool capturing(const mrl_ctx* ctx) {
+    cudaStreamCaptureStatus s = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(ctx->stream, &s) != cudaSuccess) (void)cudaGetLastError();  // the launch will say so
+    return s != cudaStreamCaptureStatusNone;
+}
+int no_growth(mrl_ctx* ctx) { return bad(ctx, "scratch cannot grow during a stream capture: make a call of this size on the stream before it"); }
+
+// The scratch of the context's current stream, made by the first call on it. Past kKvStreams streams the one unused for longest
+// is taken over, when the device has finished, so that streams that come and go do not add up; one that a captured graph
+// may use is never handed on.
+int kv_stream(mrl_ctx* ctx, mrl_kv_scratch** out) {
+    mrl_kv_scratch *k = nullptr, *oldest = nullptr;
+    size_t free_ones = 0;
+    for (mrl_kv_scratch& x : ctx->kv) {
+        if (x.stream == ctx->stream) k = &x;
+        if (x.work.captured || x.image.captured) continue;
+        ++free_ones;
+        if (!oldest || x.last < oldest->last) oldest = &x;
+    }
+    if (!k) {
+        if (capturing(ctx)) return no_growth(ctx);
+        if (free_ones < mrl_ctx::kKvStreams) {
+            ctx->kv.emplace_back();
+            k = &ctx->kv.back();
+        } else {
+            MRL_CUDA_TRY(ctx, cudaDeviceSynchronize());
+            k = oldest;
+        }
+        k->stream = ctx->stream;
+    }
+    k->last = ++ctx->kv_calls;
+    *out = k;
+    return MRL_OK;
 }
 
 // At least `bytes` in a block of the scratch, zero when they are made. A block whose address a captured graph may hold
 // is kept beside its successor; another one is freed, which waits for the device.
 int kv_grow(mrl_ctx* ctx, mrl_kv_block* b, size_t bytes) {
-    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(ctx->stream, &capture) != cudaSuccess) (void)cudaGetLastError();  // the launch will say so
-    const bool capturing = capture != cudaStreamCaptureStatusNone;
+    const bool capture = capturing(ctx);
     if (b->bytes < bytes) {
-        if (capturing) return bad(ctx, "scratch cannot grow during a stream capture: make a call of this size on the stream before it");
+        if (capture) return no_growth(ctx);
         if (b->captured) {
             ctx->kv_kept.push_back(b->p);
             *b = mrl_kv_block{};
@@ -83,7 +106,7 @@ int kv_grow(mrl_ctx* ctx, mrl_kv_block* b, size_t bytes) {
         if (int rc = ensure_buf(ctx, &b->p, &b->bytes, (bytes + (size_t)0xfffff) & ~(size_t)0xfffff)) return rc;
         MRL_CUDA_TRY(ctx, cudaMemsetAsync(b->p, 0, b->bytes, ctx->stream));
     }
-    b->captured = b->captured || capturing;
+    b->captured = b->captured || capture;
     return MRL_OK;
 }
 
@@ -91,19 +114,21 @@ int kv_grow(mrl_ctx* ctx, mrl_kv_block* b, size_t bytes) {
 // call there is room for every mrl_kv_attend of few rows.
 constexpr size_t kCounterBytes = 65536;
 int kv_scratch(mrl_ctx* ctx, size_t bytes, void** out, unsigned** counters = nullptr) {
-    mrl_kv_scratch& k = kv_stream(ctx);
+    mrl_kv_scratch* k;
+    if (int rc = kv_stream(ctx, &k)) return rc;
     for (const uint32_t d : {64u, 128u, 256u}) bytes = std::max(bytes, mrl::kv_decode_bytes(d, ctx->sms));
-    if (int rc = kv_grow(ctx, &k.work, bytes + kCounterBytes)) return rc;
-    *out = static_cast<char*>(k.work.p) + kCounterBytes;
-    if (counters) *counters = static_cast<unsigned*>(k.work.p);
+    if (int rc = kv_grow(ctx, &k->work, bytes + kCounterBytes)) return rc;
+    *out = static_cast<char*>(k->work.p) + kCounterBytes;
+    if (counters) *counters = static_cast<unsigned*>(k->work.p);
     return MRL_OK;
 }
 
 // Room for a layer's pool as f16 (launch_attend_tc).
 int kv_image(mrl_ctx* ctx, size_t bytes, void** out) {
-    mrl_kv_scratch& k = kv_stream(ctx);
-    if (int rc = kv_grow(ctx, &k.image, bytes)) return rc;
-    *out = k.image.p;
+    mrl_kv_scratch* k;
+    if (int rc = kv_stream(ctx, &k)) return rc;
+    if (int rc = kv_grow(ctx, &k->image, bytes)) return rc;
+    *out = k->image.p;
     return MRL_OK;
 }
 

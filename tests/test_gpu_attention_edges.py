@@ -611,3 +611,54 @@ def test_values_near_the_end_of_bf16_in_rows(M, dev):
         qn, kn, vn = (x.double().cpu().numpy() for x in (q, k, v))
         want, wl, big = plain_attention(qn, kn, vn, 0, causal, window, 0, d ** -0.5)
         check_rows(out.double().cpu().numpy(), lse.double().cpu().numpy(), want, wl, big, d, n, np.abs(vn).max(), U[q.dtype], U[q.dtype])
+
+
+def test_more_streams_than_scratch_is_kept_for(M):
+    """64 streams of one context, twice: some take another's scratch over, a captured graph's never; results and graph stay
+    right."""
+    own = M.Device(0)
+    rng = np.random.default_rng(13)
+    _, one = reader(M, own, rng, 8, 3000, 2, 128, 1)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        own.use_torch_stream()
+        want = one()
+    torch.cuda.synchronize()
+    out = torch.zeros_like(want)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        one(out)
+    streams = [torch.cuda.Stream(priority=-(i % 2)) for i in range(64)]
+    assert len({t.cuda_stream for t in streams}) > 40
+    free = []
+    for _ in range(2):
+        for t in streams:
+            with torch.cuda.stream(t):
+                own.use_torch_stream()
+                assert torch.equal(one(), want)
+        torch.cuda.synchronize()
+        free.append(torch.cuda.mem_get_info()[0])
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    assert free[0] - free[1] < 64 << 20
+    del g
+    own.close()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows", [4, 600])
+def test_a_nan_query_is_its_own_rows_matter(M, dev, dtype, rows):
+    """Over the cache: a NaN in one head of one row makes that head's row NaN and changes no other bit."""
+    rng = np.random.default_rng(14)
+    cache, *_ = filled_cache(M, rng, dev, [700, 650], 2, 128)
+    q = torch.from_numpy(rng.normal(0, 1, (2 * rows, 8, 128)).astype(np.float32)).to(dtype).cuda()
+    f = lambda: cache.attend(0, q, i32([0, 1]), cu_of([rows, rows]), max_q=rows, return_lse=True)  # noqa: E731
+    clean, clean_lse = f()
+    q[rows + 1, 5, 17] = float("nan")
+    out, lse = f()
+    assert bool(torch.isnan(out[rows + 1, 5]).all()) and bool(torch.isnan(lse[rows + 1, 5]))
+    out[rows + 1, 5], lse[rows + 1, 5] = clean[rows + 1, 5], clean_lse[rows + 1, 5]
+    assert torch.equal(out, clean) and torch.equal(lse, clean_lse)
