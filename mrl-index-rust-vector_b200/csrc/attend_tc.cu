@@ -22,9 +22,9 @@
 // Bounds: per 128 keys a tile pair needs 2 x 2 x 128 x 128 x D products (2,048 clocks at head_dim 128) and 2 x 16,384
 // exponentials and as many conversions (about 2,560). What a pair takes is the chain of one tile's step, about 3,500
 // clocks, the other tile in the gaps: S into registers 200, maximum 250, P 1,270, hand-over 100, P V and the next S
-// 1,100, waits. Measured on two B200s, full attention over 2 x 8,192 tokens: 16 heads of 128 in bf16 900 and 925 us, 1,222
-// and 1,189 TFLOP/s (tensor pipe 54% active); 16 heads of 64 in f16 771 and 821 us; 8 heads of 256 in bf16 1,174 and 1,182 us;
-// causal with a window of 1,024 and 4 sinks, 16 query heads on 4, 203 us. The rows of two tiles rather than one per CTA halve
+// 1,100, waits. Measured on one B200, full attention over 2 x 8,192 tokens of unit normal values: 16 heads of 128 in bf16 937
+// us, 1,173 TFLOP/s (tensor pipe 54% active); 16 heads of 64 in f16 822 us; 8 heads of 256 in bf16 1,200 us;
+// causal with a window of 1,024 and 4 sinks, 16 query heads on 4, 202 us. The rows of two tiles rather than one per CTA halve
 // the traffic of K and V from L2 (64 KB per step); 128 keys a step is what tensor memory holds beside two O.
 // The instructions' operands have to be in uniform registers: issued from one divergent lane, each product cost
 // 75 clocks and the same kernel ran at 972 instead of 1,097 TFLOP/s.

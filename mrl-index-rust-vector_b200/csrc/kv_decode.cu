@@ -15,9 +15,9 @@
 // order in the score tile is chosen so that a lane's scores are 16 consecutive tokens, V's row order.
 //
 // Bound by HBM for long contexts (2 x 64 x head_dim bytes a page), by latency for short ones. Measured on one B200, 8 kv
-// heads of 128, four query heads each: 4 sequences of 130,000 tokens 173 us (6.16 TB/s), 148 of 2,304 114 us (6.13), 48
-// of 2,304 52 us (4.34), 8 of 1,000 11.8 us, one of 37 8.8 us; 64 of 2,000, 4 kv heads of 256, 78 us (3.37); 128 of 8,000
-// through a window of 1,024, 8 kv heads of 64, 39 us (3.46). 15 to 18 us of the mid-sized ones are not the stream: 4 until
+// heads of 128, four query heads each: 4 sequences of 130,000 tokens 175 us (6.10 TB/s), 148 of 2,304 117 us (5.96), 48
+// of 2,304 53 us (4.29), 8 of 1,000 12.4 us, one of 37 9.5 us; 64 of 2,000, 4 kv heads of 256, 82 us (3.18); 128 of 8,000
+// through a window of 1,024, 8 kv heads of 64, 38 us (3.53). 15 to 18 us of the mid-sized ones are not the stream: 4 until
 // the work is dealt out, 3.5 until the first page is there, the rest joining the pieces of split items and uneven ends.
 #include <algorithm>
 
